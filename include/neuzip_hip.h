@@ -424,6 +424,76 @@ int nz_manager_erase(nz_manager* m, const char* name);
    check saw a container that failed validation. */
 int nz_manager_check(nz_manager* m, void* stream);
 
+/* ---- microscaled 4-bit weights, embedding tables ------------------------
+ *
+ * No counterpart in the reference.  These calls hold no state and allocate
+ * nothing: every buffer is the caller's, all work goes to `stream`, and all of
+ * them can be captured into a graph.  dtype is NZ_DTYPE_BF16, _F16 or _F32;
+ * dense pointers need the alignment of their elements only (rows that start
+ * 16-byte aligned are read with wide loads).
+ *
+ * The format.  A row is cut into blocks of 32 values that share a power of two
+ * X = 2^(s - 127).  s = max(E + 127 - e, 0) with E the exponent of the block's
+ * largest magnitude (floor of its base-2 logarithm); a value v is held as v / X
+ * rounded to an e2m1 number (bits = 4, e = 2, magnitudes 0 .5 1 1.5 2 3 4 6) or
+ * to an e4m3 number (bits = 8, e = 8, up to 448): to the nearest, ties to the
+ * even code, larger ones to the largest.  A block with a NaN or an infinity has
+ * s = 255 and reads as NaN throughout.
+ * Data: rows of nz_mx_row_bytes(cols, bits), values in order, the first of a
+ * pair of 4-bit codes in the low half; filled up to 128 values with zeros.
+ * Scales: rows of nz_mx_scale_bytes(cols), one byte s per block in groups of
+ * 16 blocks, block b of a group at byte 4 * (b % 4) + b / 4, the order the
+ * matrix instructions take them in (four bytes of a lane are its blocks of four
+ * successive steps of 128); filled up with zeros.
+ * Data and scales are 16-byte aligned. */
+uint64_t nz_mx_row_bytes(uint64_t cols, int bits);
+uint64_t nz_mx_scale_bytes(uint64_t cols);
+
+/* rows x cols values at dev_x, `stride` elements from row to row. */
+int nz_mx_quantize(const void* dev_x, int dtype, uint64_t rows, uint64_t cols, uint64_t stride, int bits,
+                   void* dev_data, void* dev_scales, void* stream);
+
+/* The values back, rows contiguous, rounded to dtype. */
+int nz_mx_dequantize(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int bits,
+                     void* dev_out, int dtype, void* stream);
+
+/* Rows dev_indices[0..count) (int64) of a table, times `scale`, rounded once.  An index outside the table
+   gives a row of zeros and, when dev_status is not NULL, sets bit 0 of that uint32. */
+int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int bits,
+                 const void* dev_indices, uint64_t count, float scale, void* dev_out, int dtype, void* dev_status,
+                 void* stream);
+
+/* y[m][n] = sum_k x[m][k] w[n][k] + bias[n]: w holds n rows of k values in 4 bits, the m rows of x are brought to 8
+   bits on the way.  Sums in 32 bits, one rounding to dtype.  bias may be NULL; it, x and y have the same dtype.
+   The workspace (nz_mx_linear_workspace_bytes(m, n, k), 16-byte aligned, may be 0) is free again when the call's
+   work has ended. */
+uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k);
+int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t stride, const void* dev_w_data,
+                 const void* dev_w_scales, uint64_t n, const void* dev_bias, void* dev_y, void* dev_workspace,
+                 uint64_t workspace_bytes, void* stream);
+
+/* The same for rows that are held in 8 bits already (rows that several weights share). */
+int nz_mx_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_t m, uint64_t k,
+                       const void* dev_w_data, const void* dev_w_scales, uint64_t n, const void* dev_bias, void* dev_y,
+                       int dtype, void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
+/* dx[m][k] = sum_n g[m][n] w[n][k], g with `stride` elements from row to row: the gradient of that product's rows
+   (their rounding to 8 bits is passed straight through). */
+int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
+                      const void* dev_w_scales, uint64_t k, void* dev_dx, void* stream);
+
+/* The gradient of an embedding table of rows x cols that was looked up at dev_indices[0..count) (int64):
+   out[v] = scale * sum of g[t] over the t with index v, in the order of t, in 32 bits, rounded once (the same
+   result every time).  g has `stride` elements from row to row, out is contiguous.  The row padding_idx (-1: none)
+   and indices outside the table take no part.  NZ_GRAD_BY_FREQUENCY divides each row by the number of its t;
+   NZ_GRAD_ACCUMULATE adds to out (rounded once) instead of setting it, rows without a t are then left as they are. */
+#define NZ_GRAD_BY_FREQUENCY 1u
+#define NZ_GRAD_ACCUMULATE 2u
+uint64_t nz_embedding_gradient_workspace_bytes(uint64_t count, uint64_t rows, uint64_t cols);
+int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* dev_g, int dtype, uint64_t stride,
+                          uint64_t rows, uint64_t cols, float scale, int64_t padding_idx, uint32_t flags,
+                          void* dev_out, void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

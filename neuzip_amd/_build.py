@@ -1,9 +1,10 @@
 """Compile libneuzip_hip.so for gfx950 with hipcc (cross-compiles without a GPU).
 
-Nine translation units: nz_launch.hip twice per precision (the encode kernels
-and the decode kernels of one kept-mantissa setting) and nz_api.hip (the C ABI
-and the kernels all precisions share); they compile side by side and are linked
-into one library.
+Nine translation units of the codec: nz_launch.hip twice per precision (the
+encode kernels and the decode kernels of one kept-mantissa setting) and
+nz_api.hip (the C ABI and the kernels all precisions share); two more hold the
+operators on microscaled weights (nz_mx.hip) and on embedding gradients
+(nz_embedding.hip).  They compile side by side and are linked into one library.
 """
 from __future__ import annotations
 
@@ -38,7 +39,7 @@ HIPCC_FLAGS = [
 
 
 def units(objdir: str):
-    """(source, extra flags, object file) of every translation unit."""
+    """(source, extra flags, object file) of every translation unit of the codec."""
     out = [(os.path.join(CSRC, "nz_api.hip"), [], os.path.join(objdir, "nz_api.o"))]
     # the lossless precision first: its halves take longest, the pool starts them first
     for s in PRECISIONS:
@@ -46,6 +47,12 @@ def units(objdir: str):
             out.append((os.path.join(CSRC, "nz_launch.hip"), [f"-DNZ_S={s}", f"-DNZ_PART={part}"],
                         os.path.join(objdir, f"nz_launch_s{s}_{tag}.o")))
     return out
+
+
+def operator_units(objdir: str):
+    """The same of the translation units beside the codec."""
+    return [(os.path.join(CSRC, f"{stem}.hip"), [], os.path.join(objdir, f"{stem}.o"))
+            for stem in ("nz_mx", "nz_embedding")]
 
 
 def run(cmd, verbose: bool) -> None:
@@ -67,7 +74,7 @@ def run(cmd, verbose: bool) -> None:
 def build(verbose: bool = False) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     with tempfile.TemporaryDirectory(prefix="nz_build_") as objdir:
-        tus = units(objdir)
+        tus = units(objdir) + operator_units(objdir)
 
         def compile_one(tu):
             src, extra, obj = tu

@@ -22,6 +22,7 @@ DEFAULT_CHUNK = 131072
 DEFAULT_LANE_SYMS = 256
 DEFAULT_SIZE_BUDGET = 1.01
 LANE_SYMS_AUTO = 0xFFFFFFFF
+GRAD_BY_FREQUENCY, GRAD_ACCUMULATE = 1, 2  # nz_embedding_gradient flags
 DECODE_CHECK, DECODE_STREAM_OUT, DECODE_RESIDENT_OUT = 1, 2, 4  # nz_decode flags
 
 EXPORTS = [
@@ -32,6 +33,9 @@ EXPORTS = [
     "nz_manager_meta", "nz_manager_geometry", "nz_manager_size", "nz_manager_size_reference", "nz_manager_exp_bytes", "nz_manager_packed_bytes",
     "nz_manager_norm_bytes", "nz_manager_buffers", "nz_manager_erase", "nz_manager_check",
     "nz_manager_export", "nz_manager_import", "nz_manager_trim", "nz_manager_rewrite_stats", "nz_set_lookback_spins", "nz_manager_geometry_hint",
+    "nz_mx_row_bytes", "nz_mx_scale_bytes", "nz_mx_quantize", "nz_mx_dequantize", "nz_mx_lookup",
+    "nz_mx_linear_workspace_bytes", "nz_mx_linear", "nz_mx_linear_rows8", "nz_mx_linear_grad",
+    "nz_embedding_gradient_workspace_bytes", "nz_embedding_gradient",
 ]
 
 _lib = None
@@ -131,6 +135,29 @@ def load() -> ctypes.CDLL:
     L.nz_manager_erase.argtypes = [vp, ctypes.c_char_p]
     L.nz_manager_check.restype = i32
     L.nz_manager_check.argtypes = [vp, vp]
+    L.nz_mx_row_bytes.restype = u64
+    L.nz_mx_row_bytes.argtypes = [u64, i32]
+    L.nz_mx_scale_bytes.restype = u64
+    L.nz_mx_scale_bytes.argtypes = [u64]
+    L.nz_mx_quantize.restype = i32
+    L.nz_mx_quantize.argtypes = [vp, i32, u64, u64, u64, i32, vp, vp, vp]
+    L.nz_mx_dequantize.restype = i32
+    L.nz_mx_dequantize.argtypes = [vp, vp, u64, u64, i32, vp, i32, vp]
+    L.nz_mx_lookup.restype = i32
+    L.nz_mx_lookup.argtypes = [vp, vp, u64, u64, i32, vp, u64, ctypes.c_float, vp, i32, vp, vp]
+    L.nz_mx_linear_workspace_bytes.restype = u64
+    L.nz_mx_linear_workspace_bytes.argtypes = [u64, u64, u64]
+    L.nz_mx_linear.restype = i32
+    L.nz_mx_linear.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp, vp, u64, vp]
+    L.nz_mx_linear_rows8.restype = i32
+    L.nz_mx_linear_rows8.argtypes = [vp, vp, u64, u64, vp, vp, u64, vp, vp, i32, vp, u64, vp]
+    L.nz_mx_linear_grad.restype = i32
+    L.nz_mx_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp]
+    L.nz_embedding_gradient_workspace_bytes.restype = u64
+    L.nz_embedding_gradient_workspace_bytes.argtypes = [u64, u64, u64]
+    L.nz_embedding_gradient.restype = i32
+    L.nz_embedding_gradient.argtypes = [vp, u64, vp, i32, u64, u64, u64, ctypes.c_float, ctypes.c_int64, u32, vp, vp,
+                                        u64, vp]
     _lib = L
     return L
 

@@ -14,6 +14,7 @@
 
 #include "../../include/neuzip_hip.h"
 #include "nz_launch.h"
+#include "nz_operators.h"
 
 #define NZ_MAX_DEVICES 64
 
@@ -37,6 +38,12 @@ int fail(int code, const std::string& msg) {
   g_err = msg;
   return code;
 }
+
+}  // namespace
+
+int nz_fail(int code, const char* msg) { return fail(code, msg); }
+
+namespace {
 
 #define NZ_HIP(call)                                                                  \
   do {                                                                                \

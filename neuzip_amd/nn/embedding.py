@@ -3,19 +3,28 @@
 Counterpart of neuzip/nn/embedding.py:13-39.  The reference decompresses the
 whole table on every forward; here only the chunks that hold the looked-up
 rows are decoded (``Manager.gather_rows``), which is what a one-token decode
-step needs.  Like the reference's, the table is frozen: the lookup carries no
-gradient to it.
+step needs.  Like the reference's, the table is frozen unless asked otherwise:
+the lookup carries no gradient to it.  With ``trainable=True`` it does: the
+table's gradient goes to the parameter's ``_gradient`` slot like a compressed
+Linear's, for ``neuzip_amd.compressed_lomo_hook``.  ``scale`` multiplies the rows.
 """
 from __future__ import annotations
 
 import torch
 
 from neuzip_amd.nn.module import Parameter
+from neuzip_amd.ops.embedding import CompressedEmbedding
 
 
 class Embedding(torch.nn.Module):
-    def __init__(self, manager, embedding: torch.nn.Embedding) -> None:
+    def __init__(self, manager, embedding: torch.nn.Embedding, scale: float = 1.0, trainable: bool = False) -> None:
         super().__init__()
+        if trainable and embedding.max_norm is not None:
+            raise ValueError("max_norm changes the table at every lookup: such a table cannot be trained here")
+        if trainable and embedding.sparse:
+            raise ValueError("the gradient of a compressed table is dense: sparse=True cannot be honoured")
+        self.scale = float(scale)
+        self.trainable = bool(trainable)
         self.manager = manager
         self.num_embeddings = embedding.num_embeddings
         self.embedding_dim = embedding.embedding_dim
@@ -48,9 +57,20 @@ class Embedding(torch.nn.Module):
         # the leading "!" marks a converted layer in the printed module tree
         return (f"! num_embeddings={self.num_embeddings}, embedding_dim={self.embedding_dim}, "
                 f"padding_idx={self.padding_idx}, max_norm={self.max_norm}, norm_type={self.norm_type}, "
-                f"scale_grad_by_freq={self.scale_grad_by_freq}, sparse={self.sparse}")
+                f"scale_grad_by_freq={self.scale_grad_by_freq}, sparse={self.sparse}"
+                + (f", scale={self.scale}" if self.scale != 1.0 else "") + (", trainable" if self.trainable else ""))
 
     def forward(self, x):
+        if self.trainable and torch.is_grad_enabled():
+            return CompressedEmbedding.apply(x, self._p, self)
+        return self._rows(x)
+
+    def _rows(self, x):
+        rows = self._lookup(x)
+        # the table's values are bf16 numbers: this product (in 32 bits) is the only rounding; the rows are the call's own
+        return rows if self.scale == 1.0 else rows.mul_(self.scale)
+
+    def _lookup(self, x):
         gather = getattr(self.manager, "gather_rows", None)
         if gather is None or not x.is_cuda:
             table = self._p()

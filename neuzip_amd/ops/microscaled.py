@@ -1,0 +1,244 @@
+"""Weights in microscaled 4 bits, and the products with them.
+
+Beside the entropy-coded weights of a :class:`~neuzip_amd.Manager` (any number
+of kept mantissa bits, decoded before or inside a product) stand weights in the
+form that the matrix cores multiply as it is: blocks of 32 values along a row
+share a power of two, a value is an e2m1 number times that (4.25 bits per
+value).  Activation rows are brought to 8 bits (e4m3, blocks of 32 likewise) on
+the way into a product; sums are held in 32 bits and rounded once.
+include/neuzip_hip.h states the format to the bit.
+
+The kernels are part of libneuzip_hip.so; there is no fallback without a GPU.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from neuzip_amd import _lib
+
+_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+
+
+def _dtype_code(dtype: torch.dtype) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise RuntimeError("Unsupported data type")
+    return code
+
+
+def _on_gpu(**tensors) -> torch.device:
+    """The device that all of ``tensors`` (None aside) are on, which has to be a GPU."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be on the GPU")
+        if device is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device} like the tensors before it")
+        device = t.device
+    return device
+
+
+def _call(fn, device: torch.device, *args) -> None:
+    """Make a native call on the current stream of ``device``."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:  # a launch goes to the device that is current
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.raise_for(rc)
+
+
+def _as_rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it)."""
+    rows = t.reshape(-1, width) if width else t.reshape(math.prod(t.shape[:-1]), 0)
+    if rows.stride(1) != 1 and width > 1 or rows.stride(0) < 0:
+        rows = rows.contiguous()
+    return rows
+
+
+class MXTensor:
+    """A matrix (or a stack of rows) held in microscaled 4 or 8 bits.
+
+    ``data`` and ``scales`` are the uint8 tensors of the stored form
+    (include/neuzip_hip.h), one row per row of the matrix; ``shape`` is the
+    shape of the values.  Made by :func:`mx_quantize`, or from stored tensors.
+    """
+
+    __slots__ = ("data", "scales", "bits", "shape")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, shape, bits: int = 4) -> None:
+        shape = torch.Size(shape)
+        if bits not in (4, 8):
+            raise ValueError("bits must be 4 or 8")
+        if len(shape) < 1:
+            raise ValueError("a microscaled tensor has one dimension at least")
+        L, rows = _lib.load(), math.prod(shape[:-1])
+        want = ((rows, L.nz_mx_row_bytes(shape[-1], bits)), (rows, L.nz_mx_scale_bytes(shape[-1])))
+        for name, t, size in (("data", data, want[0]), ("scales", scales, want[1])):
+            if t.dtype != torch.uint8 or tuple(t.shape) != size or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {size}")
+        if data.device != scales.device:
+            raise ValueError("data and scales must be on one device")
+        self.data, self.scales, self.shape, self.bits = data, scales, shape, bits
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        """bytes held"""
+        return self.data.numel() + self.scales.numel()
+
+    def to(self, device) -> "MXTensor":
+        return MXTensor(self.data.to(device), self.scales.to(device), self.shape, self.bits)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values as a dense tensor (bfloat16 holds all of them without rounding, subnormals aside)."""
+        code = _dtype_code(dtype)
+        device = _on_gpu(data=self.data)
+        out = torch.empty(self.shape, dtype=dtype, device=device)
+        _call(_lib.load().nz_mx_dequantize, device, self.data.data_ptr(), self.scales.data_ptr(), self.data.shape[0],
+              self.shape[-1], self.bits, out.data_ptr(), code)
+        return out
+
+    def __repr__(self) -> str:
+        return f"MXTensor(shape={tuple(self.shape)}, bits={self.bits}, device={self.device})"
+
+
+def mx_quantize(x: torch.Tensor, bits: int = 4) -> MXTensor:
+    """``x`` (bfloat16, float16 or float32, on the GPU) in microscaled form:
+    blocks of 32 values along the last axis share a power of two, values are
+    rounded to the nearest e2m1 (``bits=4``) or e4m3 (``bits=8``) number, ties to
+    the even code.  A block that holds a NaN or an infinity reads as NaN."""
+    if bits not in (4, 8):
+        raise ValueError("bits must be 4 or 8")
+    code = _dtype_code(x.dtype)
+    device = _on_gpu(x=x)
+    if x.dim() < 1:
+        raise ValueError("x must have one dimension at least")
+    L, cols = _lib.load(), x.shape[-1]
+    rows = _as_rows(x.detach(), cols)
+    n = rows.shape[0]
+    data = torch.empty((n, L.nz_mx_row_bytes(cols, bits)), dtype=torch.uint8, device=device)
+    scales = torch.empty((n, L.nz_mx_scale_bytes(cols)), dtype=torch.uint8, device=device)
+    _call(L.nz_mx_quantize, device, rows.data_ptr(), code, n, cols, rows.stride(0), bits, data.data_ptr(),
+          scales.data_ptr())
+    return MXTensor(data, scales, x.shape, bits)
+
+
+def _check_weight(weight) -> None:
+    if not isinstance(weight, MXTensor) or weight.bits != 4 or len(weight.shape) != 2:
+        raise ValueError("weight must be a matrix in microscaled 4 bits (mx_quantize)")
+
+
+def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
+    L = _lib.load()
+    n, k = weight.shape
+    shape = x.shape[:-1]
+    m = math.prod(shape)
+    code = _dtype_code(dtype)
+    if isinstance(x, MXTensor):
+        device = _on_gpu(x=x.data, weight=weight.data, bias=bias)
+    else:
+        device = _on_gpu(x=x, weight=weight.data, bias=bias)
+    y = torch.empty(*shape, n, dtype=dtype, device=device)
+    if k == 0:  # empty sums
+        return y.copy_(bias) if bias is not None else y.zero_()
+    if bias is not None:
+        bias = bias.contiguous()
+    b = None if bias is None else bias.data_ptr()
+    if isinstance(x, MXTensor):
+        _call(L.nz_mx_linear_rows8, device, x.data.data_ptr(), x.scales.data_ptr(), m, k, weight.data.data_ptr(),
+              weight.scales.data_ptr(), n, b, y.data_ptr(), code, None, 0)
+        return y
+    rows = _as_rows(x, k)
+    room = L.nz_mx_linear_workspace_bytes(m, n, k)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    _call(L.nz_mx_linear, device, rows.data_ptr(), code, m, k, rows.stride(0), weight.data.data_ptr(),
+          weight.scales.data_ptr(), n, b, y.data_ptr(), None if ws is None else ws.data_ptr(), room)
+    return y
+
+
+class MicroscaledLinear(torch.autograd.Function):
+    """``y = x W^T (+ b)`` with a frozen weight in 4 bits.  Backward gives the
+    gradients of ``x`` (the rounding of its rows to 8 bits is passed straight
+    through) and of the bias."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, dtype):
+        ctx.weight = weight
+        return _product(x, weight, bias, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        n, k = ctx.weight.shape
+        grad_x = grad_b = None
+        if ctx.needs_input_grad[0]:
+            device = grad_output.device
+            go = _as_rows(grad_output, n)
+            grad_x = torch.empty(*grad_output.shape[:-1], k, dtype=grad_output.dtype, device=device)
+            _call(_lib.load().nz_mx_linear_grad, device, go.data_ptr(), _dtype_code(go.dtype), go.shape[0], n,
+                  go.stride(0), ctx.weight.data.data_ptr(), ctx.weight.scales.data_ptr(), k, grad_x.data_ptr())
+        if ctx.needs_input_grad[2]:
+            grad_b = grad_output.reshape(-1, n).sum(0)
+        return grad_x, None, grad_b, None
+
+
+def mx_linear(x, weight: MXTensor, bias=None, dtype=None) -> torch.Tensor:
+    """``x @ W^T (+ bias)`` for a weight ``[out, in]`` in microscaled 4 bits.
+
+    ``x`` is a tensor ``[..., in]`` (bfloat16, float16 or float32), whose rows are
+    brought to 8 bits on the way and whose type the result has; or an
+    :class:`MXTensor` of 8 bits (rows that several weights share), with a result
+    of type ``dtype`` (bfloat16).  ``bias`` has the type of the result.  Autograd
+    records the gradients of ``x`` and ``bias``; the weight is frozen."""
+    _check_weight(weight)
+    n, k = weight.shape
+    if isinstance(x, MXTensor):
+        if x.bits != 8:
+            raise ValueError("activation rows are held in 8 bits (mx_quantize(x, 8))")
+        dtype = torch.bfloat16 if dtype is None else dtype
+    else:
+        if x.dim() < 1:
+            raise ValueError("x must have one dimension at least")
+        if dtype is not None and dtype != x.dtype:
+            raise ValueError("the result has the type of x")
+        dtype = x.dtype
+    _dtype_code(dtype)
+    if x.shape[-1] != k:
+        raise ValueError(f"x has {x.shape[-1]} columns, the weight {k}")
+    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype != dtype):
+        raise ValueError(f"bias must be a {dtype} tensor of {n} elements")
+    if torch.is_grad_enabled() and (not isinstance(x, MXTensor) and x.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        return MicroscaledLinear.apply(x, weight, bias, dtype)
+    return _product(x, weight, bias, dtype)
+
+
+def mx_embedding(indices: torch.Tensor, table: MXTensor, scale: float = 1.0, dtype: torch.dtype = torch.bfloat16,
+                 status=None) -> torch.Tensor:
+    """Rows ``indices`` (any integer shape) of a table in microscaled form, times
+    ``scale``, rounded once to ``dtype``.  An index outside the table gives a row
+    of zeros and sets bit 0 of ``status`` (an int32 tensor of one element)."""
+    if not isinstance(table, MXTensor) or len(table.shape) != 2:
+        raise ValueError("table must be a matrix in microscaled form (mx_quantize)")
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise ValueError("indices must be int64 or int32")
+    code = _dtype_code(dtype)
+    device = _on_gpu(table=table.data, indices=indices, status=status)
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError("status must be an int32 tensor of one element")
+    idx = indices.reshape(-1).to(torch.int64).contiguous()
+    rows, cols = table.shape
+    out = torch.empty(*indices.shape, cols, dtype=dtype, device=device)
+    _call(_lib.load().nz_mx_lookup, device, table.data.data_ptr(), table.scales.data_ptr(), rows, cols, table.bits,
+          idx.data_ptr(), idx.numel(), float(scale), out.data_ptr(), code,
+          None if status is None else status.data_ptr())
+    return out

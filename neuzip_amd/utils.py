@@ -79,3 +79,22 @@ def _convert(manager, module: torch.nn.Module, prefix: str = "") -> torch.nn.Mod
             else:
                 pending.append((child, dotted))
     return module
+
+
+def mx_convert(module: torch.nn.Module, prefix: str = "") -> torch.nn.Module:
+    """In place: the ``nn.Linear`` layers that ``Manager.convert`` would compress
+    (those whose attribute name contains ``lm_head`` are left alone) are held in
+    microscaled 4 bits instead, with their weights frozen."""
+    from neuzip_amd.nn import MXLinear
+
+    for name, child in list(module.named_children()):
+        dotted = f"{prefix}.{name}" if prefix else name
+        if "lm_head" in name:
+            continue
+        if isinstance(child, torch.nn.Linear):
+            logger.debug("Converting %s: %s", dotted, child)
+            setattr(module, name, MXLinear(child))
+            _delete_module(child)
+        else:
+            mx_convert(child, dotted)
+    return module
