@@ -465,9 +465,10 @@ int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, ui
 
 /* y[m][n] = sum_k x[m][k] w[n][k] + bias[n]: w holds n rows of k values in 4 bits, the m rows of x are brought to 8
    bits on the way.  Sums in 32 bits, one rounding to dtype.  bias may be NULL; it, x and y have the same dtype.
-   The workspace (nz_mx_linear_workspace_bytes(m, n, k), 16-byte aligned, may be 0) is free again when the call's
-   work has ended. */
-uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k);
+   k is 1 to 2^22, n at most 2^22.
+   The workspace (nz_mx_linear_workspace_bytes bytes, 16-byte aligned, none if that is 0) is free again when the
+   call's work has ended. */
+uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype);
 int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t stride, const void* dev_w_data,
                  const void* dev_w_scales, uint64_t n, const void* dev_bias, void* dev_y, void* dev_workspace,
                  uint64_t workspace_bytes, void* stream);
@@ -478,9 +479,12 @@ int nz_mx_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_
                        int dtype, void* dev_workspace, uint64_t workspace_bytes, void* stream);
 
 /* dx[m][k] = sum_n g[m][n] w[n][k], g with `stride` elements from row to row: the gradient of that product's rows
-   (their rounding to 8 bits is passed straight through). */
+   (their rounding to 8 bits is passed straight through).  n is 1 at least; the workspace is as above. */
+uint64_t nz_mx_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
+                                           uint64_t k);
 int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
-                      const void* dev_w_scales, uint64_t k, void* dev_dx, void* stream);
+                      const void* dev_w_scales, uint64_t k, void* dev_dx, void* dev_workspace,
+                      uint64_t workspace_bytes, void* stream);
 
 /* The gradient of an embedding table of rows x cols that was looked up at dev_indices[0..count) (int64):
    out[v] = scale * sum of g[t] over the t with index v, in the order of t, in 32 bits, rounded once (the same

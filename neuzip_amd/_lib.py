@@ -34,7 +34,8 @@ EXPORTS = [
     "nz_manager_norm_bytes", "nz_manager_buffers", "nz_manager_erase", "nz_manager_check",
     "nz_manager_export", "nz_manager_import", "nz_manager_trim", "nz_manager_rewrite_stats", "nz_set_lookback_spins", "nz_manager_geometry_hint",
     "nz_mx_row_bytes", "nz_mx_scale_bytes", "nz_mx_quantize", "nz_mx_dequantize", "nz_mx_lookup",
-    "nz_mx_linear_workspace_bytes", "nz_mx_linear", "nz_mx_linear_rows8", "nz_mx_linear_grad",
+    "nz_mx_linear_workspace_bytes", "nz_mx_linear", "nz_mx_linear_rows8",
+    "nz_mx_linear_grad_workspace_bytes", "nz_mx_linear_grad",
     "nz_embedding_gradient_workspace_bytes", "nz_embedding_gradient",
 ]
 
@@ -146,13 +147,15 @@ def load() -> ctypes.CDLL:
     L.nz_mx_lookup.restype = i32
     L.nz_mx_lookup.argtypes = [vp, vp, u64, u64, i32, vp, u64, ctypes.c_float, vp, i32, vp, vp]
     L.nz_mx_linear_workspace_bytes.restype = u64
-    L.nz_mx_linear_workspace_bytes.argtypes = [u64, u64, u64]
+    L.nz_mx_linear_workspace_bytes.argtypes = [u64, u64, u64, i32]
     L.nz_mx_linear.restype = i32
     L.nz_mx_linear.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp, vp, u64, vp]
     L.nz_mx_linear_rows8.restype = i32
     L.nz_mx_linear_rows8.argtypes = [vp, vp, u64, u64, vp, vp, u64, vp, vp, i32, vp, u64, vp]
     L.nz_mx_linear_grad.restype = i32
-    L.nz_mx_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp]
+    L.nz_mx_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp, u64, vp]
+    L.nz_mx_linear_grad_workspace_bytes.restype = u64
+    L.nz_mx_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
     L.nz_embedding_gradient_workspace_bytes.restype = u64
     L.nz_embedding_gradient_workspace_bytes.argtypes = [u64, u64, u64]
     L.nz_embedding_gradient.restype = i32

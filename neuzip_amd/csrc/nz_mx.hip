@@ -3,6 +3,8 @@
 // The format is stated in include/neuzip_hip.h.  A row's codes lie in order and are filled up to 128 values, so
 // that a step of the matrix instruction (128 values of a row) never ends inside one; its block scales lie in
 // groups of 16 (512 values) with the four bytes that a lane needs in four successive steps next to each other.
+#include <type_traits>
+
 #include "nz_operators.h"
 
 namespace {
@@ -27,35 +29,37 @@ struct Element<8> {
 
 // ---- elements --------------------------------------------------------------------------------------------------
 
+// Rows begin wherever their elements may: a vector of 8 is as aligned as one of them, which the memory allows.
 template <class T>
-__device__ inline void load8(const T* p, float (&v)[8]) {
-  typedef T pack __attribute__((ext_vector_type(8)));
-  const pack a = *reinterpret_cast<const pack*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-}
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+};
 
-// the first `n` of 8 values, zeros behind them
+// 8 values of which the first `n` count, zeros behind them
 template <class T>
-__device__ inline void load8_part(const T* p, long long n, float (&v)[8]) {
+__device__ inline void load8_upto(const T* p, uint32_t n, float (&v)[8]) {
+  if (n >= 8) {
+    const typename Pack<T>::type a = *reinterpret_cast<const typename Pack<T>::type*>(p);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.0f;
-}
-
-template <class T>
-__device__ inline void store8(T* p, const float (&v)[8]) {
-  typedef T pack __attribute__((ext_vector_type(8)));
-  pack a;
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
-  *reinterpret_cast<pack*>(p) = a;
+    for (int i = 0; i < 8; ++i) v[i] = (uint32_t)i < n ? (float)p[i] : 0.0f;
+  }
 }
 
 template <class T>
-__device__ inline void store8_part(T* p, long long n, const float (&v)[8]) {
+__device__ inline void store8_upto(T* p, uint32_t n, const float (&v)[8]) {
+  if (n >= 8) {
+    typename Pack<T>::type a;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = (T)v[i];
+    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+    *reinterpret_cast<typename Pack<T>::type*>(p) = a;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((uint32_t)i < n) p[i] = (T)v[i];
+  }
 }
 
 // scale byte of a block from the bits of its largest magnitude: a subnormal has exponent bits 0, which the clamp
@@ -116,6 +120,21 @@ __device__ inline void values8(uint2 codes, float factor, float (&v)[8]) {
   v[4] = c.x * factor, v[5] = c.y * factor, v[6] = d.x * factor, v[7] = d.y * factor;
 }
 
+// Scale byte of a block that four lanes share, 8 values each; a block that reads as NaN is cleared.
+template <int BITS>
+__device__ inline uint32_t block_scale(float (&v)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, true));  // lane ^ 1
+  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, true));  // lane ^ 2
+  const uint32_t s = scale_byte<BITS>(top);
+  if (s == 255)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  return s;
+}
+
 // place of block b (of a row) among the row's scale bytes
 __device__ inline uint32_t scale_at(uint32_t b) { return (b & ~15u) + 4 * (b & 3) + ((b >> 2) & 3); }
 
@@ -126,8 +145,8 @@ __device__ inline uint32_t scale_at(uint32_t b) { return (b & ~15u) + 4 * (b & 3
 
 template <int BITS, class T>
 __global__ __launch_bounds__(256) void nz_mx_quantize_kernel(const T* x, uint64_t stride, uint32_t cols,
-                                                             uint64_t waves, uint32_t groups, uint32_t wide,
-                                                             uint8_t* data, uint8_t* scales) {
+                                                             uint64_t waves, uint32_t groups, uint8_t* data,
+                                                             uint8_t* scales) {
   const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
   const uint32_t lane = threadIdx.x & 63;
@@ -136,19 +155,8 @@ __global__ __launch_bounds__(256) void nz_mx_quantize_kernel(const T* x, uint64_
   const uint32_t at = group * kGroup + lane * 8;
   const T* p = x + row * stride + at;
   float v[8];
-  if (wide && at + 8 <= cols)
-    load8(p, v);
-  else
-    load8_part(p, (long long)cols - at, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, true));  // lane ^ 1
-  top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, true));  // lane ^ 2
-  const uint32_t s = scale_byte<BITS>(top);
-  if (s == 255)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  load8_upto(p, at < cols ? cols - at : 0, v);
+  const uint32_t s = block_scale<BITS>(v);
   const float up = up_factor(s);
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
   if (at < filled) {
@@ -165,8 +173,7 @@ __global__ __launch_bounds__(256) void nz_mx_quantize_kernel(const T* x, uint64_
 template <int BITS, class T>
 __global__ __launch_bounds__(256) void nz_mx_values_kernel(const uint8_t* data, const uint8_t* scales, uint64_t rows,
                                                            uint32_t cols, const long long* index, uint64_t waves,
-                                                           uint32_t groups, uint32_t wide, float scale, T* out,
-                                                           uint32_t* status) {
+                                                           uint32_t groups, float scale, T* out, uint32_t* status) {
   const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
   const uint32_t lane = threadIdx.x & 63;
@@ -190,11 +197,7 @@ __global__ __launch_bounds__(256) void nz_mx_values_kernel(const uint8_t* data, 
     for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     if (status && at == 0) atomicOr(status, 1u);
   }
-  T* q = out + to * (uint64_t)cols + at;
-  if (wide && at + 8 <= cols)
-    store8(q, v);
-  else
-    store8_part(q, (long long)cols - at, v);
+  store8_upto(out + to * (uint64_t)cols + at, cols - at, v);
 }
 
 // ---- product ---------------------------------------------------------------------------------------------------
@@ -215,106 +218,511 @@ __device__ inline f4 step(i4v w, i4v x0, i4v x1, f4 acc, uint32_t sw, uint32_t s
   }
 }
 
-// 16 weight rows against 16 MT activation rows; the wavefronts of a workgroup share the values of a row.
-template <int MT, class T>
-__global__ __launch_bounds__(512) void nz_mx_product_kernel(const uint8_t* xd, const uint8_t* xs, uint64_t m,
-                                                            const uint8_t* wd, const uint8_t* ws, uint64_t n,
-                                                            uint32_t k, const T* bias, T* y) {
+// 16 bytes of every lane to LDS: lane l's to `to` (the same for all lanes) + 16 l.
+__device__ inline void to_lds16(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// Wait until all but the last N loads of this wavefront have arrived.
+template <int N>
+__device__ inline void wait_loads() {
+  static_assert(N < 64, "what the counter holds");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ inline void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Tile of the workgroup.  Workgroups go to the eight dies in turn: a die takes a run of consecutive tiles, and
+// tiles are numbered through columns of eight tiles along m, so that what a die has in work at a time shares rows of
+// both sides in its L2.
+__device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& tm, uint32_t& tn) {
+  const uint32_t total = mt * nt, per = total / 8, rest = total % 8, die = id % 8;
+  id = die * per + min(die, rest) + id / 8;
+  const uint32_t column = id / (8 * nt), at = id - column * (8 * nt), high = min(mt - column * 8, 8u);
+  tm = column * 8 + at % high;
+  tn = at / high;
+}
+
+// Add the bias to a workgroup's tile and store it, or store it as it is among the parts.  A lane (r, g) of wavefront
+// (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], columns c0 .. c0 + 4 TN - 1.
+template <int WM, int WN, int TM, int TN, class T>
+__device__ inline void finish_tile(f4 (&acc)[TM][TN], uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+                                   const T* bias, T* y, float* part) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
-  const uint32_t steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
-  const uint64_t n0 = (uint64_t)blockIdx.x * 16, m0 = (uint64_t)blockIdx.y * (16 * MT);
-  const uint64_t wrow = min(n0 + r, n - 1);
-  const uint8_t* wp = wd + wrow * (steps * 64ull) + g * 16;
-  const uint8_t* wsp = ws + wrow * (groups * 16ull) + g * 4;
-  const uint8_t* xp[MT];
-  const uint8_t* xsp[MT];
-  f4 acc[MT];
+  const uint32_t wm = wave % WM, wn = wave / WM, c0 = n0 + wn * TN * 16 + g * TN * 4;
+  if (part) {
+    part += (uint64_t)blockIdx.y * m * n;
+    const bool wide = n % 4 == 0;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const uint64_t xrow = min(m0 + t * 16 + r, m - 1);
-    xp[t] = xd + xrow * (steps * 128ull) + g * 16;
-    xsp[t] = xs + xrow * (groups * 16ull) + g * 4;
-    acc[t] = f4{0, 0, 0, 0};
-  }
-  for (uint32_t group = wave; group < groups; group += 8) {
-    const uint32_t sw = *reinterpret_cast<const uint32_t*>(wsp + group * 16);
-    uint32_t sx[MT];
+    for (int i = 0; i < TM; ++i) {
+      const uint32_t row = m0 + (wm * TM + i) * 16 + r;
+      if (row >= m) continue;
+      float* q = part + (uint64_t)row * n;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) sx[t] = *reinterpret_cast<const uint32_t*>(xsp[t] + group * 16);
+      for (int j = 0; j < TN; ++j) {
+        const uint32_t c = c0 + j * 4;
+        if (wide && c < n)
+          *(f4*)(q + c) = acc[i][j];
+        else
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t s = group * 4 + j;
-      if (s < steps) {
-        const i4v w = *reinterpret_cast<const i4v*>(wp + s * 64ull);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          const i4v x0 = *reinterpret_cast<const i4v*>(xp[t] + s * 128ull);
-          const i4v x1 = *reinterpret_cast<const i4v*>(xp[t] + s * 128ull + 64);
-          acc[t] = step(w, x0, x1, acc[t], sw, sx[t], j);
-        }
+          for (int e = 0; e < 4; ++e)
+            if (c + e < n) q[c + e] = acc[i][j][e];
       }
     }
+    return;
   }
-  __shared__ float part[8][MT * 256];
+  if (bias) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[wave][t * 256 + r * 16 + g * 4 + j] = acc[t][j];
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < MT * 256; i += 512) {
-    float sum = part[0][i];
+      for (int e = 0; e < 4; ++e) {
+        const float v = (float)bias[min(c0 + j * 4 + e, n - 1)];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) sum += part[w][i];
-    const uint64_t row = m0 + i / 16, col = n0 + i % 16;
-    if (row < m && col < n) {
-      if (bias) sum += (float)bias[col];
-      y[row * n + col] = (T)sum;
+        for (int i = 0; i < TM; ++i) acc[i][j][e] += v;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    const uint32_t row = m0 + (wm * TM + i) * 16 + r;
+    if (row >= m) continue;
+    T* q = y + (uint64_t)row * n;
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const uint32_t c = c0 + j * 4;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e], v[4 + e] = acc[i][j + 1][e];
+      if (c < n) store8_upto(q + c, n - c, v);
     }
   }
 }
 
-// ---- gradient of the rows --------------------------------------------------------------------------------------
+// A tile of WM TM x WN TN matrix instructions' results, WM x WN wavefronts with TM x TN each.
+//
+// The rows of both sides are staged through LDS in steps of 128 values, NS stages deep, by loads that go to LDS
+// without registers; a wavefront counts its own loads down, and one barrier a step tells that everybody's have
+// arrived and that the stage before is used up.  Staged rows are exchanged in chunks of 16 bytes (x: chunk c of row
+// r at c ^ (r & 7); w: at c ^ ((r >> 1) & 3)) so that eight lanes in turn read from all banks, and the weight rows of
+// a wavefront are staged in an order that leaves each lane 4 TN consecutive columns of the result.  Scales are
+// staged once per 512 values.
+template <int WM, int WN, int TM, int TN, int NS, class T>
+__global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles_kernel(const uint8_t* xd, const uint8_t* xs, uint32_t m,
+                                                                   const uint8_t* wd, const uint8_t* ws, uint32_t n,
+                                                                   uint32_t k, const T* bias, T* y, uint32_t mt,
+                                                                   uint32_t nt, uint32_t part_groups, float* part) {
+  constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+  constexpr int XB = BM * 128, WB = BN * 64, STAGE = XB + WB;
+  constexpr int XI = BM / 8 / W, WI = BN / 16 / W, LOADS = XI + WI;
+  constexpr int SI = (BM + BN + 63) / 64, SB = SI * 1024;  // scales: 64 rows of 16 bytes a load
+  static_assert(XI * 8 * W == BM && WI * 16 * W == BN && SI <= W, "loads per wavefront");
+  static_assert(NS >= 3 && NS <= 8, "two buffers of scales reach 8 stages");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + 2 * SB];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+  const uint32_t all_steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
+  const uint32_t from = blockIdx.y * part_groups, steps = min(all_steps - from * 4, part_groups * 4);
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, mt, nt, tm, tn);
+  const uint32_t m0 = tm * BM, n0 = tn * BN;
+  const uint32_t m_last = min((uint32_t)BM, m - m0) - 1, n_last = min((uint32_t)BN, n - n0) - 1;
 
-template <class T>
-__global__ __launch_bounds__(256) void nz_mx_grad_kernel(const T* g, uint64_t stride, uint64_t m, uint64_t n,
-                                                         const uint8_t* wd, const uint8_t* ws, uint32_t k, T* dx) {
-  __shared__ float sg[32][65], sw[32][64];
-  const uint32_t steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
-  const uint32_t k0 = blockIdx.x * 64;
-  const uint64_t m0 = (uint64_t)blockIdx.y * 64;
-  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (uint64_t n0 = 0; n0 < n; n0 += 32) {
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 64 * 32; i += 256) {
-      const uint64_t row = m0 + i / 32, col = n0 + i % 32;
-      sg[i % 32][i / 32] = row < m && col < n ? (float)g[row * stride + col] : 0.0f;
-    }
-    {
-      const uint32_t i = threadIdx.x;  // 32 rows of 64 values, 8 a lane
-      const uint64_t row = n0 + i / 8;
-      const uint32_t at = k0 + (i % 8) * 8;
-      float v[8] = {};
-      if (row < n && at < steps * kStep)
-        values4(*reinterpret_cast<const uint32_t*>(wd + row * (steps * 64ull) + at / 2),
-                down_factor(ws[row * (groups * 16ull) + scale_at(at / 32)]), v);
+  // Where this lane loads from: a base of the workgroup and an offset.  Rows behind the last one are read as the last.
+  const uint8_t* xb = xd + (uint64_t)m0 * (all_steps * 128ull) + from * 512ull;
+  const uint8_t* wb = wd + (uint64_t)n0 * (all_steps * 64ull) + from * 256ull;
+  const auto column = [](uint32_t row) {  // of the tile, for a staged weight row
+    return row / (TN * 16) * (TN * 16) + row % 16 / 4 * (TN * 4) + row / 16 % TN * 4 + row % 4;
+  };
+  uint32_t xo[XI], wo[WI];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sw[i / 8][(i % 8) * 8 + j] = v[j];
-    }
-    __syncthreads();
-    for (int j = 0; j < 32; ++j) {
+  for (int i = 0; i < XI; ++i)
+    xo[i] = min((wave * XI + i) * 8 + lane / 8, m_last) * (all_steps * 128) + ((lane & 7) ^ (lane / 8)) * 16;
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+  for (int i = 0; i < WI; ++i)
+    wo[i] = min(column((wave * WI + i) * 16 + lane / 4), n_last) * (all_steps * 64) +
+            ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
+  const uint32_t si = wave % SI, srow = min(si * 64 + lane, BM + BN - 1u);  // more wavefronts than loads: some load the same
+  const uint8_t* sb = (srow < BM ? xs + ((uint64_t)m0 + min(srow, m_last)) * (groups * 16ull)
+                                 : ws + ((uint64_t)n0 + min(column(srow - BM), n_last)) * (groups * 16ull)) +
+                      from * 16;
+  uint32_t sbuf = 0;
+  const auto load_stage = [&](uint32_t s, uint32_t buf, bool scales) {
+    s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
+    uint8_t* to = lds + buf * STAGE;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] += sg[j][ty * 4 + a] * sw[j][tx * 4 + b];
+    for (int i = 0; i < XI; ++i) to_lds16(xb + s * 128ull + xo[i], to + (wave * XI + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < WI; ++i) to_lds16(wb + s * 64ull + wo[i], to + XB + (wave * WI + i) * 1024);
+    if (scales) to_lds16(sb + (s >> 2) * 16, lds + NS * STAGE + sbuf * SB + si * 1024), sbuf ^= 1;
+  };
+
+  const uint32_t wm = wave % WM, wn = wave / WM;
+  f4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4{0, 0, 0, 0};
+  uint32_t sx[TM], sw[TN];
+  const uint32_t xr = (wm * TM * 16 + r) * 128, x0c = (g ^ (r & 7)) * 16, x1c = x0c ^ 64;
+  const uint32_t wr = XB + (wn * TN * 16 + r) * 64 + (g ^ ((r >> 1) & 3)) * 16;
+
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) load_stage(i, i, i % 4 == 0);
+  uint32_t buf = 0, cur = 0;
+  const auto body = [&](uint32_t s, auto b4) {
+    constexpr int byte = decltype(b4)::value;  // s % 4
+    // loads behind those of stage s: NS - 2 stages, with scales where a stage begins a group
+    constexpr int starts = (byte + NS - 2) / 4;
+    wait_loads<(NS - 2) * LOADS + starts>();
+    block_barrier();  // stage s is there, stage s - 1 is used up
+    const uint8_t* b = lds + buf * STAGE;
+    if (byte == 0) {
+      const uint8_t* st = lds + NS * STAGE + cur * SB;
+      cur ^= 1;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) sx[i] = *(const uint32_t*)(st + (wm * TM * 16 + i * 16 + r) * 16 + g * 4);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) sw[j] = *(const uint32_t*)(st + (BM + wn * TN * 16 + j * 16 + r) * 16 + g * 4);
     }
+    i4v x0[TM], x1[TM], w[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      x0[i] = *(const i4v*)(b + xr + i * 2048 + x0c);
+      x1[i] = *(const i4v*)(b + xr + i * 2048 + x1c);
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) w[j] = *(const i4v*)(b + wr + j * 1024);
+    load_stage(s + NS - 1, buf == 0 ? NS - 1 : buf - 1, (byte + NS - 1) % 4 == 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) acc[i][j] = step(w[j], x0[i], x1[i], acc[i][j], sw[j], sx[i], byte);
+    buf = buf == NS - 1 ? 0 : buf + 1;
+    __builtin_amdgcn_sched_barrier(0);  // matrix instructions stay inside their step
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  using B2 = std::integral_constant<int, 2>;
+  using B3 = std::integral_constant<int, 3>;
+  uint32_t s = 0;
+  for (; s + 4 <= steps; s += 4) {
+    body(s, B0());
+    body(s + 1, B1());
+    body(s + 2, B2());
+    body(s + 3, B3());
   }
-  for (int a = 0; a < 4; ++a)
-    for (int b = 0; b < 4; ++b) {
-      const uint64_t row = m0 + ty * 4 + a;
-      const uint32_t col = k0 + tx * 4 + b;
-      if (row < m && col < k) dx[row * k + col] = (T)acc[a][b];
+  if (s < steps) body(s, B0());
+  if (s + 1 < steps) body(s + 1, B1());
+  if (s + 2 < steps) body(s + 2, B2());
+  wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
+
+  finish_tile<WM, WN, TM, TN>(acc, m, n, m0, n0, bias, y, part);
+}
+
+// The parts of a product whose rows were cut, added in their order.
+template <class T>
+__global__ __launch_bounds__(256) void nz_mx_join_kernel(const float* part, uint32_t parts, uint64_t size, uint32_t n,
+                                                         const T* bias, T* y) {
+  const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= size) return;
+  if (size % 4 == 0) {
+    f4 sum = *(const f4*)(part + at);
+    for (uint32_t i = 1; i < parts; ++i) sum += *(const f4*)(part + i * size + at);
+    const uint32_t col = (uint32_t)(at % n);
+    typedef T pack __attribute__((ext_vector_type(4)));
+    pack v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)(bias ? sum[e] + (float)bias[(col + e) % n] : sum[e]);
+    *(pack*)(y + at) = v;
+    return;
+  }
+  for (uint64_t i = at; i < min(at + 4, size); ++i) {
+    float sum = part[i];
+    for (uint32_t p = 1; p < parts; ++p) sum += part[p * size + i];
+    y[i] = (T)(bias ? sum + (float)bias[i % n] : sum);
+  }
+}
+
+// Up to 16 rows, where reading the weight is all that counts: no staging and no barrier in the way of it.  The eight
+// wavefronts are KW that share the values of a row (512 at a time, in turn) times 8 / KW with NT x 16 weight rows
+// each; a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
+// (QUANTIZE) as they are: then every workgroup brings them to 8 bits in LDS while its first weights are on their way.
+template <int NT, bool QUANTIZE, class T>
+__global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t stride, const uint8_t* xs,
+                                                        uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t n,
+                                                        uint32_t k, const T* bias, T* y, uint32_t kw) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+  const uint32_t steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
+  const uint32_t kwave = wave % kw, tile0 = (blockIdx.x * (8 / kw) + wave / kw) * NT;
+  const uint8_t* wp[NT];
+  const uint8_t* sp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const uint64_t row = min((tile0 + j) * 16 + r, n - 1);
+    wp[j] = wd + row * (steps * 64ull) + g * 16;
+    sp[j] = ws + row * (groups * 16ull) + g * 4;
+  }
+  struct Held {
+    i4v w[NT][4];
+    uint32_t s[NT];
+  } a, b;
+  const auto load = [&](Held& h, uint32_t group) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      h.s[j] = *(const uint32_t*)(sp[j] + group * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h.w[j][i] = *(const i4v*)(wp[j] + (uint64_t)min(group * 4 + i, steps - 1) * 64);
     }
+  };
+  if (kwave < groups) load(a, kwave);
+
+  const uint32_t row = min(r, m - 1);
+  const uint8_t *xp, *xsp;
+  if constexpr (QUANTIZE) {
+    // rows of groups * 528 bytes: 512 values and their scales per group
+    const T* xt = (const T*)x;
+    for (uint32_t i = wave; i < m * groups; i += 8) {
+      const uint32_t to = i / groups, group = i - to * groups, at = group * kGroup + lane * 8;
+      float v[8];
+      load8_upto(xt + to * stride + at, at < k ? k - at : 0, v);
+      const uint32_t s = block_scale<8>(v);
+      uint8_t* q = few_lds + i * 528u;
+      *(uint2*)(q + lane * 8) = codes8(v, up_factor(s));
+      if ((lane & 3) == 0) q[512 + scale_at(lane / 4)] = (uint8_t)s;
+    }
+    __syncthreads();
+    xp = few_lds + row * groups * 528u + g * 16;
+    xsp = few_lds + row * groups * 528u + 512 + g * 4;
+  } else {
+    xp = (const uint8_t*)x + row * (steps * 128ull) + g * 16;
+    xsp = xs + row * (groups * 16ull) + g * 4;
+  }
+  f4 acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = f4{0, 0, 0, 0};
+  const auto multiply = [&](const Held& h, uint32_t group) {
+    const uint32_t sx = *(const uint32_t*)(xsp + group * (QUANTIZE ? 528 : 16));
+    const auto one = [&](auto b4) {
+      constexpr int i = decltype(b4)::value;
+      if (group * 4 + i >= steps) return;
+      const uint8_t* p = xp + (QUANTIZE ? group * 528 : (uint64_t)group * 512) + i * 128;
+      const i4v x0 = *(const i4v*)p, x1 = *(const i4v*)(p + 64);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[j] = step(h.w[j][i], x0, x1, acc[j], h.s[j], sx, i);
+    };
+    one(std::integral_constant<int, 0>());
+    one(std::integral_constant<int, 1>());
+    one(std::integral_constant<int, 2>());
+    one(std::integral_constant<int, 3>());
+  };
+  for (uint32_t group = kwave; group < groups; group += 2 * kw) {  // one group is on its way while one is multiplied
+    if (group + kw < groups) load(b, group + kw);
+    multiply(a, group);
+    if (group + kw >= groups) break;
+    if (group + 2 * kw < groups) load(a, group + 2 * kw);
+    multiply(b, group + kw);
+  }
+  // the wavefronts that share rows add up in their order
+  __syncthreads();
+  float* part = (float*)few_lds;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) *(f4*)(part + ((wave * NT + j) * 16 + r) * 16 + g * 4) = acc[j];
+  __syncthreads();
+  const uint32_t tiles = 8 / kw * NT;
+  for (uint32_t i = threadIdx.x; i < m * tiles * 16; i += 512) {
+    const uint32_t to = i / (tiles * 16), c = i - to * (tiles * 16), t = c / 16;
+    const uint32_t col = blockIdx.x * tiles * 16 + c;
+    if (col >= n) continue;
+    float sum = 0;
+    for (uint32_t q = 0; q < kw; ++q) sum += part[(((t / NT * kw + q) * NT + t % NT) * 16 + to) * 16 + c % 16];
+    if (bias) sum += (float)bias[col];
+    y[(uint64_t)to * n + col] = (T)sum;
+  }
+}
+
+// ---- products of 16-bit rows -----------------------------------------------------------------------------------
+//
+// What the scaled instruction cannot do: the gradient of the rows, whose sums run over the weight's rows (a lane
+// would need a scale per value), and results in float32 (the scaled instruction drops what lies 16 bits below the
+// largest of its 128 products: 1.5e-5 of a sum, measured, against 6e-8 of this one).  A weight's values are exact in
+// bf16, and so is an activation of 8 bits; a gradient of 16 or 32 bits is the sum of two or three bf16 numbers, laid
+// side by side along the summed axis.
+
+typedef nz_bf16 b8v __attribute__((ext_vector_type(8)));
+typedef nz_bf16 b4v __attribute__((ext_vector_type(4)));
+typedef nz_bf16 b2v __attribute__((ext_vector_type(2)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+// 8 codes as bf16 numbers.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
+__device__ inline b8v bf16_of_codes(uint32_t codes, uint32_t s) {
+  const float scale = __uint_as_float(s << 23);
+  const b2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
+  const b2v b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+  const b2v c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
+  const b2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+  return b8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Rows cut into P bf16 planes, [m][P][padded]: each plane takes the 8 leading bits that the planes before it left, so
+// three hold all 24 bits of a float32 and two the 11 of a float16.  What is not finite stays in the first.
+template <int P, class T>
+__global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t stride, uint64_t m, uint32_t n,
+                                                           uint32_t padded, nz_bf16* out) {
+  const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const uint64_t row = at / padded;
+  const uint32_t c = (uint32_t)(at - row * padded);
+  if (row >= m) return;
+  float v[8];
+  load8_upto(g + row * stride + c, c < n ? n - c : 0, v);
+  nz_bf16* q = out + row * P * padded + c;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    b8v b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __float_as_uint(v[i]), hi = (u >> 23 & 255) == 255 && (u & 0x7FFFFF) ? u | 0x400000 : u;
+      const float first = __uint_as_float(hi & 0xFFFF0000u);
+      b[i] = __builtin_bit_cast(nz_bf16, (unsigned short)(hi >> 16));
+      v[i] = (u >> 23 & 255) == 255 ? 0.0f : v[i] - first;
+    }
+    *(b8v*)(q + (uint64_t)p * padded) = b;
+  }
+}
+
+// A tile of C[m][cols] = sum over c of A[m][c] B(c, col), c running `planes` times through the summed axis.
+// ROWS: B(c, col) = w[c][col], the gradient; else w[col][c], the product itself.
+//
+// Steps of 64 values.  A is staged three deep by loads that go to LDS without registers (16-byte chunk c of a row at
+// c ^ (row & 7)); the weight is loaded as codes two steps ahead and written to LDS as bf16 one step ahead.  Where the
+// sums run over the weight's rows its tile lies in LDS as in memory, and the operand is read by the instruction that
+// transposes 4 x 16 values on the way; its rows exchange 8-byte slots (slot ^ (row & 3)) against bank conflicts.
+// A lane ends with 4 TN consecutive columns, as in nz_mx_tiles_kernel.
+template <int WM, int WN, int TM, int TN, bool ROWS, class T>
+__global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf16* a, uint64_t a_stride, uint32_t m,
+                                                                     const uint8_t* wd, const uint8_t* ws,
+                                                                     uint32_t w_rows, uint32_t w_cols, uint32_t steps_1,
+                                                                     uint32_t planes, uint32_t cols, const T* bias,
+                                                                     T* y, uint32_t mt, uint32_t nt,
+                                                                     uint32_t part_steps, float* part) {
+  constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+  constexpr int AB = BM * 128, BB = BN * 128, XI = BM / 8 / W;
+  constexpr int CW = BN / (8 * W), CODES = 8 * CW;  // words and codes of the weight, per lane and step
+  static_assert(XI * 8 * W == BM && CW * 8 * W == BN && (CW == 2 || CW == 4), "loads per wavefront");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * AB + 2 * BB];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+  const uint32_t from = blockIdx.y * part_steps, steps = min(steps_1 * planes - from, part_steps);
+  const uint32_t w_steps = (w_cols + kStep - 1) / kStep, w_groups = (w_cols + kGroup - 1) / kGroup;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, mt, nt, tm, tn);
+  const uint32_t m0 = tm * BM, n0 = tn * BN, m_last = min((uint32_t)BM, m - m0) - 1;
+
+  const uint8_t* ab = (const uint8_t*)(a + (uint64_t)m0 * a_stride) + from * 128ull;
+  uint32_t ao[XI];
+#pragma unroll
+  for (int i = 0; i < XI; ++i)
+    ao[i] = min((wave * XI + i) * 8 + lane / 8, m_last) * (uint32_t)(a_stride * 2) + ((lane & 7) ^ (lane / 8)) * 16;
+  const auto load_a = [&](uint32_t s, uint32_t buf) {
+    s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
+#pragma unroll
+    for (int i = 0; i < XI; ++i) to_lds16(ab + s * 128ull + ao[i], lds + buf * AB + (wave * XI + i) * 1024);
+  };
+
+  // this lane's codes of the weight: ROWS: CODES columns of row l_row; else CODES values of column l_row of the tile
+  const uint32_t across = (ROWS ? BN : 64) / CODES, l_row = threadIdx.x / across, l_at = threadIdx.x % across * CODES;
+  typedef uint32_t words __attribute__((ext_vector_type(CW)));
+  words codes;
+  uint32_t scale;
+  const auto load_w = [&](uint32_t s) {
+    s = (min(s, steps - 1) + from) % steps_1;
+    uint32_t row, at;
+    if constexpr (ROWS) {
+      row = min(s * 64 + l_row, w_rows - 1);
+      at = min(n0 + l_at, w_steps * kStep - CODES);
+    } else {
+      row = min(n0 + l_row / (TN * 16) * (TN * 16) + l_row % 16 / 4 * (TN * 4) + l_row / 16 % TN * 4 + l_row % 4,
+                w_rows - 1);
+      at = s * 64 + l_at;
+    }
+    codes = *(const words*)(wd + row * (w_steps * 64ull) + at / 2);
+    scale = ws[row * (w_groups * 16ull) + scale_at(at / 32)];
+  };
+  const auto store_w = [&](uint32_t buf) {
+    uint8_t* to = lds + 3 * AB + buf * BB + l_row * (ROWS ? BN * 2 : 128);
+#pragma unroll
+    for (int j = 0; j < CW; ++j) {
+      const i4v v = __builtin_bit_cast(i4v, bf16_of_codes(codes[j], scale));
+      const uint32_t chunk = l_at / 8 + j;
+      if constexpr (ROWS)
+        *(i4v*)(to + (chunk ^ (l_row >> 1 & 1)) * 16) = l_row & 1 ? i4v{v.z, v.w, v.x, v.y} : v;
+      else
+        *(i4v*)(to + (chunk ^ (l_row & 7)) * 16) = v;
+    }
+  };
+
+  const uint32_t wm = wave % WM, wn = wave / WM;
+  f4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f4{0, 0, 0, 0};
+  const uint32_t xr = (wm * TM * 16 + r) * 128;
+
+  load_w(0);
+  load_a(0, 0);
+  store_w(0);
+  load_w(1);
+  __builtin_amdgcn_sched_barrier(0);
+  load_a(1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  uint32_t buf = 0;
+  for (uint32_t s = 0; s < steps; ++s) {
+    // behind the rows of step s: those of step s + 1 and the codes and scales of step s + 1
+    wait_loads<XI + 2>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();  // step s is in LDS, step s - 1 is used up
+    const uint8_t* pa = lds + buf * AB;
+    const uint8_t* pb = lds + 3 * AB + (s & 1) * BB;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      b8v av[TM], bv[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) av[i] = *(const b8v*)(pa + xr + i * 2048 + ((h * 4 + g) ^ (r & 7)) * 16);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        if constexpr (ROWS) {
+          s4v half[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t row = h * 32 + g * 8 + q * 4 + r / 4, slot = (wn * TN * 4 + r % 4 * TN + j) ^ (r / 4);
+            half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s4v*)(pb + row * (BN * 2) + slot * 8));
+          }
+          bv[j] = __builtin_bit_cast(b8v, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+          bv[j] = *(const b8v*)(pb + (wn * TN * 16 + j * 16 + r) * 128 + ((h * 4 + g) ^ (r & 7)) * 16);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j], av[i], acc[i][j], 0, 0, 0);
+      if (h == 0) {
+        store_w((s + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_w(s + 2);
+        load_a(s + 2, buf == 0 ? 2 : buf - 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    buf = buf == 2 ? 0 : buf + 1;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  wait_loads<0>();
+  finish_tile<WM, WN, TM, TN>(acc, m, cols, m0, n0, bias, y, part);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------
@@ -349,9 +757,6 @@ int check_grid(uint64_t blocks) {
   return blocks <= 0x7FFFFFFFull ? NZ_OK : nz_fail(NZ_ERR_ARG, "too many rows for one launch");
 }
 
-// rows of `stride` elements that all start 16-byte aligned
-bool wide_rows(const void* p, uint64_t stride, uint32_t size) { return aligned(p, 16) && stride * size % 16 == 0; }
-
 template <class F>
 void by_dtype(int dtype, F f) {
   if (dtype == NZ_DTYPE_BF16)
@@ -367,14 +772,13 @@ void launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uin
   const uint32_t groups = (cols + kGroup - 1) / kGroup;
   const uint64_t waves = rows * groups;
   const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
-  const uint32_t wide = wide_rows(x, stride, nz_dtype_bytes(dtype));
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (bits == 4)
-      nz_mx_quantize_kernel<4, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups, wide,
+      nz_mx_quantize_kernel<4, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups,
                                                         (uint8_t*)data, (uint8_t*)scales);
     else
-      nz_mx_quantize_kernel<8, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups, wide,
+      nz_mx_quantize_kernel<8, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups,
                                                         (uint8_t*)data, (uint8_t*)scales);
   });
 }
@@ -385,46 +789,197 @@ int launch_values(const void* data, const void* scales, uint64_t rows, uint64_t 
   const uint64_t waves = nz_mul(count, groups);
   if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
   const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
-  const uint32_t wide = wide_rows(out, cols, nz_dtype_bytes(dtype));
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (bits == 4)
       nz_mx_values_kernel<4, T><<<grid, 256, 0, st>>>((const uint8_t*)data, (const uint8_t*)scales, rows,
-                                                      (uint32_t)cols, (const long long*)index, waves, groups, wide,
+                                                      (uint32_t)cols, (const long long*)index, waves, groups,
                                                       scale, (T*)out, (uint32_t*)status);
     else
       nz_mx_values_kernel<8, T><<<grid, 256, 0, st>>>((const uint8_t*)data, (const uint8_t*)scales, rows,
-                                                      (uint32_t)cols, (const long long*)index, waves, groups, wide,
+                                                      (uint32_t)cols, (const long long*)index, waves, groups,
                                                       scale, (T*)out, (uint32_t*)status);
   });
   return nz_launched();
 }
 
-int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n, uint32_t k,
-                   const void* bias, void* y, int dtype, hipStream_t st) {
-  const uint64_t mt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
-  const dim3 grid((uint32_t)nz_ceil_div(n, 16), (uint32_t)nz_ceil_div(m, 16 * mt));
+uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+// How a product is cut: the kernel's tile, and the parts the summed axis is cut into.
+struct Cut {
+  uint32_t bm, bn, parts, part_length, mt, nt;
+  uint64_t part_bytes(uint64_t m, uint64_t cols) const { return parts > 1 ? align256(parts * m * cols * 4) : 0; }
+};
+
+Cut cut_into(uint32_t bm, uint32_t bn, uint64_t m, uint64_t cols, uint64_t length, uint64_t parts) {
+  Cut c;
+  c.bm = bm, c.bn = bn;
+  c.mt = (uint32_t)nz_ceil_div(m, bm), c.nt = (uint32_t)nz_ceil_div(cols, bn);
+  c.part_length = (uint32_t)nz_ceil_div(length, parts ? parts : 1);
+  c.parts = (uint32_t)nz_ceil_div(length, c.part_length);
+  return c;
+}
+
+uint64_t tiles(uint64_t m, uint64_t n, uint32_t bm, uint32_t bn) { return nz_ceil_div(m, bm) * nz_ceil_div(n, bn); }
+
+uint64_t units() {
+  const uint32_t cus = nz_compute_units();
+  return cus ? cus : 256;
+}
+
+// The product of 8-bit rows: the largest tile that leaves enough workgroups; the smallest is cut along k as well,
+// into parts of 1024 values at least.
+Cut cut_product(uint64_t m, uint64_t n, uint64_t k) {
+  const uint64_t cus = units(), groups = nz_ceil_div(k, kGroup);
+  if (tiles(m, n, 256, 256) >= 4 * cus && k >= 2048) return cut_into(256, 256, m, n, groups, 1);
+  if (tiles(m, n, 128, 128) * 2 >= 3 * cus) return cut_into(128, 128, m, n, groups, 1);
+  if (tiles(m, n, 64, 128) * 2 >= cus) return cut_into(64, 128, m, n, groups, 1);
+  const uint64_t t = tiles(m, n, 64, 64), parts = (cus + t / 2) / t, most = groups / 2;
+  return cut_into(64, 64, m, n, groups, parts < most ? parts : most);
+}
+
+// The products of 16-bit rows, in steps of 64.
+Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) {
+  const uint64_t cus = units();
+  if (tiles(m, cols, 128, 128) * 2 >= cus) return cut_into(128, 128, m, cols, steps, 1);
+  const uint64_t t = tiles(m, cols, 64, 64), parts = (2 * cus + t / 2) / t, most = steps / 8;
+  return cut_into(64, 64, m, cols, steps, parts < most ? parts : most);
+}
+
+void launch_join(const float* part, const Cut& c, uint64_t m, uint64_t n, const void* bias, void* y, int dtype,
+                 hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-#define NZ_MX_PRODUCT(MT)                                                                                        \
-  nz_mx_product_kernel<MT, T><<<grid, 512, 0, st>>>((const uint8_t*)xd, (const uint8_t*)xs, m, (const uint8_t*)wd, \
-                                                    (const uint8_t*)ws, n, k, (const T*)bias, (T*)y)
-    if (mt == 1)
-      NZ_MX_PRODUCT(1);
-    else if (mt == 2)
-      NZ_MX_PRODUCT(2);
-    else
-      NZ_MX_PRODUCT(4);
-#undef NZ_MX_PRODUCT
+    nz_mx_join_kernel<T><<<(uint32_t)nz_ceil_div(m * n, 1024), 256, 0, st>>>(part, c.parts, m * n, (uint32_t)n,
+                                                                            (const T*)bias, (T*)y);
   });
+}
+
+template <bool ROWS>
+int launch_tiles16(const Cut& c, const void* a, uint64_t a_stride, uint64_t m, const void* wd, const void* ws,
+                   uint64_t w_rows, uint64_t w_cols, uint64_t steps_1, uint32_t planes, uint64_t cols,
+                   const void* bias, void* y, int dtype, void* part, hipStream_t st) {
+  const dim3 grid(c.mt * c.nt, c.parts);
+  float* p = c.parts > 1 ? (float*)part : nullptr;
+  by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if constexpr (!ROWS && !std::is_same<T, float>::value) {
+      return;  // the product itself has results of 16 bits from the scaled instruction
+    } else {
+#define NZ_TILES16(WM, WN, TM, TN)                                                                                     \
+  nz_mx_tiles16_kernel<WM, WN, TM, TN, ROWS, T><<<grid, 64 * WM * WN, 0, st>>>(                                        \
+      (const nz_bf16*)a, a_stride, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)w_rows,              \
+      (uint32_t)w_cols, (uint32_t)steps_1, planes, (uint32_t)cols, (const T*)bias, (T*)y, c.mt, c.nt, c.part_length, p)
+      if (c.bm == 128)
+        NZ_TILES16(2, 2, 4, 4);
+      else
+        NZ_TILES16(2, 2, 2, 2);
+#undef NZ_TILES16
+    }
+  });
+  if (p) launch_join(p, c, m, cols, bias, y, dtype, st);
   return nz_launched();
 }
 
-// what both forms of the product, and its gradient, ask of the weight and the counts
+// rows that are brought to 8 bits inside the kernel: as many as one workgroup does at little cost
+bool few_rows(uint64_t m, uint64_t k) { return m <= 16 && m * nz_ceil_div(k, kGroup) <= 64; }
+
+template <bool QUANTIZE, class T>
+void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n,
+                uint32_t k, const T* bias, T* y, hipStream_t st) {
+  const uint32_t groups = (k + kGroup - 1) / kGroup;
+  uint32_t kw = groups >= 8 ? 8 : groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
+  const uint64_t t = nz_ceil_div(n, 16);
+  if (kw == 8 && t > 2 * units()) kw = 4;
+  const uint32_t lds = QUANTIZE ? (uint32_t)m * groups * 528 : 0;
+  nz_mx_few_kernel<1, QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
+      x, stride, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, bias, y, kw);
+}
+
+template <class T>
+void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n,
+                  uint32_t k, const T* bias, T* y, float* part, hipStream_t st) {
+  const dim3 grid(c.mt * c.nt, c.parts);
+#define NZ_TILES(WM, WN, TM, TN, NS)                                                                               \
+  nz_mx_tiles_kernel<WM, WN, TM, TN, NS, T><<<grid, 64 * WM * WN, 0, st>>>(                                        \
+      (const uint8_t*)xd, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, \
+      bias, y, c.mt, c.nt, c.part_length, part)
+  if (c.bm == 256)
+    NZ_TILES(4, 2, 4, 8, 3);
+  else if (c.bm == 128)
+    NZ_TILES(2, 2, 4, 4, 3);
+  else if (c.bn == 128)
+    NZ_TILES(2, 2, 2, 4, 4);
+  else
+    NZ_TILES(2, 2, 2, 2, 4);
+#undef NZ_TILES
+}
+
+// Where a product's workspace holds what: rows in 8 bits, their values for a float32 result, parts.
+struct Room {
+  uint64_t xd, xs, values, parts, bytes;
+};
+Room product_room(uint64_t m, uint64_t n, uint64_t k, int dtype) {
+  Room r;
+  r.xd = 0;
+  r.xs = align256(nz_mul(m, nz_mx_row_bytes(k, 8)));
+  r.values = align256(r.xs + nz_mul(m, nz_mx_scale_bytes(k)));
+  const uint64_t pad = filled(k);
+  if (dtype == NZ_DTYPE_F32) {
+    r.parts = align256(r.values + nz_mul(m, pad * 2));
+    r.bytes = r.parts + cut_product16(m, n, pad / 64).part_bytes(m, n);
+  } else {
+    r.parts = r.values;
+    r.bytes = r.parts + cut_product(m, n, k).part_bytes(m, n);
+  }
+  return r;
+}
+
+int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n, uint32_t k,
+                   const void* bias, void* y, int dtype, const Room& room, uint8_t* workspace, hipStream_t st) {
+  if (dtype == NZ_DTYPE_F32) {
+    const uint64_t pad = filled(k);
+    if (int rc = launch_values(xd, xs, m, pad, 8, nullptr, m, 1.0f, workspace + room.values, NZ_DTYPE_BF16, nullptr,
+                               st))
+      return rc;
+    return launch_tiles16<false>(cut_product16(m, n, pad / 64), workspace + room.values, pad, m, wd, ws, n, k, pad / 64,
+                                 1, n, bias, y, dtype, workspace + room.parts, st);
+  }
+  const Cut c = cut_product(m, n, k);
+  float* part = c.parts > 1 ? (float*)(workspace + room.parts) : nullptr;
+  if (dtype == NZ_DTYPE_BF16)
+    launch_tiles(c, xd, xs, m, wd, ws, n, k, (const nz_bf16*)bias, (nz_bf16*)y, part, st);
+  else
+    launch_tiles(c, xd, xs, m, wd, ws, n, k, (const nz_f16*)bias, (nz_f16*)y, part, st);
+  if (part) launch_join(part, c, m, n, bias, y, dtype, st);
+  return nz_launched();
+}
+
+// What the products ask of the weight and the counts: an offset inside a tile has 32 bits.
 int check_product(uint64_t m, uint64_t n, uint64_t k, const void* wd, const void* ws) {
-  if (k == 0 || !cols_ok(k)) return nz_fail(NZ_ERR_ARG, "rows must hold 1 to 2^30 values");
-  if (m > 65535ull * 64 || n > 0x7FFFFFFFull) return nz_fail(NZ_ERR_ARG, "too many rows for one launch");
+  if (k == 0 || k > 1ull << 22 || n > 1ull << 22) return nz_fail(NZ_ERR_ARG, "a weight must have 1 to 2^22 columns and up to 2^22 rows");
+  if (m > 1ull << 24) return nz_fail(NZ_ERR_ARG, "too many rows for one launch");
   return check_mx(wd, ws);
+}
+
+int check_workspace(const void* workspace, uint64_t bytes, uint64_t need) {
+  if (bytes < need) return nz_fail(NZ_ERR_CAPACITY, "workspace too small");
+  if (need && (!workspace || !aligned(workspace, 16))) return nz_fail(NZ_ERR_ALIGN, "misaligned workspace");
+  return NZ_OK;
+}
+
+// The gradient's rows as planes of bf16, or as they are.
+struct Planes {
+  uint32_t count;
+  uint64_t padded, bytes;
+};
+Planes planes_of(const void* g, int dtype, uint64_t m, uint64_t n, uint64_t stride) {
+  Planes p;
+  p.count = dtype == NZ_DTYPE_BF16 ? 1 : dtype == NZ_DTYPE_F16 ? 2 : 3;
+  p.padded = nz_ceil_div(n, 64) * 64;
+  const bool as_is = dtype == NZ_DTYPE_BF16 && n % 64 == 0 && stride % 8 == 0 && stride < 1ull << 24 && aligned(g, 16);
+  p.bytes = as_is ? 0 : align256(nz_mul(m, p.padded * p.count * 2));
+  return p;
 }
 
 }  // namespace
@@ -469,9 +1024,10 @@ int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, ui
                        (hipStream_t)stream);
 }
 
-uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k) {
-  (void)n;
-  return (m * nz_mx_row_bytes(k, 8) + 255) / 256 * 256 + m * nz_mx_scale_bytes(k);
+uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype) {
+  if (m == 0 || n == 0 || k == 0) return 0;
+  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) return 0;
+  return product_room(m, n, k, dtype).bytes;
 }
 
 int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t stride, const void* dev_w_data,
@@ -481,45 +1037,87 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
   if (m == 0 || n == 0) return NZ_OK;
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
   if (!dev_x || !dev_y) return nz_fail(NZ_ERR_ARG, "null rows or output");
-  if (workspace_bytes < nz_mx_linear_workspace_bytes(m, n, k)) return nz_fail(NZ_ERR_CAPACITY, "workspace too small");
-  if (!dev_workspace || !aligned(dev_workspace, 16)) return nz_fail(NZ_ERR_ALIGN, "misaligned workspace");
-  uint8_t* xd = (uint8_t*)dev_workspace;
-  uint8_t* xs = xd + (m * nz_mx_row_bytes(k, 8) + 255) / 256 * 256;
-  launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, xd, xs, (hipStream_t)stream);
-  return launch_product(xd, xs, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, dtype,
-                        (hipStream_t)stream);
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, nz_mx_linear_workspace_bytes(m, n, k, dtype))) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) {
+    if (dtype == NZ_DTYPE_BF16)
+      launch_few<true>(dev_x, stride, nullptr, m, dev_w_data, dev_w_scales, n, (uint32_t)k, (const nz_bf16*)dev_bias,
+                       (nz_bf16*)dev_y, st);
+    else
+      launch_few<true>(dev_x, stride, nullptr, m, dev_w_data, dev_w_scales, n, (uint32_t)k, (const nz_f16*)dev_bias,
+                       (nz_f16*)dev_y, st);
+    return nz_launched();
+  }
+  const Room room = product_room(m, n, k, dtype);
+  uint8_t* base = (uint8_t*)dev_workspace;
+  launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st);
+  return launch_product(base + room.xd, base + room.xs, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y,
+                        dtype, room, base, st);
 }
 
 int nz_mx_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_t m, uint64_t k,
                        const void* dev_w_data, const void* dev_w_scales, uint64_t n, const void* dev_bias, void* dev_y,
                        int dtype, void* dev_workspace, uint64_t workspace_bytes, void* stream) {
-  (void)dev_workspace, (void)workspace_bytes;
   if (int rc = check_dtype(dtype, dev_bias, dev_y, nullptr)) return rc;
   if (m == 0 || n == 0) return NZ_OK;
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
   if (int rc = check_mx(dev_x_data, dev_x_scales)) return rc;
   if (!dev_y) return nz_fail(NZ_ERR_ARG, "null output");
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, nz_mx_linear_workspace_bytes(m, n, k, dtype))) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) {
+    if (dtype == NZ_DTYPE_BF16)
+      launch_few<false>(dev_x_data, 0, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k,
+                        (const nz_bf16*)dev_bias, (nz_bf16*)dev_y, st);
+    else
+      launch_few<false>(dev_x_data, 0, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k,
+                        (const nz_f16*)dev_bias, (nz_f16*)dev_y, st);
+    return nz_launched();
+  }
   return launch_product(dev_x_data, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, dtype,
-                        (hipStream_t)stream);
+                        product_room(m, n, k, dtype), (uint8_t*)dev_workspace, st);
+}
+
+uint64_t nz_mx_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
+                                           uint64_t k) {
+  if (m == 0 || n == 0 || k == 0) return 0;
+  const Planes p = planes_of(dev_g, dtype, m, n, stride);
+  return p.bytes + cut_product16(m, k, p.padded / 64 * p.count).part_bytes(m, k);
 }
 
 int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
-                      const void* dev_w_scales, uint64_t k, void* dev_dx, void* stream) {
+                      const void* dev_w_scales, uint64_t k, void* dev_dx, void* dev_workspace,
+                      uint64_t workspace_bytes, void* stream) {
   if (int rc = check_dtype(dtype, dev_g, dev_dx, nullptr)) return rc;
   if (m == 0 || k == 0) return NZ_OK;
-  if (!dev_dx) return nz_fail(NZ_ERR_ARG, "null output");
-  if (n) {
-    if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
-    if (!dev_g) return nz_fail(NZ_ERR_ARG, "null gradient");
+  if (!dev_dx || !dev_g) return nz_fail(NZ_ERR_ARG, "null gradient or output");
+  if (n == 0) return nz_fail(NZ_ERR_ARG, "a weight without rows has no gradient to pass on");
+  if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
+  if (int rc = check_workspace(dev_workspace, workspace_bytes,
+                               nz_mx_linear_grad_workspace_bytes(dev_g, dtype, m, n, stride, k)))
+    return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  const Planes p = planes_of(dev_g, dtype, m, n, stride);
+  const uint64_t steps = p.padded / 64;
+  const void* a = dev_g;
+  uint64_t a_stride = stride;
+  if (p.bytes) {
+    a = dev_workspace, a_stride = p.padded * p.count;
+    const uint64_t blocks = nz_ceil_div(m * (p.padded / 8), 256);
+    if (int rc = check_grid(blocks)) return rc;
+#define NZ_PLANES(P, T)                                                                                           \
+  nz_mx_planes_kernel<P, T><<<(uint32_t)blocks, 256, 0, st>>>((const T*)dev_g, stride, m, (uint32_t)n,            \
+                                                              (uint32_t)p.padded, (nz_bf16*)dev_workspace)
+    if (dtype == NZ_DTYPE_BF16)
+      NZ_PLANES(1, nz_bf16);
+    else if (dtype == NZ_DTYPE_F16)
+      NZ_PLANES(2, nz_f16);
+    else
+      NZ_PLANES(3, float);
+#undef NZ_PLANES
   }
-  const dim3 grid((uint32_t)nz_ceil_div(k, 64), (uint32_t)nz_ceil_div(m, 64));
-  by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    nz_mx_grad_kernel<T><<<grid, 256, 0, (hipStream_t)stream>>>((const T*)dev_g, stride, m, n,
-                                                                (const uint8_t*)dev_w_data,
-                                                                (const uint8_t*)dev_w_scales, (uint32_t)k, (T*)dev_dx);
-  });
-  return nz_launched();
+  return launch_tiles16<true>(cut_product16(m, k, steps * p.count), a, a_stride, m, dev_w_data, dev_w_scales, n, k,
+                              steps, p.count, k, nullptr, dev_dx, dtype, (uint8_t*)dev_workspace + p.bytes, st);
 }
 
 }  // extern "C"

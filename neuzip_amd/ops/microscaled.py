@@ -153,16 +153,33 @@ def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
     if bias is not None:
         bias = bias.contiguous()
     b = None if bias is None else bias.data_ptr()
+    room = L.nz_mx_linear_workspace_bytes(m, n, k, code)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    w = None if ws is None else ws.data_ptr()
     if isinstance(x, MXTensor):
         _call(L.nz_mx_linear_rows8, device, x.data.data_ptr(), x.scales.data_ptr(), m, k, weight.data.data_ptr(),
-              weight.scales.data_ptr(), n, b, y.data_ptr(), code, None, 0)
-        return y
-    rows = _as_rows(x, k)
-    room = L.nz_mx_linear_workspace_bytes(m, n, k)
-    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    _call(L.nz_mx_linear, device, rows.data_ptr(), code, m, k, rows.stride(0), weight.data.data_ptr(),
-          weight.scales.data_ptr(), n, b, y.data_ptr(), None if ws is None else ws.data_ptr(), room)
+              weight.scales.data_ptr(), n, b, y.data_ptr(), code, w, room)
+    else:
+        rows = _as_rows(x, k)
+        _call(L.nz_mx_linear, device, rows.data_ptr(), code, m, k, rows.stride(0), weight.data.data_ptr(),
+              weight.scales.data_ptr(), n, b, y.data_ptr(), w, room)
     return y
+
+
+def _input_gradient(grad: torch.Tensor, weight: MXTensor) -> torch.Tensor:
+    L = _lib.load()
+    n, k = weight.shape
+    device = _on_gpu(weight=weight.data, grad=grad)
+    dx = torch.empty(*grad.shape[:-1], k, dtype=grad.dtype, device=device)
+    if n == 0:  # empty sums
+        return dx.zero_()
+    go, code = _as_rows(grad, n), _dtype_code(grad.dtype)
+    args = (go.data_ptr(), code, go.shape[0], n, go.stride(0))
+    room = L.nz_mx_linear_grad_workspace_bytes(*args, k)
+    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
+    _call(L.nz_mx_linear_grad, device, *args, weight.data.data_ptr(), weight.scales.data_ptr(), k, dx.data_ptr(),
+          None if ws is None else ws.data_ptr(), room)
+    return dx
 
 
 class MicroscaledLinear(torch.autograd.Function):
@@ -178,16 +195,11 @@ class MicroscaledLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        n, k = ctx.weight.shape
         grad_x = grad_b = None
         if ctx.needs_input_grad[0]:
-            device = grad_output.device
-            go = _as_rows(grad_output, n)
-            grad_x = torch.empty(*grad_output.shape[:-1], k, dtype=grad_output.dtype, device=device)
-            _call(_lib.load().nz_mx_linear_grad, device, go.data_ptr(), _dtype_code(go.dtype), go.shape[0], n,
-                  go.stride(0), ctx.weight.data.data_ptr(), ctx.weight.scales.data_ptr(), k, grad_x.data_ptr())
+            grad_x = _input_gradient(grad_output, ctx.weight)
         if ctx.needs_input_grad[2]:
-            grad_b = grad_output.reshape(-1, n).sum(0)
+            grad_b = grad_output.reshape(-1, ctx.weight.shape[0]).sum(0)
         return grad_x, None, grad_b, None
 
 

@@ -420,3 +420,34 @@ def test_captured_calls_replay_beside_eager_ones():
         torch.cuda.synchronize()
         for a, b in zip(outs, eager):
             same(a, b)
+
+
+def test_float32_results_keep_what_is_small_beside_the_large():
+    """x: multiples of 2^-2 up to 448, w: of 2^-1 up to 6, 64 of them: products are multiples of 2^-3 below 2^12,
+    partial sums below 2^18, 21 bits: exact in 32 bits"""
+    m, n, k = 5, 40, 64
+    g = torch.Generator().manual_seed(3)
+    x = torch.randint(-15, 16, (m, k), generator=g).float() * torch.exp2(torch.randint(-2, 5, (m, k), generator=g).float())
+    x[:, 3], x[:, 40] = 448.0, -448.0
+    wd = whole_numbers(n, k, 6, 4)
+    wd[:, 3] = wd[:, 40] = 6.0
+    assert (held(x, 8) % 0.25 == 0).all() and (held(wd, 4) % 0.5 == 0).all()
+    w = ops.mx_quantize(wd.to(DEV), 4)
+    want = held(x, 8) @ held(wd, 4).t()
+    same(ops.mx_linear(x.to(DEV), w), want)
+    same(ops.mx_linear(ops.mx_quantize(x.to(DEV), 8), w, dtype=torch.float32), want)
+
+
+def test_smallest_scales_of_a_weight():
+    """blocks of subnormal weights: their scale is 2^-127"""
+    wd = torch.arange(1, 7).repeat(64)[:64 * 5].float().view(5, 64) * 2.0 ** -127
+    x = torch.full((2, 64), 2.0 ** 100)
+    w = ops.mx_quantize(wd.to(DEV), 4)
+    assert (w.scales[:, [0, 4]] == 0).all()
+    want = held(x, 8) @ held(wd, 4).t()
+    same(ops.mx_linear(x.to(DEV), w), want)
+    same(ops.mx_linear(x.to(torch.bfloat16).to(DEV), w), round_to(want, torch.bfloat16))
+    g = torch.full((3, 5), 2.0 ** 100, requires_grad=False)
+    xg = torch.zeros(3, 64, device=DEV, requires_grad=True)
+    ops.mx_linear(xg, w).backward(g.to(DEV))
+    same(xg.grad, g.double() @ held(wd, 4))

@@ -41,20 +41,27 @@ def test_refusals_of_the_abi():
     refused(L.nz_mx_lookup(p, p, 5, 1, 4, None, 3, 1.0, p, 0, None, None), A, "null indices")
     refused(L.nz_mx_lookup(p, p, 5, 1, 4, p + 4, 3, 1.0, p, 0, None, None), B, "misaligned")
     refused(L.nz_mx_lookup(p, p, 5, 1, 4, p, 3, 1.0, p, 0, p + 2, None), B, "misaligned")
-    refused(L.nz_mx_linear(p, 0, 1, 0, 1, p, p, 1, None, p, p, 1 << 30, None), A, "1 to 2^30")
+    refused(L.nz_mx_linear(p, 0, 1, 0, 1, p, p, 1, None, p, p, 1 << 30, None), A, "1 to 2^22")
     refused(L.nz_mx_linear(p, 0, 1, 32, 32, None, p, 1, None, p, p, 1 << 30, None), A, "null data")
     refused(L.nz_mx_linear(p, 0, 1, 32, 32, p, p, 1, None, None, p, 1 << 30, None), A, "null rows or output")
     refused(L.nz_mx_linear(p, 0, 1, 32, 32, p, p, 1, p + 1, p, p, 1 << 30, None), B, "aligned to their elements")
     refused(L.nz_mx_linear(p, 0, 1 << 40, 32, 32, p, p, 1, None, p, p, 1 << 30, None), A, "too many rows")
-    need = L.nz_mx_linear_workspace_bytes(1000, 512, 512)
+    need = L.nz_mx_linear_workspace_bytes(1000, 512, 512, 0)
     assert need >= 1000 * 512
     refused(L.nz_mx_linear(p, 0, 1000, 512, 512, p, p, 512, None, p, p, need - 1, None), D, "workspace")
     refused(L.nz_mx_linear(p, 0, 1000, 512, 512, p, p, 512, None, p, p + 8, need, None), B, "workspace")
     refused(L.nz_mx_linear_rows8(p, p + 4, 1, 32, p, p, 1, None, p, 0, None, 0, None), B, "16-byte aligned")
     assert L.nz_mx_linear(None, 0, 0, 32, 32, None, None, 7, None, None, None, 0, None) == _lib.OK
-    refused(L.nz_mx_linear_grad(p, 9, 1, 1, 1, p, p, 1, p, None), C, "Unsupported data type")
-    refused(L.nz_mx_linear_grad(None, 0, 1, 1, 1, p, p, 1, p, None), A, "null gradient")
-    assert L.nz_mx_linear_grad(None, 0, 0, 1, 1, None, None, 1, None, None) == _lib.OK
+    refused(L.nz_mx_linear_rows8(p, p, 1000, 512, p, p, 512, None, p, 0, p, 0, None), D, "workspace")
+    refused(L.nz_mx_linear_grad(p, 9, 1, 1, 1, p, p, 1, p, p, 1 << 30, None), C, "Unsupported data type")
+    refused(L.nz_mx_linear_grad(None, 0, 1, 1, 1, p, p, 1, p, p, 1 << 30, None), A, "null gradient")
+    refused(L.nz_mx_linear_grad(p, 0, 1, 0, 1, p, p, 1, p, p, 1 << 30, None), A, "without rows")
+    refused(L.nz_mx_linear_grad(p, 0, 1, 1 << 23, 1 << 23, p, p, 1, p, p, 1 << 30, None), A, "2^22")
+    assert L.nz_mx_linear_grad_workspace_bytes(p, 0, 100, 512, 512, 512) < 100 * 512 * 2 < (
+        L.nz_mx_linear_grad_workspace_bytes(p, 1, 100, 512, 512, 512))
+    need = L.nz_mx_linear_grad_workspace_bytes(p + 2, 0, 100, 512, 512, 512)
+    refused(L.nz_mx_linear_grad(p + 2, 0, 100, 512, 512, p, p, 512, p, p, need - 1, None), D, "workspace")
+    assert L.nz_mx_linear_grad(None, 0, 0, 1, 1, None, None, 1, None, None, 0, None) == _lib.OK
     grad = L.nz_embedding_gradient
     refused(grad(p, 1, p, 7, 1, 1, 1, 1.0, -1, 0, p, p, 1 << 30, None), C, "Unsupported data type")
     refused(grad(p, 1, p, 0, 1, 1, 1, 1.0, -1, 4, p, p, 1 << 30, None), A, "unknown flags")
