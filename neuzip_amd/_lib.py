@@ -157,7 +157,7 @@ def load() -> ctypes.CDLL:
     L.nz_mx_linear_grad_workspace_bytes.restype = u64
     L.nz_mx_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
     L.nz_embedding_gradient_workspace_bytes.restype = u64
-    L.nz_embedding_gradient_workspace_bytes.argtypes = [u64, u64, u64]
+    L.nz_embedding_gradient_workspace_bytes.argtypes = [u64, u64]
     L.nz_embedding_gradient.restype = i32
     L.nz_embedding_gradient.argtypes = [vp, u64, vp, i32, u64, u64, u64, ctypes.c_float, ctypes.c_int64, u32, vp, vp,
                                         u64, vp]

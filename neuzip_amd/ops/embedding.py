@@ -15,7 +15,7 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     ``indices`` (any shape) and multiplied by ``scale``, for the gradient ``grad``
     (``[*indices.shape, dim]``) of the rows.
 
-    Tokens are sorted, a row's gradients are added in their order in 32 bits and
+    Tokens are sorted, a row's gradients are added in a fixed order in 32 bits and
     rounded once to the type of ``grad``: the same bits every time.  The row
     ``padding_idx`` and indices outside the table take no part;
     ``scale_grad_by_freq`` divides a row's gradient by the number of its tokens.
@@ -44,7 +44,7 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     L = _lib.load()
     idx = indices.reshape(-1).to(torch.int64).contiguous()
     g = _as_rows(grad.detach(), cols)
-    room = L.nz_embedding_gradient_workspace_bytes(idx.numel(), num_embeddings, cols)
+    room = L.nz_embedding_gradient_workspace_bytes(idx.numel(), cols)
     ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
     _call(L.nz_embedding_gradient, device, idx.data_ptr(), idx.numel(), g.data_ptr(), code, g.stride(0),
           num_embeddings, cols, float(scale), -1 if padding_idx is None else padding_idx, flags, out.data_ptr(),
