@@ -2,27 +2,31 @@
 //
 // The rows of the table that no token names are most of what has to be written, so the first launch clears the table
 // while some of its workgroups sort the tokens (clearing is bound by memory, sorting by arithmetic and latency); the
-// second adds up the rows of g.  Its launches:
+// others add up the rows of g.  The launches:
 //
-//   sort   64 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller indices plus that
-//          of equal ones before it, counted by comparing with all of them from LDS: no passes, no exchange between
-//          workgroups, and the same place every time.
-//   merge  (more than one tile) the place among all tokens: the same counts in the other tiles, by bisection.
-//   sum    one wavefront per 512 columns of up to 64 tokens of a row, in their order, in float32.
-//   join   (more than 64 tokens) the pieces of rows with more than 64 tokens, in their order.
+//   sort   64 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller keys (index, then
+//          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
+//          the same place every time.
+//   merge  (more than one tile) the place among all tokens: the same count in the other tiles, by bisection.
+//   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
+//          lie in one window is done; what reaches beyond it is kept as a piece.
+//   join   (more than one window) the pieces of rows that reach over several windows, in their order.
 #include "nz_operators.h"
 
 namespace {
 
-constexpr uint32_t kTile = 8192;     // tokens that are compared with each other
-constexpr uint32_t kPiece = 64;      // tokens that one wavefront adds up
-constexpr uint32_t kNone = ~0u;      // the index of a token that takes no part
-constexpr uint32_t kClear = 1 << 16; // bytes a workgroup clears
+constexpr uint32_t kTile = 8192;      // tokens that are compared with each other
+constexpr uint32_t kTileBits = 13;
+constexpr uint32_t kClear = 1 << 16;  // bytes a workgroup clears
+constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
 
-// A token in its place: index, token, tokens of the same index before it, tokens of this index.
-typedef uint32_t Place __attribute__((ext_vector_type(4)));
+// A sorted token: its index (the number of rows if it takes no part) and where it stands.
+struct Place {
+  uint32_t row, token;
+};
 
-__global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long* index, uint32_t count, uint64_t rows,
+template <class Key>
+__global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long* index, uint32_t count, uint32_t rows,
                                                                 long long skip, Place* places, uint32_t sorters,
                                                                 uint8_t* out, uint64_t bytes) {
   if (blockIdx.x >= sorters) {  // clear
@@ -41,53 +45,44 @@ __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long*
     }
     return;
   }
-  __shared__ __attribute__((aligned(16))) uint32_t keys[kTile];
-  __shared__ uint32_t smaller[8][64], equal[8][64], before[8][64];
+  typedef Key key4 __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(32))) Key keys[kTile];
+  __shared__ uint32_t smaller[8][64];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
   const uint32_t block = blockIdx.x % (kTile / 64), base = blockIdx.x / (kTile / 64) * kTile;
   const uint32_t here = min(kTile, count - base), blocks = (here + 63) / 64;
   for (uint32_t i = threadIdx.x; i < blocks * 64; i += 512) {
     const long long v = i < here ? index[base + i] : -1;
-    keys[i] = v >= 0 && (uint64_t)v < rows && v != skip ? (uint32_t)v : kNone;
+    const uint32_t row = v >= 0 && v < (long long)rows && v != skip ? (uint32_t)v : rows;
+    keys[i] = (Key)row << kTileBits | i;
   }
   __syncthreads();
-  const uint32_t mine = keys[block * 64 + lane];
-  uint32_t lt = 0, eq = 0, eqb = 0;
+  const Key mine = keys[block * 64 + lane];
+  uint32_t less = 0;
   const uint32_t first = blocks * wave / 8, last = blocks * (wave + 1) / 8;
   for (uint32_t b = first; b < last; ++b) {
-    const uint32_t* p = keys + b * 64;
-    if (b == block) {
-      eqb = eq;
-      for (uint32_t j = 0; j < 64; ++j) {
-        const bool e = p[j] == mine;
-        lt += p[j] < mine;
-        eq += e;
-        eqb += e && j < lane;
-      }
-    } else {
 #pragma unroll
-      for (uint32_t j = 0; j < 64; j += 4) {
-        const Place k = *(const Place*)(p + j);
-        lt += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
-        eq += (k.x == mine) + (k.y == mine) + (k.z == mine) + (k.w == mine);
-      }
+    for (uint32_t j = 0; j < 64; j += 4) {
+      const key4 k = *(const key4*)(keys + b * 64 + j);
+      less += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
     }
   }
-  if (last <= block) eqb = eq;
-  smaller[wave][lane] = lt, equal[wave][lane] = eq, before[wave][lane] = eqb;
+  smaller[wave][lane] = less;
   __syncthreads();
-  if (wave || block * 64 + lane >= here) return;
-  lt = eq = eqb = 0;
-  for (uint32_t w = 0; w < 8; ++w) lt += smaller[w][lane], eq += equal[w][lane], eqb += before[w][lane];
-  places[base + lt + eqb] = Place{mine, base + block * 64 + lane, eqb, eq};
+  const uint32_t i = block * 64 + lane;
+  if (wave || i >= here) return;
+  less = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < 8; ++w) less += smaller[w][lane];
+  places[base + less] = Place{(uint32_t)(mine >> kTileBits), base + i};
 }
 
-// tokens of a sorted tile whose index is less than `key`
-__device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t key) {
+// tokens of a sorted tile whose index is less than `row`
+__device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t row) {
   uint32_t lo = 0;
   while (n) {
     const uint32_t half = n / 2;
-    if (tile[lo + half].x < key)
+    if (tile[lo + half].row < row)
       lo += half + 1, n -= half + 1;
     else
       n = half;
@@ -98,16 +93,11 @@ __device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t key) {
 __global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* tiles, uint32_t count, Place* places) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= count) return;
-  Place p = tiles[i];
-  uint32_t at = i % kTile;
-  for (uint32_t base = 0; base < count; base += kTile) {
-    if (base == i / kTile * kTile) continue;
-    const uint32_t n = min(kTile, count - base);
-    const uint32_t lt = below(tiles + base, n, p.x), eq = below(tiles + base, n, (uint64_t)p.x + 1) - lt;
-    at += lt;
-    p.w += eq;
-    if (base < i) at += eq, p.z += eq;
-  }
+  const Place p = tiles[i];
+  const uint32_t own = i / kTile * kTile;
+  uint32_t at = i - own;
+  for (uint32_t base = 0; base < count; base += kTile)  // equal ones of the tiles before stand before
+    if (base != own) at += below(tiles + base, min(kTile, count - base), (uint64_t)p.row + (base < own));
   places[at] = p;
 }
 
@@ -116,109 +106,177 @@ struct Pack {
   typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
+// The 8 columns a lane works on: from `c` as loaded (all inside the row, or the row has fewer than 8), of which those
+// from `from` on, `n` of them, are its own.  The last lane of a row whose width is no multiple of 8 begins earlier
+// than its own columns do, so that every load is a whole one.
+struct Columns {
+  uint32_t c, from, n;
+  bool whole;
+};
+__device__ inline Columns columns_of(uint32_t slice, uint32_t lane, uint32_t cols) {
+  const uint32_t own = slice * 512 + lane * 8;
+  Columns k;
+  k.whole = cols >= 8;
+  k.c = k.whole ? min(own, cols - 8) : 0;
+  k.from = own - k.c;
+  k.n = own < cols ? min(8u, cols - own) : 0;
+  return k;
+}
+
 template <class T>
-__device__ inline void add8(const T* p, uint32_t n, float (&sum)[8]) {
-  if (n >= 8) {
-    const typename Pack<T>::type v = *(const typename Pack<T>::type*)p;
+__device__ inline void load8(const T* row, const Columns& k, uint32_t cols, float (&v)[8]) {
+  if (k.whole) {
+    const typename Pack<T>::type a = *(const typename Pack<T>::type*)(row + k.c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += (float)v[i];
+    for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (uint32_t)i < cols ? (float)row[i] : 0.0f;
+  }
+}
+
+template <class T>
+__device__ inline void store8(T* row, const Columns& k, const float (&v)[8]) {
+  if (k.n == 8) {
+    typename Pack<T>::type a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+    *(typename Pack<T>::type*)(row + k.c) = a;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if ((uint32_t)i < n) sum[i] += (float)p[i];
+      if (i >= (int)k.from && i < (int)(k.from + k.n)) row[k.c + i] = (T)v[i];
   }
 }
 
 // 8 sums of a row with `tokens` tokens into the table
 template <class T>
-__device__ inline void put8(T* q, uint32_t n, const float (&sum)[8], uint32_t tokens, float scale, uint32_t flags) {
+__device__ inline void put8(T* row, const Columns& k, uint32_t cols, const float (&sum)[8], uint32_t tokens,
+                            float scale, uint32_t flags) {
   const float f = flags & NZ_GRAD_BY_FREQUENCY ? scale / (float)tokens : scale;
-  float v[8];
+  float v[8], old[8] = {};
+  if (flags & NZ_GRAD_ACCUMULATE) load8(row, k, cols, old);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = sum[i] * f;
-  if (flags & NZ_GRAD_ACCUMULATE) add8(q, n, v);
-  if (n >= 8) {
-    typename Pack<T>::type a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
-    *(typename Pack<T>::type*)q = a;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if ((uint32_t)i < n) q[i] = (T)v[i];
-  }
+  for (int i = 0; i < 8; ++i) v[i] = old[i] + sum[i] * f;
+  store8(row, k, v);
 }
 
-// Where a piece that begins at place i is kept: of the places i / 64 * 64 .. + 63, at most one begins a row of more
-// than 64 tokens, and at most one a later piece of such a row.
-__device__ inline uint64_t piece_at(uint32_t i, uint32_t before) { return (uint64_t)(i / kPiece) * 2 + (before == 0); }
+// Of a window, at most one row began before it (piece 0) and one begins in it and goes on behind it (piece 1).
+__device__ inline uint64_t piece_at(uint64_t window, uint32_t which, uint32_t cols) {
+  return (window * 2 + which) * cols;
+}
 
 template <class T>
-__global__ __launch_bounds__(256) void nz_embedding_sum_kernel(const Place* places, uint32_t count, const T* g,
-                                                               uint64_t stride, uint32_t cols, uint32_t slices,
-                                                               float scale, uint32_t flags, T* out, float* pieces) {
+__global__ __launch_bounds__(256) void nz_embedding_sum_kernel(const Place* places, uint32_t count, uint32_t rows,
+                                                               uint32_t size, const T* g, uint64_t stride,
+                                                               uint32_t cols, uint32_t slices, float scale,
+                                                               uint32_t flags, T* out, float* pieces) {
   const uint64_t id = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const uint32_t i = (uint32_t)(id / slices), lane = threadIdx.x & 63;
-  if (i >= count) return;
-  const Place p = places[i];
-  if (p.x == kNone || p.z % kPiece) return;
-  const uint32_t c = (uint32_t)(id % slices) * 512 + lane * 8;
-  const uint32_t n = c < cols ? cols - c : 0, tokens = min(kPiece, p.w - p.z);
-  const uint32_t token = places[min(i + lane, count - 1)].y;
+  const uint64_t window = id / slices, first = window * size;
+  if (first >= count) return;
+  const uint32_t lane = threadIdx.x & 63, end = (uint32_t)min((uint64_t)count, first + size);
+  const Columns k = columns_of((uint32_t)(id - window * slices), lane, cols);
   float sum[8] = {};
-  uint32_t t = 0;
-  for (; t + 8 <= tokens; t += 8) {  // eight rows on their way at a time, added one after the other
-    float v[8][8] = {};
+  uint32_t tokens = 0;
+  bool begun = first == 0 || places[first - 1].row != places[first].row;  // the row being added up: in this window
+  for (uint32_t at = (uint32_t)first; at < end; at += kBatch) {
+    // lanes 0 .. 15: the places of the batch; lanes 1 .. 16 look at the one behind each
+    const Place mine = places[min(at + lane, count - 1)];
+    typename Pack<T>::type v[kBatch];
+    float w[kBatch][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) add8(g + __builtin_amdgcn_readlane(token, t + j) * stride + c, n, v[j]);
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const T* row = g + __builtin_amdgcn_readlane(mine.token, j) * stride;
+      if (k.whole)
+        v[j] = *(const typename Pack<T>::type*)(row + k.c);
+      else
+        load8(row, k, cols, w[j]);
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      if (at + j >= end) break;
+      const uint32_t row = __builtin_amdgcn_readlane(mine.row, j);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += v[j][e];
-  }
-  for (; t < tokens; ++t) add8(g + __builtin_amdgcn_readlane(token, t) * stride + c, n, sum);
-  if (p.w <= kPiece) {
-    if (n) put8(out + p.x * (uint64_t)cols + c, n, sum, p.w, scale, flags);
-  } else {
-    float* q = pieces + piece_at(i, p.z) * cols + c;
+      for (int e = 0; e < 8; ++e) sum[e] += k.whole ? (float)v[j][e] : w[j][e];
+      ++tokens;
+      const bool ends = at + j + 1 == count || __builtin_amdgcn_readlane(mine.row, j + 1) != row;
+      if (!ends && at + j + 1 < end) continue;
+      if (row != rows && k.n) {
+        if (begun && ends)
+          put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
+        else
+          store8(pieces + piece_at(window, begun, cols), k, sum);
+      }
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if ((uint32_t)e < n) q[e] = sum[e];
+      for (int e = 0; e < 8; ++e) sum[e] = 0;
+      tokens = 0;
+      begun = true;
+    }
   }
 }
 
-// One wavefront per 512 columns and 64 places: at most one row of more than 64 tokens begins there.
+// One wavefront per 512 columns and window: the row that begins in it and goes on behind it, if there is one.
 template <class T>
-__global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* places, uint32_t count, uint32_t cols,
-                                                                uint32_t slices, float scale, uint32_t flags, T* out,
+__global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* places, uint32_t count, uint32_t rows,
+                                                                uint32_t size, uint32_t cols, uint32_t slices,
+                                                                float scale, uint32_t flags, T* out,
                                                                 const float* pieces) {
   const uint64_t id = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const uint64_t from = id / slices * kPiece;
-  const uint32_t lane = threadIdx.x & 63;
-  if (from >= count) return;
-  const Place mine = places[min((uint32_t)from + lane, count - 1)];
-  const uint64_t heads = __ballot(from + lane < count && mine.x != kNone && mine.z == 0 && mine.w > kPiece);
-  if (!heads) return;
-  const uint32_t i = (uint32_t)from + __builtin_ctzll(heads);
-  const Place p = places[i];
-  const uint32_t c = (uint32_t)(id % slices) * 512 + lane * 8;
-  if (c >= cols) return;
-  float sum[8] = {};
-  for (uint32_t t = 0; t < p.w; t += kPiece) add8(pieces + piece_at(i + t, t) * cols + c, cols - c, sum);
-  put8(out + p.x * (uint64_t)cols + c, cols - c, sum, p.w, scale, flags);
+  const uint64_t window = id / slices, first = window * size, next = first + size;
+  if (next >= count) return;
+  const uint32_t row = places[next - 1].row, lane = threadIdx.x & 63;
+  if (row == rows || places[next].row != row) return;
+  if (places[first].row == row && first && places[first - 1].row == row) return;  // it began before
+  uint32_t more = 0;  // windows that it goes on in
+  for (;;) {
+    const uint64_t at = next + (uint64_t)(more + lane) * size;
+    const uint64_t other = __ballot(at >= count || places[min(at, (uint64_t)count - 1)].row != row);
+    if (other) {
+      more += __builtin_ctzll(other);
+      break;
+    }
+    more += 64;
+  }
+  uint32_t tokens = 1;
+  if (flags & NZ_GRAD_BY_FREQUENCY) {
+    tokens = (more - 1) * size;
+    for (uint32_t i = 0; i < size; i += 64) {  // of the first window and of the last one
+      tokens += __popcll(__ballot(i + lane < size && places[first + min(i + lane, size - 1)].row == row));
+      const uint64_t at = next + (uint64_t)(more - 1) * size + i + lane;
+      tokens += __popcll(__ballot(i + lane < size && at < count && places[min(at, (uint64_t)count - 1)].row == row));
+    }
+  }
+  const Columns k = columns_of((uint32_t)(id - window * slices), lane, cols);
+  float sum[8];
+  load8(pieces + piece_at(window, 1, cols), k, cols, sum);
+  for (uint32_t q = 1; q <= more; q += 8) {
+    float v[8][8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)  // the last piece again where there are fewer
+      load8(pieces + piece_at(window + min(q + j, more), 0, cols), k, cols, v[j]);
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = q + j <= more ? sum[e] + v[j][e] : sum[e];
+  }
+  if (k.n) put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+// Places a window holds: few while there are few tokens, for the sake of many wavefronts.
+uint32_t window_of(uint64_t count) { return count <= 32768 ? kBatch : 4 * kBatch; }
 
 // Where the workspace holds what: sorted tiles (more than one), places, pieces.
 struct Room {
   uint64_t places, pieces, bytes;
 };
 Room room_of(uint64_t count, uint64_t cols) {
+  const uint64_t window = window_of(count);
   Room r;
   r.places = count > kTile ? align256(count * sizeof(Place)) : 0;
   r.pieces = r.places + align256(count * sizeof(Place));
-  r.bytes = r.pieces + (count > kPiece ? nz_mul(nz_ceil_div(count, kPiece) * 2 * 4, cols) : 0);
+  r.bytes = r.pieces + (count > window ? nz_mul(nz_ceil_div(count, window) * 2 * 4, cols) : 0);
   return r;
 }
 
@@ -255,21 +313,29 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)dev_workspace;
   Place *places = (Place*)(ws + room.places), *tiles = (Place*)ws;
-  nz_embedding_sort_kernel<<<(uint32_t)clearers + sorters, 512, 0, st>>>(
-      (const long long*)dev_indices, (uint32_t)count, rows, padding_idx, count > kTile ? tiles : places, sorters,
-      (uint8_t*)dev_out, bytes);
+  Place* sorted = count > kTile ? tiles : places;
+  const dim3 grid((uint32_t)clearers + sorters);
+  if (rows < 1u << (32 - kTileBits))
+    nz_embedding_sort_kernel<uint32_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
+                                                             (uint32_t)rows, padding_idx, sorted, sorters,
+                                                             (uint8_t*)dev_out, bytes);
+  else
+    nz_embedding_sort_kernel<uint64_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
+                                                             (uint32_t)rows, padding_idx, sorted, sorters,
+                                                             (uint8_t*)dev_out, bytes);
   if (count > kTile)
     nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 256), 256, 0, st>>>(tiles, (uint32_t)count, places);
   if (count) {
     float* pieces = (float*)(ws + room.pieces);
-    const uint32_t sums = (uint32_t)nz_ceil_div(count * slices, 4);
-    const uint32_t joins = (uint32_t)nz_ceil_div(nz_ceil_div(count, kPiece) * slices, 4);
-#define NZ_GRADIENT(T)                                                                                            \
-  nz_embedding_sum_kernel<T><<<sums, 256, 0, st>>>(places, (uint32_t)count, (const T*)dev_g, stride, (uint32_t)cols, \
-                                                   (uint32_t)slices, scale, flags, (T*)dev_out, pieces);          \
-  if (count > kPiece)                                                                                             \
-  nz_embedding_join_kernel<T><<<joins, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)cols, (uint32_t)slices,   \
-                                                     scale, flags, (T*)dev_out, pieces)
+    const uint32_t window = window_of(count);
+    const uint32_t waves = (uint32_t)nz_ceil_div(nz_ceil_div(count, window) * slices, 4);
+#define NZ_GRADIENT(T)                                                                                               \
+  nz_embedding_sum_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (const T*)dev_g, \
+                                                    stride, (uint32_t)cols, (uint32_t)slices, scale, flags,          \
+                                                    (T*)dev_out, pieces);                                            \
+  if (count > window)                                                                                                \
+  nz_embedding_join_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (uint32_t)cols, \
+                                                     (uint32_t)slices, scale, flags, (T*)dev_out, pieces)
     if (dtype == NZ_DTYPE_BF16) {
       NZ_GRADIENT(nz_bf16);
     } else if (dtype == NZ_DTYPE_F16) {

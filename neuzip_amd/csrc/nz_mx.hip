@@ -598,7 +598,8 @@ __global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t 
 // Steps of 64 values.  A is staged three deep by loads that go to LDS without registers (16-byte chunk c of a row at
 // c ^ (row & 7)); the weight is loaded as codes two steps ahead and written to LDS as bf16 one step ahead.  Where the
 // sums run over the weight's rows its tile lies in LDS as in memory, and the operand is read by the instruction that
-// transposes 4 x 16 values on the way; its rows exchange 8-byte slots (slot ^ (row & 3)) against bank conflicts.
+// transposes 4 x 16 values on the way; its rows exchange 8-byte slots (slot ^ (row & 7)) against bank conflicts of
+// the writes and of the reads.
 // A lane ends with 4 TN consecutive columns, as in nz_mx_tiles_kernel.
 template <int WM, int WN, int TM, int TN, bool ROWS, class T>
 __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf16* a, uint64_t a_stride, uint32_t m,
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf
       const i4v v = __builtin_bit_cast(i4v, bf16_of_codes(codes[j], scale));
       const uint32_t chunk = l_at / 8 + j;
       if constexpr (ROWS)
-        *(i4v*)(to + (chunk ^ (l_row >> 1 & 1)) * 16) = l_row & 1 ? i4v{v.z, v.w, v.x, v.y} : v;
+        *(i4v*)(to + (chunk ^ (l_row >> 1 & 3)) * 16) = l_row & 1 ? i4v{v.z, v.w, v.x, v.y} : v;
       else
         *(i4v*)(to + (chunk ^ (l_row & 7)) * 16) = v;
     }
@@ -696,7 +697,7 @@ __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf
           s4v half[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const uint32_t row = h * 32 + g * 8 + q * 4 + r / 4, slot = (wn * TN * 4 + r % 4 * TN + j) ^ (r / 4);
+            const uint32_t row = h * 32 + g * 8 + q * 4 + r / 4, slot = (wn * TN * 4 + r % 4 * TN + j) ^ (q * 4 + r / 4);
             half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s4v*)(pb + row * (BN * 2) + slot * 8));
           }

@@ -6,7 +6,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from neuzip_amd import _lib
-from neuzip_amd.ops.microscaled import _as_rows, _call, _dtype_code, _on_gpu
+from neuzip_amd.ops.microscaled import _as_rows, _call, _dtype_code, _on_gpu, _workspace
 
 
 def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings: int, scale: float = 1.0,
@@ -32,23 +32,24 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
             raise ValueError("padding_idx must be within num_embeddings")
         padding_idx %= num_embeddings
     code = _dtype_code(grad.dtype)
-    device = _on_gpu(grad=grad, indices=indices, out=out)
+    index = _on_gpu(grad=grad, indices=indices, out=out)
     cols = grad.shape[-1]
     flags = _lib.GRAD_BY_FREQUENCY if scale_grad_by_freq else 0
     if out is None:
-        out = torch.empty(num_embeddings, cols, dtype=grad.dtype, device=device)
+        out = grad.new_empty((num_embeddings, cols))
     else:
         if tuple(out.shape) != (num_embeddings, cols) or out.dtype != grad.dtype or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {grad.dtype} tensor of shape {(num_embeddings, cols)}")
         flags |= _lib.GRAD_ACCUMULATE
     L = _lib.load()
-    idx = indices.reshape(-1).to(torch.int64).contiguous()
-    g = _as_rows(grad.detach(), cols)
-    room = L.nz_embedding_gradient_workspace_bytes(idx.numel(), cols)
-    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    _call(L.nz_embedding_gradient, device, idx.data_ptr(), idx.numel(), g.data_ptr(), code, g.stride(0),
-          num_embeddings, cols, float(scale), -1 if padding_idx is None else padding_idx, flags, out.data_ptr(),
-          None if ws is None else ws.data_ptr(), room)
+    idx = indices if indices.dtype == torch.int64 else indices.to(torch.int64)
+    idx = idx.contiguous()
+    count = idx.numel()
+    g, _, stride = _as_rows(grad, cols)
+    room = L.nz_embedding_gradient_workspace_bytes(count, cols)
+    ws, at = _workspace(room, g)
+    _call(L.nz_embedding_gradient, index, idx.data_ptr(), count, g.data_ptr(), code, stride, num_embeddings, cols,
+          float(scale), -1 if padding_idx is None else padding_idx, flags, out.data_ptr(), at, room)
     return out
 
 

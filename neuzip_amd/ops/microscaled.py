@@ -29,36 +29,55 @@ def _dtype_code(dtype: torch.dtype) -> int:
     return code
 
 
-def _on_gpu(**tensors) -> torch.device:
-    """The device that all of ``tensors`` (None aside) are on, which has to be a GPU."""
-    device = None
+# These calls take a few microseconds on the device: what surrounds them is kept short as well.  (The stream's
+# address and the current device are asked for directly, 2 us less a call than through torch.cuda.)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _on_gpu(**tensors) -> int:
+    """The index of the device that all of ``tensors`` (None aside) are on, which has to be a GPU."""
+    index = None
     for name, t in tensors.items():
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise ValueError(f"{name} must be on the GPU")
-        if device is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device} like the tensors before it")
-        device = t.device
-    return device
+        if index is not None and at != index:
+            raise ValueError(f"{name} is on {t.device}, not on cuda:{index} like the tensors before it")
+        index = at
+    return index
 
 
-def _call(fn, device: torch.device, *args) -> None:
-    """Make a native call on the current stream of ``device``."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call(fn, index: int, *args) -> None:
+    """Make a native call on the current stream of device ``index``."""
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:  # a launch goes to the device that is current
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.raise_for(rc)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.raise_for(rc)
 
 
-def _as_rows(t: torch.Tensor, width: int) -> torch.Tensor:
-    """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it)."""
-    rows = t.reshape(-1, width) if width else t.reshape(math.prod(t.shape[:-1]), 0)
-    if rows.stride(1) != 1 and width > 1 or rows.stride(0) < 0:
+def _as_rows(t: torch.Tensor, width: int):
+    """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it): the
+    tensor, its rows, elements from row to row."""
+    if t.is_contiguous():
+        return t, t.numel() // width if width else math.prod(t.shape[:-1]), width
+    rows = t.reshape(-1, width)
+    if rows.stride(1) != 1 and width > 1:
         rows = rows.contiguous()
-    return rows
+    return rows, rows.shape[0], rows.stride(0)
+
+
+def _workspace(room: int, like: torch.Tensor):
+    """(the tensor that keeps it, its address)"""
+    if not room:
+        return None, None
+    ws = like.new_empty(room, dtype=torch.uint8)
+    return ws, ws.data_ptr()
 
 
 class MXTensor:
@@ -86,6 +105,13 @@ class MXTensor:
             raise ValueError("data and scales must be on one device")
         self.data, self.scales, self.shape, self.bits = data, scales, shape, bits
 
+    @classmethod
+    def _of(cls, data, scales, shape, bits) -> "MXTensor":
+        """the same of tensors that are known to fit"""
+        self = object.__new__(cls)
+        self.data, self.scales, self.shape, self.bits = data, scales, shape, bits
+        return self
+
     @property
     def device(self) -> torch.device:
         return self.data.device
@@ -101,9 +127,10 @@ class MXTensor:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values as a dense tensor (bfloat16 holds all of them without rounding, subnormals aside)."""
         code = _dtype_code(dtype)
-        device = _on_gpu(data=self.data)
-        out = torch.empty(self.shape, dtype=dtype, device=device)
-        _call(_lib.load().nz_mx_dequantize, device, self.data.data_ptr(), self.scales.data_ptr(), self.data.shape[0],
+        data = self.data
+        index = _on_gpu(data=data)
+        out = data.new_empty(self.shape, dtype=dtype)
+        _call(_lib.load().nz_mx_dequantize, index, data.data_ptr(), self.scales.data_ptr(), data.shape[0],
               self.shape[-1], self.bits, out.data_ptr(), code)
         return out
 
@@ -119,17 +146,16 @@ def mx_quantize(x: torch.Tensor, bits: int = 4) -> MXTensor:
     if bits not in (4, 8):
         raise ValueError("bits must be 4 or 8")
     code = _dtype_code(x.dtype)
-    device = _on_gpu(x=x)
-    if x.dim() < 1:
+    index = _on_gpu(x=x)
+    shape = x.shape
+    if not shape:
         raise ValueError("x must have one dimension at least")
-    L, cols = _lib.load(), x.shape[-1]
-    rows = _as_rows(x.detach(), cols)
-    n = rows.shape[0]
-    data = torch.empty((n, L.nz_mx_row_bytes(cols, bits)), dtype=torch.uint8, device=device)
-    scales = torch.empty((n, L.nz_mx_scale_bytes(cols)), dtype=torch.uint8, device=device)
-    _call(L.nz_mx_quantize, device, rows.data_ptr(), code, n, cols, rows.stride(0), bits, data.data_ptr(),
-          scales.data_ptr())
-    return MXTensor(data, scales, x.shape, bits)
+    L, cols = _lib.load(), shape[-1]
+    rows, n, stride = _as_rows(x, cols)
+    data = x.new_empty((n, L.nz_mx_row_bytes(cols, bits)), dtype=torch.uint8)
+    scales = x.new_empty((n, L.nz_mx_scale_bytes(cols)), dtype=torch.uint8)
+    _call(L.nz_mx_quantize, index, rows.data_ptr(), code, n, cols, stride, bits, data.data_ptr(), scales.data_ptr())
+    return MXTensor._of(data, scales, shape, bits)
 
 
 def _check_weight(weight) -> None:
@@ -140,45 +166,45 @@ def _check_weight(weight) -> None:
 def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
     L = _lib.load()
     n, k = weight.shape
-    shape = x.shape[:-1]
-    m = math.prod(shape)
-    code = _dtype_code(dtype)
-    if isinstance(x, MXTensor):
-        device = _on_gpu(x=x.data, weight=weight.data, bias=bias)
-    else:
-        device = _on_gpu(x=x, weight=weight.data, bias=bias)
-    y = torch.empty(*shape, n, dtype=dtype, device=device)
+    code, wd = _dtype_code(dtype), weight.data
+    held = isinstance(x, MXTensor)
+    xt = x.data if held else x
+    index = _on_gpu(x=xt, weight=wd, bias=bias)
+    y = xt.new_empty((*x.shape[:-1], n), dtype=dtype)
     if k == 0:  # empty sums
         return y.copy_(bias) if bias is not None else y.zero_()
+    b = None
     if bias is not None:
         bias = bias.contiguous()
-    b = None if bias is None else bias.data_ptr()
-    room = L.nz_mx_linear_workspace_bytes(m, n, k, code)
-    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    w = None if ws is None else ws.data_ptr()
-    if isinstance(x, MXTensor):
-        _call(L.nz_mx_linear_rows8, device, x.data.data_ptr(), x.scales.data_ptr(), m, k, weight.data.data_ptr(),
-              weight.scales.data_ptr(), n, b, y.data_ptr(), code, w, room)
+        b = bias.data_ptr()
+    if held:
+        m = xt.shape[0]
     else:
-        rows = _as_rows(x, k)
-        _call(L.nz_mx_linear, device, rows.data_ptr(), code, m, k, rows.stride(0), weight.data.data_ptr(),
-              weight.scales.data_ptr(), n, b, y.data_ptr(), w, room)
+        xt, m, stride = _as_rows(x, k)
+    room = L.nz_mx_linear_workspace_bytes(m, n, k, code)
+    ws, at = _workspace(room, xt)
+    if held:
+        _call(L.nz_mx_linear_rows8, index, xt.data_ptr(), x.scales.data_ptr(), m, k, wd.data_ptr(),
+              weight.scales.data_ptr(), n, b, y.data_ptr(), code, at, room)
+    else:
+        _call(L.nz_mx_linear, index, xt.data_ptr(), code, m, k, stride, wd.data_ptr(), weight.scales.data_ptr(), n, b,
+              y.data_ptr(), at, room)
     return y
 
 
 def _input_gradient(grad: torch.Tensor, weight: MXTensor) -> torch.Tensor:
     L = _lib.load()
     n, k = weight.shape
-    device = _on_gpu(weight=weight.data, grad=grad)
-    dx = torch.empty(*grad.shape[:-1], k, dtype=grad.dtype, device=device)
+    index = _on_gpu(weight=weight.data, grad=grad)
+    dx = grad.new_empty((*grad.shape[:-1], k))
     if n == 0:  # empty sums
         return dx.zero_()
-    go, code = _as_rows(grad, n), _dtype_code(grad.dtype)
-    args = (go.data_ptr(), code, go.shape[0], n, go.stride(0))
+    rows, m, stride = _as_rows(grad, n)
+    args = (rows.data_ptr(), _dtype_code(grad.dtype), m, n, stride)
     room = L.nz_mx_linear_grad_workspace_bytes(*args, k)
-    ws = torch.empty(room, dtype=torch.uint8, device=device) if room else None
-    _call(L.nz_mx_linear_grad, device, *args, weight.data.data_ptr(), weight.scales.data_ptr(), k, dx.data_ptr(),
-          None if ws is None else ws.data_ptr(), room)
+    ws, at = _workspace(room, rows)
+    _call(L.nz_mx_linear_grad, index, *args, weight.data.data_ptr(), weight.scales.data_ptr(), k, dx.data_ptr(), at,
+          room)
     return dx
 
 
@@ -244,13 +270,17 @@ def mx_embedding(indices: torch.Tensor, table: MXTensor, scale: float = 1.0, dty
     if indices.dtype not in (torch.int64, torch.int32):
         raise ValueError("indices must be int64 or int32")
     code = _dtype_code(dtype)
-    device = _on_gpu(table=table.data, indices=indices, status=status)
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
-        raise ValueError("status must be an int32 tensor of one element")
-    idx = indices.reshape(-1).to(torch.int64).contiguous()
+    data = table.data
+    index = _on_gpu(table=data, indices=indices, status=status)
+    at = None
+    if status is not None:
+        if status.dtype != torch.int32 or status.numel() != 1:
+            raise ValueError("status must be an int32 tensor of one element")
+        at = status.data_ptr()
+    idx = indices if indices.dtype == torch.int64 else indices.to(torch.int64)
+    idx = idx.contiguous()
     rows, cols = table.shape
-    out = torch.empty(*indices.shape, cols, dtype=dtype, device=device)
-    _call(_lib.load().nz_mx_lookup, device, table.data.data_ptr(), table.scales.data_ptr(), rows, cols, table.bits,
-          idx.data_ptr(), idx.numel(), float(scale), out.data_ptr(), code,
-          None if status is None else status.data_ptr())
+    out = data.new_empty((*indices.shape, cols), dtype=dtype)
+    _call(_lib.load().nz_mx_lookup, index, data.data_ptr(), table.scales.data_ptr(), rows, cols, table.bits,
+          idx.data_ptr(), idx.numel(), float(scale), out.data_ptr(), code, at)
     return out
