@@ -218,10 +218,21 @@ __device__ inline f4 step(i4v w, i4v x0, i4v x1, f4 acc, uint32_t sw, uint32_t s
   }
 }
 
-// 16 bytes of every lane to LDS: lane l's to `to` (the same for all lanes) + 16 l.
-__device__ inline void to_lds16(const uint8_t* from, uint8_t* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// 16 (4) bytes of every lane to LDS: lane l's to `to` (an LDS address, the same for all lanes) + 16 l (4 l), from
+// `from`, the same for all lanes, + `offset`.  In assembly because the compiler, where it knows of such loads, waits
+// for all of them in front of other reads of LDS, the next steps' loads among them.  It has no register to give to
+// anything else too early, the kernels count these loads themselves (wait_loads), and nothing else here uses m0.
+__device__ inline void to_lds16(const uint8_t* from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
+               : "memory");
+}
+__device__ inline void to_lds4(const uint8_t* from, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from)
+               : "memory");
+}
+
+__device__ inline uint32_t lds_address(uint8_t* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)p;
 }
 
 // Wait until all but the last N loads of this wavefront have arrived.
@@ -310,7 +321,7 @@ __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint32_t m, uint32_t n, ui
 // a wavefront are staged in an order that leaves each lane 4 TN consecutive columns of the result.  Scales are
 // staged once per 512 values.
 template <int WM, int WN, int TM, int TN, int NS, class T>
-__global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles_kernel(const uint8_t* xd, const uint8_t* xs, uint32_t m,
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_mx_tiles_kernel(const uint8_t* xd, const uint8_t* xs, uint32_t m,
                                                                    const uint8_t* wd, const uint8_t* ws, uint32_t n,
                                                                    uint32_t k, const T* bias, T* y, uint32_t mt,
                                                                    uint32_t nt, uint32_t part_groups, float* part) {
@@ -321,7 +332,9 @@ __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles_kernel(const uint8_t
   static_assert(XI * 8 * W == BM && WI * 16 * W == BN && SI <= W, "loads per wavefront");
   static_assert(NS >= 3 && NS <= 8, "two buffers of scales reach 8 stages");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + 2 * SB];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+  const uint32_t base = lds_address(lds);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t r = lane & 15, g = lane / 16;
   const uint32_t all_steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
   const uint32_t from = blockIdx.y * part_groups, steps = min(all_steps - from * 4, part_groups * 4);
   uint32_t tm, tn;
@@ -343,19 +356,21 @@ __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles_kernel(const uint8_t
   for (int i = 0; i < WI; ++i)
     wo[i] = min(column((wave * WI + i) * 16 + lane / 4), n_last) * (all_steps * 64) +
             ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
-  const uint32_t si = wave % SI, srow = min(si * 64 + lane, BM + BN - 1u);  // more wavefronts than loads: some load the same
-  const uint8_t* sb = (srow < BM ? xs + ((uint64_t)m0 + min(srow, m_last)) * (groups * 16ull)
-                                 : ws + ((uint64_t)n0 + min(column(srow - BM), n_last)) * (groups * 16ull)) +
+  // more wavefronts than loads of scales: some load the same
+  const uint32_t si = wave % SI, srow = min(si * 64 + lane, BM + BN - 1u);
+  const uint8_t* sb = (si * 64 < BM ? xs + (uint64_t)m0 * (groups * 16ull) : ws + (uint64_t)n0 * (groups * 16ull)) +
                       from * 16;
+  static_assert(BM % 64 == 0, "a load takes scales of one side");
+  const uint32_t so = (srow < BM ? min(srow, m_last) : min(column(srow - BM), n_last)) * (groups * 16);
   uint32_t sbuf = 0;
   const auto load_stage = [&](uint32_t s, uint32_t buf, bool scales) {
     s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
-    uint8_t* to = lds + buf * STAGE;
+    const uint32_t to = base + buf * STAGE;
 #pragma unroll
-    for (int i = 0; i < XI; ++i) to_lds16(xb + s * 128ull + xo[i], to + (wave * XI + i) * 1024);
+    for (int i = 0; i < XI; ++i) to_lds16(xb + s * 128ull, xo[i], to + (wave * XI + i) * 1024);
 #pragma unroll
-    for (int i = 0; i < WI; ++i) to_lds16(wb + s * 64ull + wo[i], to + XB + (wave * WI + i) * 1024);
-    if (scales) to_lds16(sb + (s >> 2) * 16, lds + NS * STAGE + sbuf * SB + si * 1024), sbuf ^= 1;
+    for (int i = 0; i < WI; ++i) to_lds16(wb + s * 64ull, wo[i], to + XB + (wave * WI + i) * 1024);
+    if (scales) to_lds16(sb + (s >> 2) * 16, so, base + NS * STAGE + sbuf * SB + si * 1024), sbuf ^= 1;
   };
 
   const uint32_t wm = wave % WM, wn = wave / WM;
@@ -595,72 +610,89 @@ __global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t 
 // A tile of C[m][cols] = sum over c of A[m][c] B(c, col), c running `planes` times through the summed axis.
 // ROWS: B(c, col) = w[c][col], the gradient; else w[col][c], the product itself.
 //
-// Steps of 64 values.  A is staged three deep by loads that go to LDS without registers (16-byte chunk c of a row at
-// c ^ (row & 7)); the weight is loaded as codes two steps ahead and written to LDS as bf16 one step ahead.  Where the
-// sums run over the weight's rows its tile lies in LDS as in memory, and the operand is read by the instruction that
-// transposes 4 x 16 values on the way; its rows exchange 8-byte slots (slot ^ (row & 7)) against bank conflicts of
-// the writes and of the reads.
-// A lane ends with 4 TN consecutive columns, as in nz_mx_tiles_kernel.
+// Steps of 64 values.  Rows of A, codes and scales go to LDS without registers two steps ahead (16-byte chunk c of a
+// row of A at c ^ (row & 7)); a step ahead, the codes are written to LDS once more as bf16, once for all wavefronts.
+// Where the sums run over the weight's rows that tile lies as in memory, and the operand is read by the instruction
+// that transposes 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns, as in nz_mx_tiles_kernel.
 template <int WM, int WN, int TM, int TN, bool ROWS, class T>
-__global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf16* a, uint64_t a_stride, uint32_t m,
-                                                                     const uint8_t* wd, const uint8_t* ws,
-                                                                     uint32_t w_rows, uint32_t w_cols, uint32_t steps_1,
-                                                                     uint32_t planes, uint32_t cols, const T* bias,
-                                                                     T* y, uint32_t mt, uint32_t nt,
-                                                                     uint32_t part_steps, float* part) {
-  constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
-  constexpr int AB = BM * 128, BB = BN * 128, XI = BM / 8 / W;
-  constexpr int CW = BN / (8 * W), CODES = 8 * CW;  // words and codes of the weight, per lane and step
-  static_assert(XI * 8 * W == BM && CW * 8 * W == BN && (CW == 2 || CW == 4), "loads per wavefront");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * AB + 2 * BB];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_mx_tiles16_kernel(
+    const nz_bf16* a, uint64_t a_stride, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t w_rows,
+    uint32_t w_cols, uint32_t steps_1, uint32_t planes, uint32_t cols, const T* bias, T* y, uint32_t mt, uint32_t nt,
+    uint32_t part_steps, float* part) {
+  constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16, XI = BM / 8 / W, ROW = ROWS ? BN : 64;
+  constexpr int AB = BM * 128, BB = BN * 128, CB = BN * 32, SB = BN * 8;  // bytes a step: A, bf16, codes, scales
+  constexpr int B_AT = 3 * AB, C_AT = B_AT + 2 * BB, S_AT = C_AT + 3 * CB, LOADS = XI + 2;
+  static_assert(XI * 8 * W == BM && BN * 64 == 16 * 64 * W, "16 rows of A and 16 codes per lane");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[S_AT + 3 * SB];
+  const uint32_t base = lds_address(lds);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t r = lane & 15, g = lane / 16;
   const uint32_t from = blockIdx.y * part_steps, steps = min(steps_1 * planes - from, part_steps);
   const uint32_t w_steps = (w_cols + kStep - 1) / kStep, w_groups = (w_cols + kGroup - 1) / kGroup;
+  const uint32_t w_bytes = w_steps * 64, s_bytes = w_groups * 16;
   uint32_t tm, tn;
   tile_of(blockIdx.x, mt, nt, tm, tn);
   const uint32_t m0 = tm * BM, n0 = tn * BN, m_last = min((uint32_t)BM, m - m0) - 1;
 
+  // Loads: a base of the workgroup, moved from step to step, and an offset of the lane.
   const uint8_t* ab = (const uint8_t*)(a + (uint64_t)m0 * a_stride) + from * 128ull;
   uint32_t ao[XI];
 #pragma unroll
   for (int i = 0; i < XI; ++i)
     ao[i] = min((wave * XI + i) * 8 + lane / 8, m_last) * (uint32_t)(a_stride * 2) + ((lane & 7) ^ (lane / 8)) * 16;
   const auto load_a = [&](uint32_t s, uint32_t buf) {
-    s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
+    // past the end the last stage is loaded again, into a buffer that is not read
+    const uint8_t* at = ab + min(s, steps - 1) * 128ull;
 #pragma unroll
-    for (int i = 0; i < XI; ++i) to_lds16(ab + s * 128ull + ao[i], lds + buf * AB + (wave * XI + i) * 1024);
+    for (int i = 0; i < XI; ++i) to_lds16(at, ao[i], base + buf * AB + (wave * XI + i) * 1024);
   };
-
-  // this lane's codes of the weight: ROWS: CODES columns of row l_row; else CODES values of column l_row of the tile
-  const uint32_t across = (ROWS ? BN : 64) / CODES, l_row = threadIdx.x / across, l_at = threadIdx.x % across * CODES;
-  typedef uint32_t words __attribute__((ext_vector_type(CW)));
-  words codes;
-  uint32_t scale;
-  const auto load_w = [&](uint32_t s) {
-    s = (min(s, steps - 1) + from) % steps_1;
-    uint32_t row, at;
-    if constexpr (ROWS) {
-      row = min(s * 64 + l_row, w_rows - 1);
-      at = min(n0 + l_at, w_steps * kStep - CODES);
-    } else {
-      row = min(n0 + l_row / (TN * 16) * (TN * 16) + l_row % 16 / 4 * (TN * 4) + l_row / 16 % TN * 4 + l_row % 4,
-                w_rows - 1);
-      at = s * 64 + l_at;
-    }
-    codes = *(const words*)(wd + row * (w_steps * 64ull) + at / 2);
-    scale = ws[row * (w_groups * 16ull) + scale_at(at / 32)];
+  // Codes: 16 bytes, a block of 32, of a lane; scales: the four bytes that hold that block's.  The first 2 BN lanes'
+  // are all; the others load the same again.  The last rows of a weight have offsets of their own, so that none
+  // behind the last is read.
+  const uint32_t id = threadIdx.x % (2 * BN), id_row = id / (ROW / 32), id_block = id % (ROW / 32);
+  uint32_t co, so, co_last, so_last;
+  if constexpr (ROWS) {
+    const uint32_t block = min(n0 / 32 + id_block, w_steps * 4 - 1), last = min(id_row, (w_rows - 1) % 64);
+    const uint32_t group = block / 16 * 16 + block % 4 * 4;
+    co = id_row * w_bytes + block * 16, co_last = last * w_bytes + block * 16;
+    so = id_row * s_bytes + group, so_last = last * s_bytes + group;
+  } else {
+    const uint32_t col =
+        id_row / (TN * 16) * (TN * 16) + id_row % 16 / 4 * (TN * 4) + id_row / 16 % TN * 4 + id_row % 4;
+    const uint32_t row = min(n0 + col, w_rows - 1) - n0;
+    co = co_last = row * w_bytes + id_block * 16;
+    so = so_last = row * s_bytes + id_block * 4;
+    wd += (uint64_t)n0 * w_bytes, ws += (uint64_t)n0 * s_bytes;
+  }
+  uint32_t w_step = from % steps_1;  // of the codes that are loaded next
+  const auto load_w = [&](uint32_t buf) {
+    const bool last = ROWS && w_step + 1 == steps_1;
+    const uint8_t* c = wd + (ROWS ? (uint64_t)w_step * 64 * w_bytes : w_step * 32ull);
+    const uint8_t* s = ws + (ROWS ? (uint64_t)w_step * 64 * s_bytes : w_step / 8 * 16ull + (w_step & 1) * 8);
+    to_lds16(c, last ? co_last : co, base + C_AT + buf * CB + wave % (BN / 32) * 1024);
+    to_lds4(s, last ? so_last : so, base + S_AT + buf * SB + wave % (BN / 32) * 256);
+    w_step = w_step + 1 == steps_1 ? 0 : w_step + 1;
   };
-  const auto store_w = [&](uint32_t buf) {
-    uint8_t* to = lds + 3 * AB + buf * BB + l_row * (ROWS ? BN * 2 : 128);
+  // To bf16: 16 codes of a lane, neighbours' from eight rows.  Rows exchange 16-byte pieces (piece c of row r at
+  // c ^ (r & 7)) so that eight lanes write to all banks; ROWS: in rows 2 and 3 of four, 8-byte halves of a piece as
+  // well, so that the four rows of a transposing read do not meet.
+  constexpr uint32_t ACROSS = ROW / 16;
+  const uint32_t l_row = threadIdx.x / (8 * ACROSS) * 8 + threadIdx.x % 8, l_at = threadIdx.x / 8 % ACROSS * 16;
+  const uint32_t swap = ROWS && (l_row & 2) ? 16 : 0;
+  const uint32_t c_at = C_AT + l_row * (ROW / 2) + l_at / 2, s_at = S_AT + l_row * (ROW / 8) + l_at / 32 * 4;
+  uint32_t to[2];
 #pragma unroll
-    for (int j = 0; j < CW; ++j) {
-      const i4v v = __builtin_bit_cast(i4v, bf16_of_codes(codes[j], scale));
-      const uint32_t chunk = l_at / 8 + j;
-      if constexpr (ROWS)
-        *(i4v*)(to + (chunk ^ (l_row >> 1 & 3)) * 16) = l_row & 1 ? i4v{v.z, v.w, v.x, v.y} : v;
-      else
-        *(i4v*)(to + (chunk ^ (l_row & 7)) * 16) = v;
-    }
+  for (int j = 0; j < 2; ++j) to[j] = B_AT + l_row * (ROW * 2) + ((l_at / 8 + j) ^ (l_row & 7)) * 16;
+  uint32_t c_step = from % steps_1;  // of the codes that are written next
+  const auto convert = [&](uint32_t buf, uint32_t half) {
+    const uint2 codes = *(const uint2*)(lds + c_at + buf * CB);
+    const uint32_t scale = lds[s_at + buf * SB + (ROWS ? n0 / 128 & 3 : c_step / 2 & 3)];
+    const uint32_t word[2] = {codes.x, codes.y};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *(b8v*)(lds + to[j] + half * BB) =
+          bf16_of_codes(ROWS ? __builtin_amdgcn_alignbit(word[j], word[j], swap) : word[j], scale);
+    c_step = c_step + 1 == steps_1 ? 0 : c_step + 1;
   };
 
   const uint32_t wm = wave % WM, wn = wave / WM;
@@ -669,60 +701,89 @@ __global__ __launch_bounds__(64 * WM * WN) void nz_mx_tiles16_kernel(const nz_bf
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f4{0, 0, 0, 0};
-  const uint32_t xr = (wm * TM * 16 + r) * 128;
+  // operand addresses; the halves of a step lie at constant distances
+  uint32_t ra[2], rb[TN * 2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) ra[h] = (wm * TM * 16 + r) * 128 + ((h * 4 + g) ^ (r & 7)) * 16;
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t row = g * 8 + q * 4 + r / 4, slot = wn * TN * 4 + r % 4 * TN + j;
+      rb[j * 2 + q] = base + B_AT + row * (BN * 2) + (slot ^ (row & 7) * 2 ^ (row >> 1 & 1)) * 8;
+    }
+  const uint32_t rw = B_AT + (wn * TN * 16 + r) * 128;
 
   load_w(0);
   load_a(0, 0);
-  store_w(0);
   load_w(1);
-  __builtin_amdgcn_sched_barrier(0);
   load_a(1, 1);
-  __builtin_amdgcn_sched_barrier(0);
-  uint32_t buf = 0;
-  for (uint32_t s = 0; s < steps; ++s) {
-    // behind the rows of step s: those of step s + 1 and the codes and scales of step s + 1
-    wait_loads<XI + 2>();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    block_barrier();  // step s is in LDS, step s - 1 is used up
-    const uint8_t* pa = lds + buf * AB;
-    const uint8_t* pb = lds + 3 * AB + (s & 1) * BB;
+  load_w(2);
+  wait_loads<2 * LOADS>();  // codes of step 0
+  block_barrier();
+  convert(0, 0);
+  wait_loads<LOADS>();  // rows of step 0, codes of step 1
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  block_barrier();
+
+  // Operands of a half step are read while the other half's are multiplied, across the barrier as well: behind it
+  // the first half of step s + 1 while the second of step s is multiplied.
+  struct Operands {
+    b8v a[TM], b[TN];
+  } first, second;
+  const auto read = [&](Operands& o, uint32_t buf, uint32_t odd, int h) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      b8v av[TM], bv[TN];
+    for (int j = 0; j < TN; ++j) {
+      if constexpr (ROWS) {
+        s4v part[2];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) av[i] = *(const b8v*)(pa + xr + i * 2048 + ((h * 4 + g) ^ (r & 7)) * 16);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (ROWS) {
-          s4v half[2];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t row = h * 32 + g * 8 + q * 4 + r / 4, slot = (wn * TN * 4 + r % 4 * TN + j) ^ (q * 4 + r / 4);
-            half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s4v*)(pb + row * (BN * 2) + slot * 8));
-          }
-          bv[j] = __builtin_bit_cast(b8v, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        } else {
-          bv[j] = *(const b8v*)(pb + (wn * TN * 16 + j * 16 + r) * 128 + ((h * 4 + g) ^ (r & 7)) * 16);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[j], av[i], acc[i][j], 0, 0, 0);
-      if (h == 0) {
-        store_w((s + 1) & 1);
-        __builtin_amdgcn_sched_barrier(0);
-        load_w(s + 2);
-        load_a(s + 2, buf == 0 ? 2 : buf - 1);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int q = 0; q < 2; ++q)
+          part[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4v*)(uintptr_t)(rb[j * 2 + q] + odd * BB + h * 64 * BN));
+        o.b[j] = __builtin_bit_cast(b8v, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      } else {
+        o.b[j] = *(const b8v*)(lds + odd * BB + rw + j * 2048 + ((h * 4 + g) ^ (r & 7)) * 16);
       }
     }
-    buf = buf == 2 ? 0 : buf + 1;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) o.a[i] = *(const b8v*)(lds + buf * AB + ra[h] + i * 2048);
+  };
+  const auto multiply = [&](const Operands& o) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o.b[j], o.a[i], acc[i][j], 0, 0, 0);
+  };
+  uint32_t buf = 0;  // s % 3
+  read(first, 0, 0, 0);
+  const auto body = [&](uint32_t s, auto odd) {
+    constexpr uint32_t here = decltype(odd)::value;  // s % 2
+    const uint32_t after = buf == 2 ? 0 : buf + 1, free = buf == 0 ? 2 : buf - 1;
+    read(second, buf, here, 1);
+    load_a(s + 2, free);
+    load_w(buf);
+    __builtin_amdgcn_sched_barrier(0);  // the compiler would read late, to save registers
+    multiply(first);
+    convert(after, here ^ 1);
     __builtin_amdgcn_sched_barrier(0);
+    // behind the rows of step s + 1 and the codes of step s + 2: what has just been asked for
+    wait_loads<LOADS>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();  // step s + 1 is in LDS, step s is used up
+    read(first, after, here ^ 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(second);
+    buf = after;
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t s = 0;
+  for (; s + 2 <= steps; s += 2) {
+    body(s, std::integral_constant<uint32_t, 0>());
+    body(s + 1, std::integral_constant<uint32_t, 1>());
   }
-  wait_loads<0>();
+  if (s < steps) body(s, std::integral_constant<uint32_t, 0>());
+  wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
   finish_tile<WM, WN, TM, TN>(acc, m, cols, m0, n0, bias, y, part);
 }
 
@@ -842,7 +903,7 @@ Cut cut_product(uint64_t m, uint64_t n, uint64_t k) {
 // The products of 16-bit rows, in steps of 64.
 Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) {
   const uint64_t cus = units();
-  if (tiles(m, cols, 128, 128) * 2 >= cus) return cut_into(128, 128, m, cols, steps, 1);
+  if (tiles(m, cols, 256, 128) * 2 >= cus) return cut_into(256, 128, m, cols, steps, 1);
   const uint64_t t = tiles(m, cols, 64, 64), parts = (2 * cus + t / 2) / t, most = steps / 8;
   return cut_into(64, 64, m, cols, steps, parts < most ? parts : most);
 }
@@ -871,8 +932,8 @@ int launch_tiles16(const Cut& c, const void* a, uint64_t a_stride, uint64_t m, c
   nz_mx_tiles16_kernel<WM, WN, TM, TN, ROWS, T><<<grid, 64 * WM * WN, 0, st>>>(                                        \
       (const nz_bf16*)a, a_stride, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)w_rows,              \
       (uint32_t)w_cols, (uint32_t)steps_1, planes, (uint32_t)cols, (const T*)bias, (T*)y, c.mt, c.nt, c.part_length, p)
-      if (c.bm == 128)
-        NZ_TILES16(2, 2, 4, 4);
+      if (c.bm == 256)
+        NZ_TILES16(4, 2, 4, 4);
       else
         NZ_TILES16(2, 2, 2, 2);
 #undef NZ_TILES16
