@@ -48,6 +48,16 @@ __device__ inline void load8_upto(const T* p, uint32_t n, float (&v)[8]) {
   }
 }
 
+// 8 values to a place that is aligned for vectors
+template <class T>
+__device__ inline void store8(T* p, const float (&v)[8]) {
+  typedef T whole __attribute__((ext_vector_type(8)));
+  whole a;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = (T)v[i];
+  *reinterpret_cast<whole*>(p) = a;
+}
+
 template <class T>
 __device__ inline void store8_upto(T* p, uint32_t n, const float (&v)[8]) {
   if (n >= 8) {
@@ -259,56 +269,65 @@ __device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& 
 }
 
 // Add the bias to a workgroup's tile and store it, or store it as it is among the parts.  A lane (r, g) of wavefront
-// (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], columns c0 .. c0 + 4 TN - 1.
-template <int WM, int WN, int TM, int TN, class T>
-__device__ inline void finish_tile(f4 (&acc)[TM][TN], uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+// (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], 4 TN consecutive columns.
+//
+// The tile goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold
+// pieces of 16 rows, the stores of a 256x256 tile took 14 us, a fifth of the product of 8192 x (14336x4096).
+template <int WM, int WN, int TM, int TN, int LDS, class T>
+__device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
                                    const T* bias, T* y, float* part) {
+  constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
-  const uint32_t wm = wave % WM, wn = wave / WM, c0 = n0 + wn * TN * 16 + g * TN * 4;
+  const uint32_t wm = wave % WM, wn = wave / WM, c0 = wn * TN * 16 + g * TN * 4;
   if (part) {
     part += (uint64_t)blockIdx.y * m * n;
-    const bool wide = n % 4 == 0;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const uint32_t row = m0 + (wm * TM + i) * 16 + r;
-      if (row >= m) continue;
-      float* q = part + (uint64_t)row * n;
+      if (row >= m) break;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const uint32_t c = c0 + j * 4;
-        if (wide && c < n)
-          *(f4*)(q + c) = acc[i][j];
-        else
+      for (int j = 0; j < TN; j += 2) {
+        const uint32_t c = n0 + c0 + j * 4;
+        float v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < n) q[c + e] = acc[i][j][e];
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][j + e / 4][e % 4];
+        if (c < n) store8_upto(part + (uint64_t)row * n + c, n - c, v);
       }
     }
     return;
   }
-  if (bias) {
+  constexpr int PITCH = BN * sizeof(T) + 16;  // eight lanes in turn write to all banks
+  static_assert(BM * PITCH <= LDS, "a tile of the result");
+  block_barrier();
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+  for (int j = 0; j < TN; j += 2) {
+    float b[8] = {};
+    const uint32_t c = n0 + c0 + j * 4;
+    if (bias && c < n) load8_upto(bias + c, n - c, b);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = (float)bias[min(c0 + j * 4 + e, n - 1)];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) acc[i][j][e] += v;
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const uint32_t row = m0 + (wm * TM + i) * 16 + r;
-    if (row >= m) continue;
-    T* q = y + (uint64_t)row * n;
-#pragma unroll
-    for (int j = 0; j < TN; j += 2) {
-      const uint32_t c = c0 + j * 4;
+    for (int i = 0; i < TM; ++i) {
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e], v[4 + e] = acc[i][j + 1][e];
-      if (c < n) store8_upto(q + c, n - c, v);
+      for (int e = 0; e < 8; ++e) v[e] = acc[i][j + e / 4][e % 4] + b[e];
+      store8(reinterpret_cast<T*>(lds + ((wm * TM + i) * 16 + r) * PITCH) + c0 + j * 4, v);
     }
+  }
+  __syncthreads();
+  constexpr int V = 16 / sizeof(T), ACROSS = BN / V;
+  typedef T whole __attribute__((ext_vector_type(V)));
+  typedef T piece __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+#pragma unroll
+  for (int i = 0; i < BM * ACROSS / (64 * W); ++i) {
+    const uint32_t at = i * (64 * W) + threadIdx.x, row = at / ACROSS, c = at % ACROSS * V;
+    const whole v = *(const whole*)(lds + row * PITCH + c * sizeof(T));
+    if (m0 + row >= m || n0 + c >= n) continue;
+    T* q = y + (uint64_t)(m0 + row) * n + n0 + c;
+    if (n0 + c + V <= n)
+      *(piece*)q = v;
+    else
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (n0 + c + e < n) q[e] = v[e];
   }
 }
 
@@ -316,7 +335,9 @@ __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint32_t m, uint32_t n, ui
 //
 // The rows of both sides are staged through LDS in steps of 128 values, NS stages deep, by loads that go to LDS
 // without registers; a wavefront counts its own loads down, and one barrier a step tells that everybody's have
-// arrived and that the stage before is used up.  Staged rows are exchanged in chunks of 16 bytes (x: chunk c of row
+// arrived and that the stage before is used up.  (Reading operands ahead across the barrier, or with 32x32x64
+// instructions, does not pay: from 8192 to 16384 values of a row the loop runs at 3.1 PFLOP/s as it is, the instruction
+// itself at 3.6 to 3.9 on such data.)  Staged rows are exchanged in chunks of 16 bytes (x: chunk c of row
 // r at c ^ (r & 7); w: at c ^ ((r >> 1) & 3)) so that eight lanes in turn read from all banks, and the weight rows of
 // a wavefront are staged in an order that leaves each lane 4 TN consecutive columns of the result.  Scales are
 // staged once per 512 values.
@@ -433,7 +454,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   if (s + 2 < steps) body(s + 2, B2());
   wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
 
-  finish_tile<WM, WN, TM, TN>(acc, m, n, m0, n0, bias, y, part);
+  finish_tile<WM, WN, TM, TN, NS * STAGE + 2 * SB>(acc, lds, m, n, m0, n0, bias, y, part);
 }
 
 // The parts of a product whose rows were cut, added in their order.
@@ -640,11 +661,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
   for (int i = 0; i < XI; ++i)
     ao[i] = min((wave * XI + i) * 8 + lane / 8, m_last) * (uint32_t)(a_stride * 2) + ((lane & 7) ^ (lane / 8)) * 16;
-  const auto load_a = [&](uint32_t s, uint32_t buf) {
+  const auto load_a = [&](uint32_t s, uint32_t buf, int i) {  // the i-th of XI
     // past the end the last stage is loaded again, into a buffer that is not read
-    const uint8_t* at = ab + min(s, steps - 1) * 128ull;
-#pragma unroll
-    for (int i = 0; i < XI; ++i) to_lds16(at, ao[i], base + buf * AB + (wave * XI + i) * 1024);
+    to_lds16(ab + min(s, steps - 1) * 128ull, ao[i], base + buf * AB + (wave * XI + i) * 1024);
   };
   // Codes: 16 bytes, a block of 32, of a lane; scales: the four bytes that hold that block's.  The first 2 BN lanes'
   // are all; the others load the same again.  The last rows of a weight have offsets of their own, so that none
@@ -715,9 +734,11 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   const uint32_t rw = B_AT + (wn * TN * 16 + r) * 128;
 
   load_w(0);
-  load_a(0, 0);
+#pragma unroll
+  for (int i = 0; i < XI; ++i) load_a(0, 0, i);
   load_w(1);
-  load_a(1, 1);
+#pragma unroll
+  for (int i = 0; i < XI; ++i) load_a(1, 1, i);
   load_w(2);
   wait_loads<2 * LOADS>();  // codes of step 0
   block_barrier();
@@ -731,51 +752,58 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   struct Operands {
     b8v a[TM], b[TN];
   } first, second;
-  const auto read = [&](Operands& o, uint32_t buf, uint32_t odd, int h) {
+  constexpr int READS = TN + TM;
+  const auto read = [&](Operands& o, uint32_t buf, uint32_t odd, int h, int q) {  // the q-th of READS
+    if (q >= TN) {
+      o.a[q - TN] = *(const b8v*)(lds + buf * AB + ra[h] + (q - TN) * 2048);
+    } else if constexpr (ROWS) {
+      s4v part[2];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      if constexpr (ROWS) {
-        s4v part[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          part[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4v*)(uintptr_t)(rb[j * 2 + q] + odd * BB + h * 64 * BN));
-        o.b[j] = __builtin_bit_cast(b8v, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
-      } else {
-        o.b[j] = *(const b8v*)(lds + odd * BB + rw + j * 2048 + ((h * 4 + g) ^ (r & 7)) * 16);
-      }
+      for (int p = 0; p < 2; ++p)
+        part[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s4v*)(uintptr_t)(rb[q * 2 + p] + odd * BB + h * 64 * BN));
+      o.b[q] = __builtin_bit_cast(b8v, __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      o.b[q] = *(const b8v*)(lds + odd * BB + rw + q * 2048 + ((h * 4 + g) ^ (r & 7)) * 16);
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i) o.a[i] = *(const b8v*)(lds + buf * AB + ra[h] + i * 2048);
-  };
-  const auto multiply = [&](const Operands& o) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o.b[j], o.a[i], acc[i][j], 0, 0, 0);
   };
   uint32_t buf = 0;  // s % 3
-  read(first, 0, 0, 0);
+#pragma unroll
+  for (int q = 0; q < READS; ++q) read(first, 0, 0, 0, q);
   const auto body = [&](uint32_t s, auto odd) {
     constexpr uint32_t here = decltype(odd)::value;  // s % 2
+    // reads and loads go beside the instructions, as in nz_mx_tiles_kernel
+    constexpr int M = TM * TN, EARLY = M - M / 4;
+    const auto multiply = [&](const Operands& o, auto beside) {
+#pragma unroll
+      for (int t = 0; t < M; ++t) {
+        const int i = t % TM, j = t / TM;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(o.b[j], o.a[i], acc[i][j], 0, 0, 0);
+        beside(t);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
     const uint32_t after = buf == 2 ? 0 : buf + 1, free = buf == 0 ? 2 : buf - 1;
-    read(second, buf, here, 1);
-    load_a(s + 2, free);
-    load_w(buf);
-    __builtin_amdgcn_sched_barrier(0);  // the compiler would read late, to save registers
-    multiply(first);
-    convert(after, here ^ 1);
-    __builtin_amdgcn_sched_barrier(0);
+    multiply(first, [&](int t) {
+      if (t == 0) convert(after, here ^ 1);
+#pragma unroll
+      for (int q = 0; q < READS; ++q)
+        if (q * EARLY / READS == t) read(second, buf, here, 1, q);
+#pragma unroll
+      for (int i = 0; i < XI; ++i)
+        if (i * M / XI == t) load_a(s + 2, free, i);
+      if (t == M - 1) load_w(buf);
+    });
     // behind the rows of step s + 1 and the codes of step s + 2: what has just been asked for
     wait_loads<LOADS>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     block_barrier();  // step s + 1 is in LDS, step s is used up
-    read(first, after, here ^ 1, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(second);
+    multiply(second, [&](int t) {
+#pragma unroll
+      for (int q = 0; q < READS; ++q)
+        if (q * EARLY / READS == t) read(first, after, here ^ 1, 0, q);
+    });
     buf = after;
-    __builtin_amdgcn_sched_barrier(0);
   };
   uint32_t s = 0;
   for (; s + 2 <= steps; s += 2) {
@@ -784,7 +812,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   }
   if (s < steps) body(s, std::integral_constant<uint32_t, 0>());
   wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
-  finish_tile<WM, WN, TM, TN>(acc, m, cols, m0, n0, bias, y, part);
+  finish_tile<WM, WN, TM, TN, S_AT + 3 * SB>(acc, lds, m, cols, m0, n0, bias, y, part);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------
