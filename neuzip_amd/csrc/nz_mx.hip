@@ -272,7 +272,7 @@ __device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& 
 // (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], 4 TN consecutive columns.
 //
 // The tile goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold
-// pieces of 16 rows, the stores of a 256x256 tile took 14 us, a fifth of the product of 8192 x (14336x4096).
+// pieces of 16 rows, the stores of 256 tiles of 256x256 took 14 us, of 61 that 4096 values of a row take.
 template <int WM, int WN, int TM, int TN, int LDS, class T>
 __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
                                    const T* bias, T* y, float* part) {
@@ -350,8 +350,9 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   constexpr int XB = BM * 128, WB = BN * 64, STAGE = XB + WB;
   constexpr int XI = BM / 8 / W, WI = BN / 16 / W, LOADS = XI + WI;
   constexpr int SI = (BM + BN + 63) / 64, SB = SI * 1024;  // scales: 64 rows of 16 bytes a load
-  static_assert(XI * 8 * W == BM && WI * 16 * W == BN && SI <= W, "loads per wavefront");
-  static_assert(NS >= 3 && NS <= 8, "two buffers of scales reach 8 stages");
+  static_assert(XI * 8 * W == BM && WI * 16 * W == BN, "loads per wavefront");
+  constexpr int SL = (SI + W - 1) / W;
+  static_assert(NS >= 2 && NS <= 8, "two buffers of scales reach 8 stages");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + 2 * SB];
   const uint32_t base = lds_address(lds);
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -377,12 +378,17 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   for (int i = 0; i < WI; ++i)
     wo[i] = min(column((wave * WI + i) * 16 + lane / 4), n_last) * (all_steps * 64) +
             ((lane & 3) ^ ((lane >> 3) & 3)) * 16;
-  // more wavefronts than loads of scales: some load the same
-  const uint32_t si = wave % SI, srow = min(si * 64 + lane, BM + BN - 1u);
-  const uint8_t* sb = (si * 64 < BM ? xs + (uint64_t)m0 * (groups * 16ull) : ws + (uint64_t)n0 * (groups * 16ull)) +
-                      from * 16;
+  // where wavefronts and loads of scales do not match, some load the same
+  const uint8_t* sb[SL];
+  uint32_t so[SL], si[SL];
+#pragma unroll
+  for (int i = 0; i < SL; ++i) {
+    si[i] = (i * W + wave) % SI;
+    const uint32_t row = min(si[i] * 64 + lane, BM + BN - 1u);
+    sb[i] = (si[i] * 64 < BM ? xs + (uint64_t)m0 * (groups * 16ull) : ws + (uint64_t)n0 * (groups * 16ull)) + from * 16;
+    so[i] = (row < BM ? min(row, m_last) : min(column(row - BM), n_last)) * (groups * 16);
+  }
   static_assert(BM % 64 == 0, "a load takes scales of one side");
-  const uint32_t so = (srow < BM ? min(srow, m_last) : min(column(srow - BM), n_last)) * (groups * 16);
   uint32_t sbuf = 0;
   const auto load_stage = [&](uint32_t s, uint32_t buf, bool scales) {
     s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
@@ -391,7 +397,12 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     for (int i = 0; i < XI; ++i) to_lds16(xb + s * 128ull, xo[i], to + (wave * XI + i) * 1024);
 #pragma unroll
     for (int i = 0; i < WI; ++i) to_lds16(wb + s * 64ull, wo[i], to + XB + (wave * WI + i) * 1024);
-    if (scales) to_lds16(sb + (s >> 2) * 16, so, base + NS * STAGE + sbuf * SB + si * 1024), sbuf ^= 1;
+    if (scales) {
+#pragma unroll
+      for (int i = 0; i < SL; ++i)
+        to_lds16(sb[i] + (s >> 2) * 16, so[i], base + NS * STAGE + sbuf * SB + si[i] * 1024);
+      sbuf ^= 1;
+    }
   };
 
   const uint32_t wm = wave % WM, wn = wave / WM;
@@ -411,7 +422,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     constexpr int byte = decltype(b4)::value;  // s % 4
     // loads behind those of stage s: NS - 2 stages, with scales where a stage begins a group
     constexpr int starts = (byte + NS - 2) / 4;
-    wait_loads<(NS - 2) * LOADS + starts>();
+    wait_loads<(NS - 2) * LOADS + starts * SL>();
     block_barrier();  // stage s is there, stage s - 1 is used up
     const uint8_t* b = lds + buf * STAGE;
     if (byte == 0) {
@@ -921,7 +932,7 @@ uint64_t units() {
 // into parts of 1024 values at least.
 Cut cut_product(uint64_t m, uint64_t n, uint64_t k) {
   const uint64_t cus = units(), groups = nz_ceil_div(k, kGroup);
-  if (tiles(m, n, 256, 256) >= 4 * cus && k >= 2048) return cut_into(256, 256, m, n, groups, 1);
+  if (tiles(m, n, 128, 256) >= 8 * cus && k >= 2048) return cut_into(128, 256, m, n, groups, 1);
   if (tiles(m, n, 128, 128) * 2 >= 3 * cus) return cut_into(128, 128, m, n, groups, 1);
   if (tiles(m, n, 64, 128) * 2 >= cus) return cut_into(64, 128, m, n, groups, 1);
   const uint64_t t = tiles(m, n, 64, 64), parts = (cus + t / 2) / t, most = groups / 2;
@@ -994,8 +1005,8 @@ void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, cons
   nz_mx_tiles_kernel<WM, WN, TM, TN, NS, T><<<grid, 64 * WM * WN, 0, st>>>(                                        \
       (const uint8_t*)xd, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, \
       bias, y, c.mt, c.nt, c.part_length, part)
-  if (c.bm == 256)
-    NZ_TILES(4, 2, 4, 8, 3);
+  if (c.bn == 256)
+    NZ_TILES(2, 2, 4, 8, 2);
   else if (c.bm == 128)
     NZ_TILES(2, 2, 4, 4, 3);
   else if (c.bn == 128)
