@@ -4,7 +4,7 @@
 // while some of its workgroups sort the tokens (clearing is bound by memory, sorting by arithmetic and latency); the
 // others add up the rows of g.  The launches:
 //
-//   sort   64 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller keys (index, then
+//   sort   32 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller keys (index, then
 //          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
 //          the same place every time.
 //   merge  (more than one tile) the place among all tokens: the same count in the other tiles, by bisection.
@@ -17,6 +17,7 @@ namespace {
 
 constexpr uint32_t kTile = 8192;      // tokens that are compared with each other
 constexpr uint32_t kTileBits = 13;
+constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
 constexpr uint32_t kClear = 1 << 16;  // bytes a workgroup clears
 constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
 
@@ -49,31 +50,32 @@ __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long*
   __shared__ __attribute__((aligned(32))) Key keys[kTile];
   __shared__ uint32_t smaller[8][64];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const uint32_t block = blockIdx.x % (kTile / 64), base = blockIdx.x / (kTile / 64) * kTile;
-  const uint32_t here = min(kTile, count - base), blocks = (here + 63) / 64;
-  for (uint32_t i = threadIdx.x; i < blocks * 64; i += 512) {
+  const uint32_t block = blockIdx.x % (kTile / kSorted), base = blockIdx.x / (kTile / kSorted) * kTile;
+  const uint32_t here = min(kTile, count - base), blocks = (here + 31) / 32;
+  for (uint32_t i = threadIdx.x; i < blocks * 32; i += 512) {
     const long long v = i < here ? index[base + i] : -1;
     const uint32_t row = v >= 0 && v < (long long)rows && v != skip ? (uint32_t)v : rows;
     keys[i] = (Key)row << kTileBits | i;
   }
   __syncthreads();
-  const Key mine = keys[block * 64 + lane];
+  // the two halves of a wavefront hold the same tokens and look at another sixteenth of the keys each
+  const uint32_t i = block * kSorted + lane % kSorted, part = wave * 2 + lane / kSorted;
+  const Key mine = keys[i];
   uint32_t less = 0;
-  const uint32_t first = blocks * wave / 8, last = blocks * (wave + 1) / 8;
+  const uint32_t first = blocks * part / 16, last = blocks * (part + 1) / 16;
   for (uint32_t b = first; b < last; ++b) {
 #pragma unroll
-    for (uint32_t j = 0; j < 64; j += 4) {
-      const key4 k = *(const key4*)(keys + b * 64 + j);
+    for (uint32_t j = 0; j < 32; j += 4) {
+      const key4 k = *(const key4*)(keys + b * 32 + j);
       less += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
     }
   }
   smaller[wave][lane] = less;
   __syncthreads();
-  const uint32_t i = block * 64 + lane;
-  if (wave || i >= here) return;
+  if (threadIdx.x >= kSorted || i >= here) return;
   less = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < 8; ++w) less += smaller[w][lane];
+  for (uint32_t w = 0; w < 8; ++w) less += smaller[w][lane] + smaller[w][lane + kSorted];
   places[base + less] = Place{(uint32_t)(mine >> kTileBits), base + i};
 }
 
@@ -307,7 +309,7 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
     if (!dev_workspace || (uintptr_t)dev_workspace % 16) return nz_fail(NZ_ERR_ALIGN, "misaligned workspace");
   }
   const uint64_t bytes = flags & NZ_GRAD_ACCUMULATE ? 0 : rows * cols * size, clearers = nz_ceil_div(bytes, kClear);
-  const uint32_t sorters = (uint32_t)nz_ceil_div(count, 64);
+  const uint32_t sorters = (uint32_t)nz_ceil_div(count, kSorted);
   if (clearers + sorters > 0x7FFFFFFFull) return nz_fail(NZ_ERR_ARG, "table too large for one launch");
   if (clearers + sorters == 0) return NZ_OK;
   const hipStream_t st = (hipStream_t)stream;
