@@ -19,7 +19,7 @@ constexpr uint32_t kTile = 8192;      // tokens that are compared with each othe
 constexpr uint32_t kTileBits = 13;
 constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
 constexpr uint32_t kClear = 1 << 16;  // bytes a workgroup clears
-constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
+constexpr uint32_t kBatch = 16;      // rows of g that a wavefront has on their way at a time
 
 // A sorted token: its index (the number of rows if it takes no part) and where it stands.
 struct Place {
@@ -226,9 +226,11 @@ __global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* pla
   const uint64_t id = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const uint64_t window = id / slices, first = window * size, next = first + size;
   if (next >= count) return;
-  const uint32_t row = places[next - 1].row, lane = threadIdx.x & 63;
-  if (row == rows || places[next].row != row) return;
-  if (places[first].row == row && first && places[first - 1].row == row) return;  // it began before
+  // the places around the window's borders, asked for together
+  const uint32_t lane = threadIdx.x & 63, row = places[next - 1].row, behind = places[next].row;
+  const uint32_t begin = places[first].row, before = places[first ? first - 1 : 0].row;
+  if (row == rows || behind != row) return;
+  if (first && begin == row && before == row) return;  // it began before
   uint32_t more = 0;  // windows that it goes on in
   for (;;) {
     const uint64_t at = next + (uint64_t)(more + lane) * size;
@@ -251,13 +253,13 @@ __global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* pla
   const Columns k = columns_of((uint32_t)(id - window * slices), lane, cols);
   float sum[8];
   load8(pieces + piece_at(window, 1, cols), k, cols, sum);
-  for (uint32_t q = 1; q <= more; q += 8) {
-    float v[8][8];
+  for (uint32_t q = 1; q <= more; q += 16) {
+    float v[16][8];
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)  // the last piece again where there are fewer
+    for (uint32_t j = 0; j < 16; ++j)  // the last piece again where there are fewer
       load8(pieces + piece_at(window + min(q + j, more), 0, cols), k, cols, v[j]);
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
+    for (uint32_t j = 0; j < 16; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum[e] = q + j <= more ? sum[e] + v[j][e] : sum[e];
   }
