@@ -465,7 +465,7 @@ int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, ui
 
 /* y[m][n] = sum_k x[m][k] w[n][k] + bias[n]: w holds n rows of k values in 4 bits, the m rows of x are brought to 8
    bits on the way.  Sums in 32 bits, one rounding to dtype.  bias may be NULL; it, x and y have the same dtype.
-   k is 1 to 2^22, n at most 2^22.
+   k is 1 to 2^22, n at most 2^21, m at most 2^24.
    The workspace (nz_mx_linear_workspace_bytes bytes, 16-byte aligned, none if that is 0) is free again when the
    call's work has ended. */
 uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype);

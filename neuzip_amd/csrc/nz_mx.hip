@@ -868,10 +868,11 @@ void by_dtype(int dtype, F f) {
     f(float());
 }
 
-void launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint64_t stride, int bits, void* data,
-                     void* scales, hipStream_t st) {
+int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint64_t stride, int bits, void* data,
+                    void* scales, hipStream_t st) {
   const uint32_t groups = (cols + kGroup - 1) / kGroup;
-  const uint64_t waves = rows * groups;
+  const uint64_t waves = nz_mul(rows, groups);
+  if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
   const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
@@ -882,6 +883,7 @@ void launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uin
       nz_mx_quantize_kernel<8, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups,
                                                         (uint8_t*)data, (uint8_t*)scales);
   });
+  return nz_launched();
 }
 
 int launch_values(const void* data, const void* scales, uint64_t rows, uint64_t cols, int bits, const void* index,
@@ -982,7 +984,9 @@ int launch_tiles16(const Cut& c, const void* a, uint64_t a_stride, uint64_t m, c
   return nz_launched();
 }
 
-// rows that are brought to 8 bits inside the kernel: as many as one workgroup does at little cost
+// Rows that are brought to 8 bits inside the kernel: as many as one workgroup does at little cost.  8 rows against
+// 14336x4096: 12.4 us, in two launches 3.4 + 10.2; against 4096x4096 7.7 and 3.4 + 6.6; 16 rows of 2048 values against
+// 14336 rows 9.9 and 3.3 + 6.4.
 bool few_rows(uint64_t m, uint64_t k) { return m <= 16 && m * nz_ceil_div(k, kGroup) <= 64; }
 
 template <bool QUANTIZE, class T>
@@ -991,7 +995,9 @@ void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, cons
   const uint32_t groups = (k + kGroup - 1) / kGroup;
   uint32_t kw = groups >= 8 ? 8 : groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
   const uint64_t t = nz_ceil_div(n, 16);
-  if (kw == 8 && t > 2 * units()) kw = 4;
+  // weights that fill the device with fewer wavefronts to a row: fewer workgroups that each bring the rows to 8 bits.
+  // 14336x4096, with 2, 4, 8 wavefronts to a row: one row 10.3, 8.7, 9.3 us; four 10.4, 11.5, 13.0
+  if (t > 2 * units()) kw = kw < 4 ? kw : m >= 4 ? 2 : 4;
   const uint32_t lds = QUANTIZE ? (uint32_t)m * groups * 528 : 0;
   nz_mx_few_kernel<1, QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
       x, stride, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, bias, y, kw);
@@ -1058,8 +1064,10 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, c
 
 // What the products ask of the weight and the counts: an offset inside a tile has 32 bits.
 int check_product(uint64_t m, uint64_t n, uint64_t k, const void* wd, const void* ws) {
-  if (k == 0 || k > 1ull << 22 || n > 1ull << 22) return nz_fail(NZ_ERR_ARG, "a weight must have 1 to 2^22 columns and up to 2^22 rows");
-  if (m > 1ull << 24) return nz_fail(NZ_ERR_ARG, "too many rows for one launch");
+  if (k == 0 || k > 1ull << 22 || n > 1ull << 21)
+    return nz_fail(NZ_ERR_ARG, "a weight must have 1 to 2^22 columns and up to 2^21 rows");
+  if (m > 1ull << 24 || nz_ceil_div(m, 64) * nz_ceil_div(n > k ? n : k, 64) > 0x7FFFFFFFull)
+    return nz_fail(NZ_ERR_ARG, "too many rows for one launch");
   return check_mx(wd, ws);
 }
 
@@ -1078,7 +1086,7 @@ Planes planes_of(const void* g, int dtype, uint64_t m, uint64_t n, uint64_t stri
   Planes p;
   p.count = dtype == NZ_DTYPE_BF16 ? 1 : dtype == NZ_DTYPE_F16 ? 2 : 3;
   p.padded = nz_ceil_div(n, 64) * 64;
-  const bool as_is = dtype == NZ_DTYPE_BF16 && n % 64 == 0 && stride % 8 == 0 && stride < 1ull << 24 && aligned(g, 16);
+  const bool as_is = dtype == NZ_DTYPE_BF16 && n % 64 == 0 && stride % 8 == 0 && stride <= 1ull << 22 && aligned(g, 16);
   p.bytes = as_is ? 0 : align256(nz_mul(m, p.padded * p.count * 2));
   return p;
 }
@@ -1099,9 +1107,7 @@ int nz_mx_quantize(const void* dev_x, int dtype, uint64_t rows, uint64_t cols, u
   if (!cols_ok(cols)) return nz_fail(NZ_ERR_ARG, "rows must hold 1 to 2^30 values");
   if (!dev_x) return nz_fail(NZ_ERR_ARG, "null input");
   if (int rc = check_mx(dev_data, dev_scales)) return rc;
-  if (int rc = check_grid(nz_ceil_div(nz_mul(rows, nz_ceil_div(cols, kGroup)), 4))) return rc;
-  launch_quantize(dev_x, dtype, rows, (uint32_t)cols, stride, bits, dev_data, dev_scales, (hipStream_t)stream);
-  return nz_launched();
+  return launch_quantize(dev_x, dtype, rows, (uint32_t)cols, stride, bits, dev_data, dev_scales, (hipStream_t)stream);
 }
 
 int nz_mx_dequantize(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int bits,
@@ -1151,7 +1157,7 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
   }
   const Room room = product_room(m, n, k, dtype);
   uint8_t* base = (uint8_t*)dev_workspace;
-  launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st);
+  if (int rc = launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st)) return rc;
   return launch_product(base + room.xd, base + room.xs, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y,
                         dtype, room, base, st);
 }

@@ -62,6 +62,8 @@ class Embedding(torch.nn.Module):
 
     def forward(self, x):
         if self.trainable and torch.is_grad_enabled():
+            if not x.is_cuda:
+                raise ValueError("a compressed table is trained on the GPU: the indices must be there")
             return CompressedEmbedding.apply(x, self._p, self)
         return self._rows(x)
 

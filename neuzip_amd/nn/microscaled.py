@@ -66,13 +66,14 @@ class MXEmbedding(_Microscaled):
         self.embedding_dim = embedding.embedding_dim
         self.padding_idx = embedding.padding_idx
         self.scale = float(scale)
-        self.dtype = embedding.weight.dtype
+        # the type of the rows, which the module's own .to and .half change
+        self.register_buffer("_like", embedding.weight.data.new_empty(0), persistent=False)
         self._hold(embedding.weight.data)
         self.register_buffer("_status", torch.zeros(1, dtype=torch.int32, device=self.weight_data.device),
                              persistent=False)
 
     def forward(self, x):
-        return mx_embedding(x, self.weight, self.scale, self.dtype, self._status)
+        return mx_embedding(x, self.weight, self.scale, self._like.dtype, self._status)
 
     def linear(self, x):
         return mx_linear(x, self.weight)

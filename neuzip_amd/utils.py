@@ -81,20 +81,24 @@ def _convert(manager, module: torch.nn.Module, prefix: str = "") -> torch.nn.Mod
     return module
 
 
-def mx_convert(module: torch.nn.Module, prefix: str = "") -> torch.nn.Module:
+def mx_convert(module: torch.nn.Module, prefix: str = "", _made=None) -> torch.nn.Module:
     """In place: the ``nn.Linear`` layers that ``Manager.convert`` would compress
     (those whose attribute name contains ``lm_head`` are left alone) are held in
-    microscaled 4 bits instead, with their weights frozen."""
+    microscaled 4 bits instead, with their weights frozen.  A layer that stands in
+    several places is converted once."""
     from neuzip_amd.nn import MXLinear
 
-    for name, child in list(module.named_children()):
+    made = {} if _made is None else _made
+    for name, child in list(module._modules.items()):
         dotted = f"{prefix}.{name}" if prefix else name
-        if "lm_head" in name:
+        if child is None or "lm_head" in name:
             continue
         if isinstance(child, torch.nn.Linear):
-            logger.debug("Converting %s: %s", dotted, child)
-            setattr(module, name, MXLinear(child))
-            _delete_module(child)
+            if child not in made:
+                logger.debug("Converting %s: %s", dotted, child)
+                made[child] = MXLinear(child)
+                _delete_module(child)
+            setattr(module, name, made[child])
         else:
-            mx_convert(child, dotted)
+            mx_convert(child, dotted, made)
     return module

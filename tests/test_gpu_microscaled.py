@@ -365,6 +365,19 @@ def test_layers_hold_compute_and_travel():
     same(model.up.bias.grad, torch.full((352,), 18.0))
 
 
+def test_layers_that_stand_in_two_places_and_types_of_rows():
+    shared = torch.nn.Linear(64, 64).to(torch.bfloat16)
+    model = torch.nn.ModuleList([torch.nn.Sequential(shared, torch.nn.ReLU()), torch.nn.Sequential(shared)])
+    neuzip_amd.mx_convert(model)
+    assert isinstance(model[0][0], neuzip_amd.nn.MXLinear) and model[0][0] is model[1][0]
+    table = neuzip_amd.nn.MXEmbedding(torch.nn.Embedding(9, 64).to(torch.bfloat16))
+    ids = torch.arange(9, device=DEV)
+    a = table(ids)
+    b = table.half()(ids)
+    assert a.dtype == torch.bfloat16 and b.dtype == torch.float16
+    same(a, b)
+
+
 def test_rows_of_one_quantisation_serve_several_weights():
     x = rnd(20, 256, dtype=torch.float16).to(DEV)
     x8 = ops.mx_quantize(x, 8)

@@ -56,7 +56,8 @@ def test_refusals_of_the_abi():
     refused(L.nz_mx_linear_grad(p, 9, 1, 1, 1, p, p, 1, p, p, 1 << 30, None), C, "Unsupported data type")
     refused(L.nz_mx_linear_grad(None, 0, 1, 1, 1, p, p, 1, p, p, 1 << 30, None), A, "null gradient")
     refused(L.nz_mx_linear_grad(p, 0, 1, 0, 1, p, p, 1, p, p, 1 << 30, None), A, "without rows")
-    refused(L.nz_mx_linear_grad(p, 0, 1, 1 << 23, 1 << 23, p, p, 1, p, p, 1 << 30, None), A, "2^22")
+    refused(L.nz_mx_linear_grad(p, 0, 1, 1 << 22, 1 << 22, p, p, 1, p, p, 1 << 30, None), A, "2^21")
+    refused(L.nz_mx_linear(p, 0, 1 << 24, 32, 32, p, p, 1 << 21, None, p, p, 1 << 62, None), A, "too many rows")
     assert L.nz_mx_linear_grad_workspace_bytes(p, 0, 100, 512, 512, 512) < 100 * 512 * 2 < (
         L.nz_mx_linear_grad_workspace_bytes(p, 1, 100, 512, 512, 512))
     need = L.nz_mx_linear_grad_workspace_bytes(p + 2, 0, 100, 512, 512, 512)
@@ -133,6 +134,16 @@ def test_a_table_that_cannot_be_trained_is_refused():
         neuzip_amd.nn.Embedding(None, torch.nn.Embedding(4, 8, max_norm=1.0), trainable=True)
     with pytest.raises(ValueError, match="sparse"):
         neuzip_amd.nn.Embedding(None, torch.nn.Embedding(4, 8, sparse=True), trainable=True)
+
+
+def test_a_compressed_table_is_trained_on_the_gpu():
+    class Held:
+        def write(self, data):
+            return "0"
+
+    emb = neuzip_amd.nn.Embedding(Held(), torch.nn.Embedding(4, 8), trainable=True)
+    with pytest.raises(ValueError, match="trained on the GPU"):
+        emb(torch.zeros(2, dtype=torch.int64))
 
 
 def test_the_oracle_itself():
