@@ -352,8 +352,8 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   constexpr int SI = (BM + BN + 63) / 64, SB = SI * 1024;  // scales: 64 rows of 16 bytes a load
   static_assert(XI * 8 * W == BM && WI * 16 * W == BN, "loads per wavefront");
   constexpr int SL = (SI + W - 1) / W;
-  static_assert(NS >= 2 && NS <= 8, "two buffers of scales reach 8 stages");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + 2 * SB];
+  static_assert(NS >= 2 && NS <= 4, "a group's scales are asked for when the last group's have been read");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + SB];
   const uint32_t base = lds_address(lds);
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t r = lane & 15, g = lane / 16;
@@ -389,7 +389,6 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     so[i] = (row < BM ? min(row, m_last) : min(column(row - BM), n_last)) * (groups * 16);
   }
   static_assert(BM % 64 == 0, "a load takes scales of one side");
-  uint32_t sbuf = 0;
   const auto load_stage = [&](uint32_t s, uint32_t buf, bool scales) {
     s = min(s, steps - 1);  // past the end the last stage is loaded again, into a buffer that is not read
     const uint32_t to = base + buf * STAGE;
@@ -400,8 +399,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     if (scales) {
 #pragma unroll
       for (int i = 0; i < SL; ++i)
-        to_lds16(sb[i] + (s >> 2) * 16, so[i], base + NS * STAGE + sbuf * SB + si[i] * 1024);
-      sbuf ^= 1;
+        to_lds16(sb[i] + (s >> 2) * 16, so[i], base + NS * STAGE + si[i] * 1024);
     }
   };
 
@@ -417,7 +415,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
 
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) load_stage(i, i, i % 4 == 0);
-  uint32_t buf = 0, cur = 0;
+  uint32_t buf = 0;
   const auto body = [&](uint32_t s, auto b4) {
     constexpr int byte = decltype(b4)::value;  // s % 4
     // loads behind those of stage s: NS - 2 stages, with scales where a stage begins a group
@@ -426,8 +424,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     block_barrier();  // stage s is there, stage s - 1 is used up
     const uint8_t* b = lds + buf * STAGE;
     if (byte == 0) {
-      const uint8_t* st = lds + NS * STAGE + cur * SB;
-      cur ^= 1;
+      const uint8_t* st = lds + NS * STAGE;
 #pragma unroll
       for (int i = 0; i < TM; ++i) sx[i] = *(const uint32_t*)(st + (wm * TM * 16 + i * 16 + r) * 16 + g * 4);
 #pragma unroll
@@ -465,7 +462,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   if (s + 2 < steps) body(s + 2, B2());
   wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
 
-  finish_tile<WM, WN, TM, TN, NS * STAGE + 2 * SB>(acc, lds, m, n, m0, n0, bias, y, part);
+  finish_tile<WM, WN, TM, TN, NS * STAGE + SB>(acc, lds, m, n, m0, n0, bias, y, part);
 }
 
 // The parts of a product whose rows were cut, added in their order.
@@ -934,7 +931,7 @@ uint64_t units() {
 // into parts of 1024 values at least.
 Cut cut_product(uint64_t m, uint64_t n, uint64_t k) {
   const uint64_t cus = units(), groups = nz_ceil_div(k, kGroup);
-  if (tiles(m, n, 128, 256) >= 8 * cus && k >= 2048) return cut_into(128, 256, m, n, groups, 1);
+  if (tiles(m, n, 128, 256) >= 4 * cus) return cut_into(128, 256, m, n, groups, 1);
   if (tiles(m, n, 128, 128) * 2 >= 3 * cus) return cut_into(128, 128, m, n, groups, 1);
   if (tiles(m, n, 64, 128) * 2 >= cus) return cut_into(64, 128, m, n, groups, 1);
   const uint64_t t = tiles(m, n, 64, 64), parts = (cus + t / 2) / t, most = groups / 2;
@@ -1014,7 +1011,7 @@ void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, cons
   if (c.bn == 256)
     NZ_TILES(2, 2, 4, 8, 2);
   else if (c.bm == 128)
-    NZ_TILES(2, 2, 4, 4, 3);
+    NZ_TILES(2, 2, 4, 4, 2);
   else if (c.bn == 128)
     NZ_TILES(2, 2, 2, 4, 4);
   else
