@@ -38,7 +38,7 @@ __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long*
 #pragma unroll
     for (uint32_t i = 0; i < kClear / (512 * 16); ++i) {
       const uint64_t at = from + (i * 512 + threadIdx.x) * 16;
-      if (at < body) __builtin_nontemporal_store(word4{0, 0, 0, 0}, q + at / 16);
+      if (at < body) q[at / 16] = word4{0, 0, 0, 0};
     }
     if (from == 0 && threadIdx.x < 32) {  // what does not lie in whole words
       const uint64_t at = threadIdx.x < 16 ? threadIdx.x : head + body + threadIdx.x - 16;

@@ -3,6 +3,7 @@
 // The format is stated in include/neuzip_hip.h.  A row's codes lie in order and are filled up to 128 values, so
 // that a step of the matrix instruction (128 values of a row) never ends inside one; its block scales lie in
 // groups of 16 (512 values) with the four bytes that a lane needs in four successive steps next to each other.
+#include <cmath>
 #include <type_traits>
 
 #include "nz_operators.h"
@@ -911,39 +912,62 @@ struct Cut {
   uint64_t part_bytes(uint64_t m, uint64_t cols) const { return parts > 1 ? align256(parts * m * cols * 4) : 0; }
 };
 
-Cut cut_into(uint32_t bm, uint32_t bn, uint64_t m, uint64_t cols, uint64_t length, uint64_t parts) {
-  Cut c;
-  c.bm = bm, c.bn = bn;
-  c.mt = (uint32_t)nz_ceil_div(m, bm), c.nt = (uint32_t)nz_ceil_div(cols, bn);
-  c.part_length = (uint32_t)nz_ceil_div(length, parts ? parts : 1);
-  c.parts = (uint32_t)nz_ceil_div(length, c.part_length);
-  return c;
+// What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them do; 256
+// compute units, 64 steps and more, everything else idle.
+struct Tile {
+  uint32_t bm, bn, slots;
+  float full, half;
+};
+// Products of 8-bit rows, 128 values a step: 2.6, 2.1, 1.5 and 1.1 PFLOP/s where the device is full.
+constexpr Tile kTiles[] = {{128, 256, 512, 1.72f, 1.38f},
+                           {128, 128, 512, 1.04f, 0.85f},
+                           {64, 128, 256, 0.38f, 0.40f},
+                           {64, 64, 256, 0.25f, 0.31f}};
+// Products of 16-bit rows, 64 values a step: 1.06 and 0.47 PFLOP/s.
+constexpr Tile kTiles16[] = {{256, 128, 256, 1.00f, 0.85f}, {64, 64, 256, 0.29f, 0.38f}};
+
+// The cut that takes the least time by these figures.  Rounds of workgroups follow each other, a launch and a round's
+// begin and end take some 4 us; parts cost a launch of 3 us and are written, read and joined at 4 bytes each.  With
+// the tiles alone to choose from, 5366 x (576x12736) took 98 us in 420 tiles of 64x128, where two parts of 210 tiles
+// of 128x128 take 75; 64 x (4096x14336) takes 33 us in 64 tiles and 15 in four parts of them.
+template <int N>
+Cut cut_product(const Tile (&kinds)[N], uint64_t m, uint64_t cols, uint64_t units_of, uint64_t steps_per_unit,
+                uint64_t least) {
+  const uint32_t cus = nz_compute_units();
+  const float scale = cus ? cus / 256.0f : 1.0f;
+  Cut best = {};
+  float best_time = 0;
+  for (const Tile& t : kinds) {
+    const uint64_t mt = nz_ceil_div(m, t.bm), nt = nz_ceil_div(cols, t.bn);
+    const float slots = t.slots * scale;
+    for (uint64_t want = 1; want <= 16; ++want) {
+      const uint64_t length = nz_ceil_div(units_of, want), parts = nz_ceil_div(units_of, length);
+      if (parts != want || (parts > 1 && length < least)) continue;
+      const float groups = (float)(mt * nt * parts), rounds = floorf(groups / slots), rest = groups - rounds * slots;
+      float time = (rounds * t.full + (rest == 0 ? 0.0f : rest <= slots / 2 ? t.half : t.full)) *
+                       (float)(length * steps_per_unit) +
+                   4.0f * (rounds + (rest > 0));
+      if (parts > 1) time += 3.0f + (float)parts * (float)m * (float)cols * (12.0f / 5e6f);
+      if (best.parts == 0 || time < best_time) {
+        best = Cut{t.bm, t.bn, (uint32_t)parts, (uint32_t)length, (uint32_t)mt, (uint32_t)nt};
+        best_time = time;
+      }
+    }
+  }
+  return best;
 }
 
-uint64_t tiles(uint64_t m, uint64_t n, uint32_t bm, uint32_t bn) { return nz_ceil_div(m, bm) * nz_ceil_div(n, bn); }
+// The product of 8-bit rows, cut along k by groups of four steps, two at least.
+Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
+  return cut_product(kTiles, m, n, nz_ceil_div(k, kGroup), 4, 2);
+}
+
+// The products of 16-bit rows, in steps of 64.
+Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) { return cut_product(kTiles16, m, cols, steps, 1, 8); }
 
 uint64_t units() {
   const uint32_t cus = nz_compute_units();
   return cus ? cus : 256;
-}
-
-// The product of 8-bit rows: the largest tile that leaves enough workgroups; the smallest is cut along k as well,
-// into parts of 1024 values at least.
-Cut cut_product(uint64_t m, uint64_t n, uint64_t k) {
-  const uint64_t cus = units(), groups = nz_ceil_div(k, kGroup);
-  if (tiles(m, n, 128, 256) >= 4 * cus) return cut_into(128, 256, m, n, groups, 1);
-  if (tiles(m, n, 128, 128) * 2 >= 3 * cus) return cut_into(128, 128, m, n, groups, 1);
-  if (tiles(m, n, 64, 128) * 2 >= cus) return cut_into(64, 128, m, n, groups, 1);
-  const uint64_t t = tiles(m, n, 64, 64), parts = (cus + t / 2) / t, most = groups / 2;
-  return cut_into(64, 64, m, n, groups, parts < most ? parts : most);
-}
-
-// The products of 16-bit rows, in steps of 64.
-Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) {
-  const uint64_t cus = units();
-  if (tiles(m, cols, 256, 128) * 2 >= cus) return cut_into(256, 128, m, cols, steps, 1);
-  const uint64_t t = tiles(m, cols, 64, 64), parts = (2 * cus + t / 2) / t, most = steps / 8;
-  return cut_into(64, 64, m, cols, steps, parts < most ? parts : most);
 }
 
 void launch_join(const float* part, const Cut& c, uint64_t m, uint64_t n, const void* bias, void* y, int dtype,
@@ -1034,7 +1058,7 @@ Room product_room(uint64_t m, uint64_t n, uint64_t k, int dtype) {
     r.bytes = r.parts + cut_product16(m, n, pad / 64).part_bytes(m, n);
   } else {
     r.parts = r.values;
-    r.bytes = r.parts + cut_product(m, n, k).part_bytes(m, n);
+    r.bytes = r.parts + cut_product8(m, n, k).part_bytes(m, n);
   }
   return r;
 }
@@ -1049,7 +1073,7 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, c
     return launch_tiles16<false>(cut_product16(m, n, pad / 64), workspace + room.values, pad, m, wd, ws, n, k, pad / 64,
                                  1, n, bias, y, dtype, workspace + room.parts, st);
   }
-  const Cut c = cut_product(m, n, k);
+  const Cut c = cut_product8(m, n, k);
   float* part = c.parts > 1 ? (float*)(workspace + room.parts) : nullptr;
   if (dtype == NZ_DTYPE_BF16)
     launch_tiles(c, xd, xs, m, wd, ws, n, k, (const nz_bf16*)bias, (nz_bf16*)y, part, st);
