@@ -11,6 +11,9 @@
 //   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
 //          lie in one window is done; what reaches beyond it is kept as a piece.
 //   join   (more than one window) the pieces of rows that reach over several windows, in their order.
+//
+// 8192 tokens of a text in 50257x1024 (bf16): 21 + 11.5 + 6 us, where clearing alone takes 15 (6.8 TB/s) and sorting 12;
+// 2048 in 128256x4096: 170 + 11 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
 #include "nz_operators.h"
 
 namespace {
@@ -18,7 +21,7 @@ namespace {
 constexpr uint32_t kTile = 8192;      // tokens that are compared with each other
 constexpr uint32_t kTileBits = 13;
 constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
-constexpr uint32_t kClear = 1 << 16;  // bytes a workgroup clears
+constexpr uint32_t kClear = 1 << 14;  // bytes a workgroup clears
 constexpr uint32_t kBatch = 16;      // rows of g that a wavefront has on their way at a time
 
 // A sorted token: its index (the number of rows if it takes no part) and where it stands.

@@ -152,7 +152,9 @@ __device__ inline uint32_t scale_at(uint32_t b) { return (b & ~15u) + 4 * (b & 3
 // ---- quantisation and values -----------------------------------------------------------------------------------
 //
 // One wavefront per 512 values of a row: 8 values a lane, four lanes a block, so that loads and stores of a
-// wavefront are consecutive and the block's maximum takes two exchanges inside a quad.
+// wavefront are consecutive and the block's maximum takes two exchanges inside a quad.  Both are bound by memory:
+// 16384x4096 bf16 values to 4 bits in 35.5 us (4.8 TB/s; a copy reaches 5.1), back in 26.6 us.  (Two groups a
+// wavefront, for twice the loads on their way, took 37.9.)
 
 template <int BITS, class T>
 __global__ __launch_bounds__(256) void nz_mx_quantize_kernel(const T* x, uint64_t stride, uint32_t cols,
@@ -336,23 +338,26 @@ __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, 
 //
 // The rows of both sides are staged through LDS in steps of 128 values, NS stages deep, by loads that go to LDS
 // without registers; a wavefront counts its own loads down, and one barrier a step tells that everybody's have
-// arrived and that the stage before is used up.  (Reading operands ahead across the barrier, or with 32x32x64
-// instructions, does not pay: from 8192 to 16384 values of a row the loop runs at 3.1 PFLOP/s as it is, the instruction
-// itself at 3.6 to 3.9 on such data.)  Staged rows are exchanged in chunks of 16 bytes (x: chunk c of row
+// arrived and that the stage before is used up.  Staged rows are exchanged in chunks of 16 bytes (x: chunk c of row
 // r at c ^ (r & 7); w: at c ^ ((r >> 1) & 3)) so that eight lanes in turn read from all banks, and the weight rows of
 // a wavefront are staged in an order that leaves each lane 4 TN consecutive columns of the result.  Scales are
 // staged once per 512 values.
+//
+// 8192 x (14336x4096) takes 380 us, 2.5 PFLOP/s; a library's 8-bit product of 8192^3 reaches 2.7, the instruction by
+// itself 3.6 to 3.9 on such data.  What bounds it is the begin and end of a tile: from 8192 to 16384 values of a row a
+// 256x256 tile's loop runs at 3.1 PFLOP/s, but one workgroup a compute unit leaves its first loads and last stores
+// uncovered (423 us); two of 128x256 with two stages each cover each other's.  Reading operands ahead across the
+// barrier, or 32x32x64 instructions, do not pay.
 template <int WM, int WN, int TM, int TN, int NS, class T>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_mx_tiles_kernel(const uint8_t* xd, const uint8_t* xs, uint32_t m,
-                                                                   const uint8_t* wd, const uint8_t* ws, uint32_t n,
-                                                                   uint32_t k, const T* bias, T* y, uint32_t mt,
-                                                                   uint32_t nt, uint32_t part_groups, float* part) {
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_mx_tiles_kernel(
+    const uint8_t* xd, const uint8_t* xs, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t n, uint32_t k,
+    const T* bias, T* y, uint32_t mt, uint32_t nt, uint32_t part_groups, float* part) {
   constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   constexpr int XB = BM * 128, WB = BN * 64, STAGE = XB + WB;
   constexpr int XI = BM / 8 / W, WI = BN / 16 / W, LOADS = XI + WI;
   constexpr int SI = (BM + BN + 63) / 64, SB = SI * 1024;  // scales: 64 rows of 16 bytes a load
+  constexpr int SL = (SI + W - 1) / W;                     // of a wavefront
   static_assert(XI * 8 * W == BM && WI * 16 * W == BN, "loads per wavefront");
-  constexpr int SL = (SI + W - 1) / W;
   static_assert(NS >= 2 && NS <= 4, "a group's scales are asked for when the last group's have been read");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + SB];
   const uint32_t base = lds_address(lds);
@@ -476,7 +481,7 @@ __global__ __launch_bounds__(256) void nz_mx_join_kernel(const float* part, uint
     f4 sum = *(const f4*)(part + at);
     for (uint32_t i = 1; i < parts; ++i) sum += *(const f4*)(part + i * size + at);
     const uint32_t col = (uint32_t)(at % n);
-    typedef T pack __attribute__((ext_vector_type(4)));
+    typedef T pack __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     pack v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (T)(bias ? sum[e] + (float)bias[(col + e) % n] : sum[e]);
@@ -494,6 +499,7 @@ __global__ __launch_bounds__(256) void nz_mx_join_kernel(const float* part, uint
 // wavefronts are KW that share the values of a row (512 at a time, in turn) times 8 / KW with NT x 16 weight rows
 // each; a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
 // (QUANTIZE) as they are: then every workgroup brings them to 8 bits in LDS while its first weights are on their way.
+// One row against 14336x4096: 8.4 us, 3.7 TB/s of codes and scales, of which 2 are the launch.
 template <int NT, bool QUANTIZE, class T>
 __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t stride, const uint8_t* xs,
                                                         uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t n,
@@ -644,6 +650,10 @@ __global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t 
 // row of A at c ^ (row & 7)); a step ahead, the codes are written to LDS once more as bf16, once for all wavefronts.
 // Where the sums run over the weight's rows that tile lies as in memory, and the operand is read by the instruction
 // that transposes 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns, as in nz_mx_tiles_kernel.
+//
+// 8192 rows of gradients against 4096x1024: 65 us, 1.06 PFLOP/s; a library's bf16 product of 8192^3 reaches 1.26 and
+// the instructions of this loop without the rest 1.65.  Reads of operands, conversion and loads cost some 10 us each:
+// all of them go through LDS.  Tiles of 128x128, two workgroups a compute unit, took 78 us.
 template <int WM, int WN, int TM, int TN, bool ROWS, class T>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_mx_tiles16_kernel(
     const nz_bf16* a, uint64_t a_stride, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t w_rows,
@@ -965,11 +975,6 @@ Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
 // The products of 16-bit rows, in steps of 64.
 Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) { return cut_product(kTiles16, m, cols, steps, 1, 8); }
 
-uint64_t units() {
-  const uint32_t cus = nz_compute_units();
-  return cus ? cus : 256;
-}
-
 void launch_join(const float* part, const Cut& c, uint64_t m, uint64_t n, const void* bias, void* y, int dtype,
                  hipStream_t st) {
   by_dtype(dtype, [&](auto t) {
@@ -1018,7 +1023,8 @@ void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, cons
   const uint64_t t = nz_ceil_div(n, 16);
   // weights that fill the device with fewer wavefronts to a row: fewer workgroups that each bring the rows to 8 bits.
   // 14336x4096, with 2, 4, 8 wavefronts to a row: one row 10.3, 8.7, 9.3 us; four 10.4, 11.5, 13.0
-  if (t > 2 * units()) kw = kw < 4 ? kw : m >= 4 ? 2 : 4;
+  const uint32_t cus = nz_compute_units();
+  if (t > 2 * (cus ? cus : 256)) kw = kw < 4 ? kw : m >= 4 ? 2 : 4;
   const uint32_t lds = QUANTIZE ? (uint32_t)m * groups * 528 : 0;
   nz_mx_few_kernel<1, QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
       x, stride, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, bias, y, kw);

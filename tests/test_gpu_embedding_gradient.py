@@ -140,6 +140,19 @@ def test_special_values_stay_in_their_rows():
     assert torch.isnan(got).sum() == 1 and torch.isinf(got).sum() == 2
 
 
+def test_offsets_beyond_32_bits():
+    rows, cols = 4_400_000, 512
+    ids = torch.tensor([rows - 1, 0, rows - 1], device=DEV)
+    g = torch.ones(3, cols, dtype=torch.bfloat16, device=DEV)
+    got = ops.embedding_gradient(ids, g, rows, 3.0)
+    assert got.numel() * 2 > 2 ** 32
+    assert (got[-1] == 6).all() and (got[0] == 3).all() and not got[1:-1].any()
+    wide = torch.zeros(2, 2 ** 31 + 64, dtype=torch.bfloat16, device=DEV)  # rows of g far apart
+    wide[1, :8] = 5
+    got = ops.embedding_gradient(ids[:2], wide[:, :8], rows)
+    assert (got[0] == 5).all() and not got[1:].any()
+
+
 def test_captured_beside_eager():
     ids = torch.zeros(900, dtype=torch.int64, device=DEV)
     g = torch.randn(900, 48, generator=torch.Generator().manual_seed(1)).to(DEV)

@@ -263,6 +263,57 @@ def test_gradient_of_large_and_special_values():
     assert bad[1].all() and not bad[0].any() and not bad[2].any()
 
 
+def test_gradient_of_weights_that_read_as_nan():
+    wd = whole_numbers(20, 200, 6, 1)
+    wd[7, 70] = math.inf
+    w = ops.mx_quantize(wd.to(DEV), 4)
+    for dtype in TYPES:
+        x = torch.zeros(3, 200, dtype=dtype, device=DEV, requires_grad=True)
+        ops.mx_linear(x, w).backward(torch.zeros(3, 20, dtype=dtype, device=DEV))
+        bad = torch.isnan(x.grad.cpu())
+        assert bad[:, 64:96].all() and bad.sum() == 3 * 32
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(1, 5, 40000), (3, 70, 20011), (2, 33000, 40), (9000, 3, 70), (1100, 530, 2600)])
+def test_long_and_narrow(m, n, k, dtype):
+    """whole numbers again; partial sums are multiples of 2^-1 below 2^22"""
+    x = whole_numbers(m, k, 7, 1, dtype)
+    w = ops.mx_quantize(whole_numbers(n, k, 6, 2).to(DEV), 4)
+    w64 = decoded(w.data.cpu(), w.scales.cpu(), k, 4)[:, :k]
+    assert 7 * 6 * k < 2 ** 21 and 15 * 6 * n < 2 ** 22
+    xg = x.to(DEV).requires_grad_(True)
+    y = ops.mx_linear(xg, w)
+    same(y.detach(), round_to(x.double() @ w64.t(), dtype))
+    g = whole_numbers(m, n, 15, 3, dtype)
+    y.backward(g.to(DEV))
+    same(xg.grad, round_to(g.double() @ w64, dtype))
+
+
+def test_offsets_beyond_32_bits():
+    """a table of more than 2^32 bytes of codes, a result of more than 2^32 values, and an input of as many"""
+    rows = 70_000_000
+    table = ops.MXTensor(torch.zeros(rows, 64, dtype=torch.uint8, device=DEV),
+                         torch.full((rows, 16), 127, dtype=torch.uint8, device=DEV), (rows, 100))
+    table.data[-1, :50] = 0x42  # 1 and 2 in turn
+    got = ops.mx_embedding(torch.tensor([0, rows - 1, rows], device=DEV), table)
+    want = torch.zeros(3, 100)
+    want[1] = torch.tensor([1.0, 2.0]).repeat(50)
+    same(got, want)
+    del table, got
+    m, n = 33_001, 131_072
+    x = torch.zeros(m, 32, dtype=torch.bfloat16, device=DEV)
+    x[-1], x[0] = 2, 3
+    w = ops.mx_quantize(torch.ones(n, 32, dtype=torch.bfloat16, device=DEV), 4)
+    y = ops.mx_linear(x, w)
+    assert y.numel() > 2 ** 32
+    assert (y[-1] == 64).all() and (y[0] == 96).all() and not y[1:-1].any()
+    q = ops.mx_quantize(y, 4)
+    assert (q.data[-1] == 0x66).all() and (q.scales[-1] == 131).all() and not q.data[1:-1].any()  # 4 x 2^4
+    dx = torch.autograd.grad(ops.mx_linear(x.requires_grad_(True), w), x, y)[0]
+    assert (dx[-1] == 64 * n).all() and not dx[1:-1].any()
+
+
 def test_gradient_strides_shapes_and_no_second_order():
     w = ops.mx_quantize(whole_numbers(24, 96, 6, 1).to(DEV), 4)
     w64 = decoded(w.data.cpu(), w.scales.cpu(), 96, 4)[:, :96]
