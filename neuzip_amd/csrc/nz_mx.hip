@@ -496,37 +496,29 @@ __global__ __launch_bounds__(256) void nz_mx_join_kernel(const float* part, uint
 }
 
 // Up to 16 rows, where reading the weight is all that counts: no staging and no barrier in the way of it.  The eight
-// wavefronts are KW that share the values of a row (512 at a time, in turn) times 8 / KW with NT x 16 weight rows
-// each; a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
+// wavefronts are kw that share the values of a row (512 at a time, in turn) times 8 / kw with 16 weight rows each;
+// a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
 // (QUANTIZE) as they are: then every workgroup brings them to 8 bits in LDS while its first weights are on their way.
 // One row against 14336x4096: 8.4 us, 3.7 TB/s of codes and scales, of which 2 are the launch.
-template <int NT, bool QUANTIZE, class T>
+template <bool QUANTIZE, class T>
 __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t stride, const uint8_t* xs,
                                                         uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t n,
                                                         uint32_t k, const T* bias, T* y, uint32_t kw) {
   extern __shared__ __attribute__((aligned(16))) uint8_t few_lds[];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
   const uint32_t steps = (k + kStep - 1) / kStep, groups = (k + kGroup - 1) / kGroup;
-  const uint32_t kwave = wave % kw, tile0 = (blockIdx.x * (8 / kw) + wave / kw) * NT;
-  const uint8_t* wp[NT];
-  const uint8_t* sp[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const uint64_t row = min((tile0 + j) * 16 + r, n - 1);
-    wp[j] = wd + row * (steps * 64ull) + g * 16;
-    sp[j] = ws + row * (groups * 16ull) + g * 4;
-  }
+  const uint32_t kwave = wave % kw, tile = blockIdx.x * (8 / kw) + wave / kw;
+  const uint64_t w_row = min(tile * 16 + r, n - 1);
+  const uint8_t* wp = wd + w_row * (steps * 64ull) + g * 16;
+  const uint8_t* sp = ws + w_row * (groups * 16ull) + g * 4;
   struct Held {
-    i4v w[NT][4];
-    uint32_t s[NT];
+    i4v w[4];
+    uint32_t s;
   } a, b;
   const auto load = [&](Held& h, uint32_t group) {
+    h.s = *(const uint32_t*)(sp + group * 16);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      h.s[j] = *(const uint32_t*)(sp[j] + group * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h.w[j][i] = *(const i4v*)(wp[j] + (uint64_t)min(group * 4 + i, steps - 1) * 64);
-    }
+    for (int i = 0; i < 4; ++i) h.w[i] = *(const i4v*)(wp + (uint64_t)min(group * 4 + i, steps - 1) * 64);
   };
   if (kwave < groups) load(a, kwave);
 
@@ -551,9 +543,7 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
     xp = (const uint8_t*)x + row * (steps * 128ull) + g * 16;
     xsp = xs + row * (groups * 16ull) + g * 4;
   }
-  f4 acc[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = f4{0, 0, 0, 0};
+  f4 acc = {0, 0, 0, 0};
   const auto multiply = [&](const Held& h, uint32_t group) {
     const uint32_t sx = *(const uint32_t*)(xsp + group * (QUANTIZE ? 528 : 16));
     const auto one = [&](auto b4) {
@@ -561,8 +551,7 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
       if (group * 4 + i >= steps) return;
       const uint8_t* p = xp + (QUANTIZE ? group * 528 : (uint64_t)group * 512) + i * 128;
       const i4v x0 = *(const i4v*)p, x1 = *(const i4v*)(p + 64);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = step(h.w[j][i], x0, x1, acc[j], h.s[j], sx, i);
+      acc = step(h.w[i], x0, x1, acc, h.s, sx, i);
     };
     one(std::integral_constant<int, 0>());
     one(std::integral_constant<int, 1>());
@@ -579,16 +568,15 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
   // the wavefronts that share rows add up in their order
   __syncthreads();
   float* part = (float*)few_lds;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) *(f4*)(part + ((wave * NT + j) * 16 + r) * 16 + g * 4) = acc[j];
+  *(f4*)(part + (wave * 16 + r) * 16 + g * 4) = acc;
   __syncthreads();
-  const uint32_t tiles = 8 / kw * NT;
+  const uint32_t tiles = 8 / kw;
   for (uint32_t i = threadIdx.x; i < m * tiles * 16; i += 512) {
     const uint32_t to = i / (tiles * 16), c = i - to * (tiles * 16), t = c / 16;
     const uint32_t col = blockIdx.x * tiles * 16 + c;
     if (col >= n) continue;
     float sum = 0;
-    for (uint32_t q = 0; q < kw; ++q) sum += part[(((t / NT * kw + q) * NT + t % NT) * 16 + to) * 16 + c % 16];
+    for (uint32_t q = 0; q < kw; ++q) sum += part[((t * kw + q) * 16 + to) * 16 + c % 16];
     if (bias) sum += (float)bias[col];
     y[(uint64_t)to * n + col] = (T)sum;
   }
@@ -603,7 +591,6 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
 // side by side along the summed axis.
 
 typedef nz_bf16 b8v __attribute__((ext_vector_type(8)));
-typedef nz_bf16 b4v __attribute__((ext_vector_type(4)));
 typedef nz_bf16 b2v __attribute__((ext_vector_type(2)));
 typedef short s4v __attribute__((ext_vector_type(4)));
 
@@ -1026,7 +1013,7 @@ void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, cons
   const uint32_t cus = nz_compute_units();
   if (t > 2 * (cus ? cus : 256)) kw = kw < 4 ? kw : m >= 4 ? 2 : 4;
   const uint32_t lds = QUANTIZE ? (uint32_t)m * groups * 528 : 0;
-  nz_mx_few_kernel<1, QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
+  nz_mx_few_kernel<QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
       x, stride, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, (uint32_t)n, k, bias, y, kw);
 }
 

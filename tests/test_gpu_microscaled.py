@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import neuzip_amd
-from neuzip_amd import ops
+from neuzip_amd import _lib, ops
 from mx_oracle import HALF_STEP, decoded, held, round_to
 
 pytestmark = pytest.mark.gpu
@@ -290,6 +290,27 @@ def test_long_and_narrow(m, n, k, dtype):
     same(xg.grad, round_to(g.double() @ w64, dtype))
 
 
+# the larger tiles, whole and in parts, each with ragged ends
+LARGE = [(4100, 4099, 300), (2050, 1030, 2060), (1100, 1300, 2100), (1500, 2000, 600), (5001, 1537, 777),
+         (65, 1368, 8241), (2712, 130, 11041), (2775, 1437, 8752), (140, 1129, 5803), (145, 364, 5490), (2003, 2500, 1030)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_products_of_whole_numbers(m, n, k, dtype):
+    """partial sums are multiples of 2^-1 below 2^22: exact in 32 bits in any order, and in 64"""
+    x = whole_numbers(m, k, 7, 1, dtype).to(DEV).requires_grad_(True)
+    w = ops.mx_quantize(whole_numbers(n, k, 6, 2).to(DEV), 4)
+    bias = whole_numbers(1, n, 99, 3, dtype)[0].to(DEV).requires_grad_(True)
+    w64 = decoded(w.data.cpu(), w.scales.cpu(), k, 4)[:, :k].to(DEV)
+    assert 7 * 6 * k < 2 ** 21 and 15 * 6 * n < 2 ** 22
+    y = ops.mx_linear(x, w, bias)
+    same(y.detach(), round_to((x.detach().double() @ w64.t() + bias.detach().double()).cpu(), dtype))
+    g = whole_numbers(m, n, 15, 4, dtype).to(DEV)
+    y.backward(g)
+    same(x.grad, round_to((g.double() @ w64).cpu(), dtype))
+
+
 def test_offsets_beyond_32_bits():
     """a table of more than 2^32 bytes of codes, a result of more than 2^32 values, and an input of as many"""
     rows = 70_000_000
@@ -435,6 +456,46 @@ def test_rows_of_one_quantisation_serve_several_weights():
     for n in (16, 100):
         w = ops.mx_quantize(rnd(n, 256, seed=n).to(DEV), 4)
         same(ops.mx_linear(x8, w, dtype=torch.float16), ops.mx_linear(x, w))
+
+
+def guarded(rows, cols, dtype, past=5):
+    """rows x cols that start one element behind a 16-byte boundary, and what stands round them"""
+    whole = torch.full((rows * cols + 1 + past,), 9.0, dtype=dtype, device=DEV)
+    return whole, whole[1:1 + rows * cols].view(rows, cols)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(1, 33, 515), (3, 64, 512), (40, 96, 1025), (70, 128, 2048), (64, 4096, 2112),
+                                   (2712, 130, 11041)])
+def test_dense_pointers_need_their_elements_alignment_only(m, n, k, dtype):
+    """the native calls, on memory that begins between vectors; nothing round the results is written"""
+    L, code = _lib.load(), {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}.get(dtype, _lib.DTYPE_F32)
+    stream = torch.cuda.current_stream().cuda_stream
+    w = ops.mx_quantize(whole_numbers(n, k, 6, 2).to(DEV), 4)
+    x, g, bias = (guarded(*size, dtype)[1] for size in ((m, k), (m, n), (1, n)))
+    for t, most, seed in ((x, 7, 3), (g, 15, 4), (bias, 99, 5)):
+        t.copy_(whole_numbers(*t.shape, most, seed, dtype))
+    (y_all, y), (dx_all, dx) = guarded(m, n, dtype), guarded(m, k, dtype)
+
+    room = torch.empty(max(16, L.nz_mx_linear_workspace_bytes(m, n, k, code)), dtype=torch.uint8, device=DEV)
+    _lib.raise_for(L.nz_mx_linear(x.data_ptr(), code, m, k, k, w.data.data_ptr(), w.scales.data_ptr(), n,
+                                  bias.data_ptr(), y.data_ptr(), room.data_ptr(), room.numel(), stream))
+    same(y, ops.mx_linear(x.clone(), w, bias[0].clone()))
+
+    need = L.nz_mx_linear_grad_workspace_bytes(g.data_ptr(), code, m, n, n, k)
+    room = torch.empty(max(16, need), dtype=torch.uint8, device=DEV)
+    _lib.raise_for(L.nz_mx_linear_grad(g.data_ptr(), code, m, n, n, w.data.data_ptr(), w.scales.data_ptr(), k,
+                                       dx.data_ptr(), room.data_ptr(), room.numel(), stream))
+    xg = x.clone().requires_grad_(True)
+    ops.mx_linear(xg, w).backward(g.clone())
+    same(dx, xg.grad)
+
+    q_all, back = guarded(m, k, dtype)
+    x4 = ops.mx_quantize(x, 4)
+    _lib.raise_for(L.nz_mx_dequantize(x4.data.data_ptr(), x4.scales.data_ptr(), m, k, 4, back.data_ptr(), code, stream))
+    same(back, x4.dequantize(dtype))
+    for whole in (y_all, dx_all, q_all):
+        assert whole[0] == 9 and (whole[-5:] == 9).all()
 
 
 def test_calls_on_another_stream():
