@@ -6,14 +6,16 @@
 //
 //   sort   32 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller keys (index, then
 //          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
-//          the same place every time.
+//          the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
 //   merge  (more than one tile) the place among all tokens: the same count in the other tiles, by bisection.
 //   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
 //          lie in one window is done; what reaches beyond it is kept as a piece.
-//   join   (more than one window) the pieces of rows that reach over several windows, in their order.
+//   join   the pieces of rows that reach over several windows, in their order.
 //
-// 8192 tokens of a text in 50257x1024 (bf16): 21 + 11.5 + 6 us, where clearing alone takes 15 (6.8 TB/s) and sorting 12;
-// 2048 in 128256x4096: 170 + 11 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
+// Few tokens are not sorted but compared with each other where they are added up.
+//
+// 8192 tokens of a text in 50257x1024 (bf16): 16.7 + 11.6 + 5.5 us, where clearing alone takes 15 (6.8 TB/s); 2048 in
+// 128256x4096: 167 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
 #include "nz_operators.h"
 
 namespace {
@@ -22,7 +24,8 @@ constexpr uint32_t kTile = 8192;      // tokens that are compared with each othe
 constexpr uint32_t kTileBits = 13;
 constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
 constexpr uint32_t kClear = 1 << 14;  // bytes a workgroup clears
-constexpr uint32_t kBatch = 16;      // rows of g that a wavefront has on their way at a time
+constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
+constexpr uint32_t kFew = 2048;       // tokens that may go unsorted
 
 // A sorted token: its index (the number of rows if it takes no part) and where it stands.
 struct Place {
@@ -51,35 +54,44 @@ __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long*
   }
   typedef Key key4 __attribute__((ext_vector_type(4)));
   __shared__ __attribute__((aligned(32))) Key keys[kTile];
-  __shared__ uint32_t smaller[8][64];
+  __shared__ uint32_t smaller[8][kSorted];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
   const uint32_t block = blockIdx.x % (kTile / kSorted), base = blockIdx.x / (kTile / kSorted) * kTile;
-  const uint32_t here = min(kTile, count - base), blocks = (here + 31) / 32;
-  for (uint32_t i = threadIdx.x; i < blocks * 32; i += 512) {
-    const long long v = i < here ? index[base + i] : -1;
+  const uint32_t here = min(kTile, count - base), rounds = (here + 255) / 256;
+  long long value[kTile / 512];
+#pragma unroll
+  for (uint32_t j = 0; j < kTile / 512; ++j)  // all on their way at once
+    if (j * 512 < here) value[j] = index[base + min(j * 512 + threadIdx.x, here - 1)];
+#pragma unroll
+  for (uint32_t j = 0; j < kTile / 512; ++j) {
+    const uint32_t i = j * 512 + threadIdx.x;
+    const long long v = i < here ? value[j] : -1;
     const uint32_t row = v >= 0 && v < (long long)rows && v != skip ? (uint32_t)v : rows;
-    keys[i] = (Key)row << kTileBits | i;
+    if (j * 512 < here) keys[i] = (Key)row << kTileBits | i;
   }
   __syncthreads();
-  // the two halves of a wavefront hold the same tokens and look at another sixteenth of the keys each
-  const uint32_t i = block * kSorted + lane % kSorted, part = wave * 2 + lane / kSorted;
-  const Key mine = keys[i];
-  uint32_t less = 0;
-  const uint32_t first = blocks * part / 16, last = blocks * (part + 1) / 16;
-  for (uint32_t b = first; b < last; ++b) {
+  // a lane holds four of the tokens; eight lanes hold them all, and look at every 64th four of the keys
+  key4 mine = *(const key4*)(keys + block * kSorted + lane % 8 * 4);
+  uint32_t less[4] = {};
+  for (uint32_t r = 0; r < rounds; ++r) {
+    const key4 k = *(const key4*)(keys + r * 256 + wave * 32 + lane / 8 * 4);
 #pragma unroll
-    for (uint32_t j = 0; j < 32; j += 4) {
-      const key4 k = *(const key4*)(keys + b * 32 + j);
-      less += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
-    }
+    for (int e = 0; e < 4; ++e) less[e] += (k.x < mine[e]) + (k.y < mine[e]) + (k.z < mine[e]) + (k.w < mine[e]);
   }
-  smaller[wave][lane] = less;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    less[e] += __shfl_xor(less[e], 8);
+    less[e] += __shfl_xor(less[e], 16);
+    less[e] += __shfl_xor(less[e], 32);
+    if (lane < 8) smaller[wave][lane * 4 + e] = less[e];
+  }
   __syncthreads();
+  const uint32_t i = block * kSorted + threadIdx.x;
   if (threadIdx.x >= kSorted || i >= here) return;
-  less = 0;
+  uint32_t at = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < 8; ++w) less += smaller[w][lane] + smaller[w][lane + kSorted];
-  places[base + less] = Place{(uint32_t)(mine >> kTileBits), base + i};
+  for (uint32_t w = 0; w < 8; ++w) at += smaller[w][threadIdx.x];
+  places[base + at] = Place{(uint32_t)(keys[i] >> kTileBits), base + i};
 }
 
 // tokens of a sorted tile whose index is less than `row`
@@ -269,10 +281,91 @@ __global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* pla
   if (k.n) put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
 }
 
+// Few tokens, without sorting them: one workgroup per 512 columns of a token looks for the token's index among
+// all of them (a quarter a wavefront).  Where it is the first of its row it adds up the row, again a quarter of the
+// tokens a wavefront if there are many, in their order; else it is done.
+template <class T>
+__global__ __launch_bounds__(256) void nz_embedding_few_kernel(const long long* index, uint32_t count, uint32_t rows,
+                                                               long long skip, const T* g, uint64_t stride,
+                                                               uint32_t cols, uint32_t slices, float scale,
+                                                               uint32_t flags, T* out) {
+  constexpr uint32_t kQuarter = kFew / 4;
+  __shared__ uint32_t found[4];
+  __shared__ uint16_t list[4][kQuarter];
+  __shared__ float sums[3][64][9];  // a ninth: lanes apart in their banks
+  const uint32_t token = blockIdx.x / slices, lane = threadIdx.x & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const long long row = index[token];
+  if (row < 0 || row >= (long long)rows || row == skip) return;
+  bool hit[kQuarter / 64];
+#pragma unroll
+  for (uint32_t j = 0; j < kQuarter / 64; ++j) {
+    const uint32_t at = wave * kQuarter + j * 64 + lane;
+    hit[j] = index[min(at, count - 1)] == row && at < count;
+  }
+  uint32_t n = 0;
+  bool earlier = false;
+#pragma unroll
+  for (uint32_t j = 0; j < kQuarter / 64; ++j) {
+    const uint32_t at = wave * kQuarter + j * 64;
+    const uint64_t mask = __ballot(hit[j]);
+    earlier |= mask && at + __builtin_ctzll(mask) < token;
+    if (hit[j]) list[wave][n + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(at + lane);
+    n += __popcll(mask);
+  }
+  if (lane == 0) found[wave] = earlier ? ~0u : n;
+  __syncthreads();
+  uint32_t upto[4];
+  n = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < 4; ++w) {
+    const uint32_t of = __builtin_amdgcn_readfirstlane(found[w]);
+    if (of == ~0u) return;
+    upto[w] = n += of;
+  }
+  const auto token_at = [&](uint32_t i) -> uint64_t {
+    const uint32_t w = (i >= upto[0]) + (i >= upto[1]) + (i >= upto[2]);
+    return __builtin_amdgcn_readfirstlane((uint32_t)list[w][w ? i - upto[w - 1] : i]);
+  };
+  const uint32_t share = n <= 16 ? 16 : (n + 3) / 4, first = min(n, wave * share), last = min(n, first + share);
+  const Columns k = columns_of(blockIdx.x - token * slices, lane, cols);
+  float sum[8] = {};
+  for (uint32_t i = first; i < last; i += 8) {
+    float v[8][8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (i + j < last) load8(g + token_at(i + j) * stride, k, cols, v[j]);
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+      if (i + j < last)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += v[j][e];
+  }
+  if (n > 16) {
+    if (wave)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[wave - 1][lane][e] = sum[e];
+    __syncthreads();
+    if (wave == 0)
+#pragma unroll
+      for (uint32_t w = 0; w < 3; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += sums[w][lane][e];
+  }
+  if (wave == 0 && k.n) put8(out + (uint64_t)row * cols, k, cols, sum, n, scale, flags);
+}
+
 uint64_t align256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 // Places a window holds: few while there are few tokens, for the sake of many wavefronts.
 uint32_t window_of(uint64_t count) { return count <= 32768 ? kBatch : 4 * kBatch; }
+
+// Whether tokens are few enough to be compared with each other for each 512 columns; what that reads is 8 count^2
+// slices bytes.  (30000x512, bf16, against sorting: 300 tokens 13 and 19 us, 2048 19.4 and 19.4; 8000x256, 1000 tokens
+// 10 and 17, 2048 15 and 18, 3000 22 and 19; with 2048 tokens in eight slices the sums alone take 34 and 16.)
+bool unsorted(uint64_t count, uint64_t cols) {
+  return count <= kFew && count * count * nz_ceil_div(cols, 512) <= (uint64_t)kFew * kFew;
+}
 
 // Where the workspace holds what: sorted tiles (more than one), places, pieces.
 struct Room {
@@ -280,10 +373,11 @@ struct Room {
 };
 Room room_of(uint64_t count, uint64_t cols) {
   const uint64_t window = window_of(count);
-  Room r;
+  Room r = {};
+  if (unsorted(count, cols)) return r;
   r.places = count > kTile ? align256(count * sizeof(Place)) : 0;
   r.pieces = r.places + align256(count * sizeof(Place));
-  r.bytes = r.pieces + (count > window ? nz_mul(nz_ceil_div(count, window) * 2 * 4, cols) : 0);
+  r.bytes = r.pieces + nz_mul(nz_ceil_div(count, window) * 2 * 4, cols);
   return r;
 }
 
@@ -309,48 +403,57 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   if ((uintptr_t)dev_indices % 8 || (uintptr_t)dev_g % size || (uintptr_t)dev_out % size)
     return nz_fail(NZ_ERR_ALIGN, "pointers must be aligned to their elements");
   const Room room = room_of(count, cols);
-  if (count) {
+  if (room.bytes) {
     if (workspace_bytes < room.bytes) return nz_fail(NZ_ERR_CAPACITY, "workspace too small");
     if (!dev_workspace || (uintptr_t)dev_workspace % 16) return nz_fail(NZ_ERR_ALIGN, "misaligned workspace");
   }
   const uint64_t bytes = flags & NZ_GRAD_ACCUMULATE ? 0 : rows * cols * size, clearers = nz_ceil_div(bytes, kClear);
-  const uint32_t sorters = (uint32_t)nz_ceil_div(count, kSorted);
+  const bool few = unsorted(count, cols);
+  const uint32_t sorters = few ? 0 : (uint32_t)nz_ceil_div(count, kSorted);
   if (clearers + sorters > 0x7FFFFFFFull) return nz_fail(NZ_ERR_ARG, "table too large for one launch");
-  if (clearers + sorters == 0) return NZ_OK;
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)dev_workspace;
   Place *places = (Place*)(ws + room.places), *tiles = (Place*)ws;
   Place* sorted = count > kTile ? tiles : places;
   const dim3 grid((uint32_t)clearers + sorters);
-  if (rows < 1u << (32 - kTileBits))
+  if (grid.x == 0) {
+    // few tokens added to a table: nothing to clear or to sort
+  } else if (rows < 1u << (32 - kTileBits)) {
     nz_embedding_sort_kernel<uint32_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
                                                              (uint32_t)rows, padding_idx, sorted, sorters,
                                                              (uint8_t*)dev_out, bytes);
-  else
+  } else {
     nz_embedding_sort_kernel<uint64_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
                                                              (uint32_t)rows, padding_idx, sorted, sorters,
                                                              (uint8_t*)dev_out, bytes);
+  }
   if (count > kTile)
     nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 256), 256, 0, st>>>(tiles, (uint32_t)count, places);
-  if (count) {
+  const auto add_up = [&](auto type) {
+    using T = decltype(type);
+    const T* g = (const T*)dev_g;
+    T* out = (T*)dev_out;
+    if (few) {
+      nz_embedding_few_kernel<T><<<(uint32_t)(count * slices), 256, 0, st>>>(
+          (const long long*)dev_indices, (uint32_t)count, (uint32_t)rows, padding_idx, g, stride, (uint32_t)cols,
+          (uint32_t)slices, scale, flags, out);
+      return;
+    }
     float* pieces = (float*)(ws + room.pieces);
     const uint32_t window = window_of(count);
     const uint32_t waves = (uint32_t)nz_ceil_div(nz_ceil_div(count, window) * slices, 4);
-#define NZ_GRADIENT(T)                                                                                               \
-  nz_embedding_sum_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (const T*)dev_g, \
-                                                    stride, (uint32_t)cols, (uint32_t)slices, scale, flags,          \
-                                                    (T*)dev_out, pieces);                                            \
-  if (count > window)                                                                                                \
-  nz_embedding_join_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (uint32_t)cols, \
-                                                     (uint32_t)slices, scale, flags, (T*)dev_out, pieces)
-    if (dtype == NZ_DTYPE_BF16) {
-      NZ_GRADIENT(nz_bf16);
-    } else if (dtype == NZ_DTYPE_F16) {
-      NZ_GRADIENT(nz_f16);
-    } else {
-      NZ_GRADIENT(float);
-    }
-#undef NZ_GRADIENT
+    nz_embedding_sum_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, g, stride,
+                                                      (uint32_t)cols, (uint32_t)slices, scale, flags, out, pieces);
+    nz_embedding_join_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (uint32_t)cols,
+                                                       (uint32_t)slices, scale, flags, out, pieces);
+  };
+  if (count == 0) {
+  } else if (dtype == NZ_DTYPE_BF16) {
+    add_up(nz_bf16());
+  } else if (dtype == NZ_DTYPE_F16) {
+    add_up(nz_f16());
+  } else {
+    add_up(float());
   }
   return nz_launched();
 }

@@ -45,7 +45,8 @@ def summed(ids, g, rows, skip=None):
 CASES = [("uniform", 1, 1, 1), ("uniform", 5, 7, 3), ("text", 100, 40, 33), ("uniform", 64, 1000, 8), ("one", 257, 9, 64),
          ("text", 2000, 5003, 129), ("two", 1030, 300, 520), ("descending", 700, 350, 1021), ("text", 4099, 50257, 40),
          ("one", 3000, 2, 513), ("uniform", 9000, 1500, 24), ("text", 20000, 3001, 16), ("one", 70000, 3, 8),
-         ("text", 70001, 130000, 8), ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
+         ("text", 1023, 400, 24), ("text", 1024, 50257, 520), ("one", 1024, 2, 100), ("two", 1025, 30, 17),
+         ("uniform", 17, 1, 40), ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -80,7 +81,8 @@ def test_random_values_and_the_same_bits_every_time(kind, count, rows, cols, dty
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
-@pytest.mark.parametrize("kind,count,rows,cols", [("text", 800, 300, 65), ("two", 300, 9, 512), ("uniform", 20000, 77, 8)])
+@pytest.mark.parametrize("kind,count,rows,cols", [("text", 800, 300, 65), ("two", 300, 9, 512), ("uniform", 20000, 77, 8),
+                                                    ("two", 3000, 9, 512), ("text", 8192, 300, 65)])
 def test_padding_frequency_and_indices_outside(kind, count, rows, cols, dtype):
     ids = tokens(kind, count, rows, seed=4)
     ids[::7] = torch.tensor([-1, rows, 2 ** 40, -2 ** 63, rows + 5])[torch.arange(len(ids[::7])) % 5]
@@ -96,14 +98,15 @@ def test_padding_frequency_and_indices_outside(kind, count, rows, cols, dtype):
     assert ((got.cpu().double() - want).abs() <= (HALF_STEP[dtype] + 2.0 ** -22) * want.abs()).all()
 
 
+@pytest.mark.parametrize("count", (900, 3000))
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
-def test_adding_to_a_gradient(dtype):
+def test_adding_to_a_gradient(dtype, count):
     rows, cols = 500, 72
     old = torch.randint(-50, 51, (rows, cols), generator=torch.Generator().manual_seed(6)).to(dtype)
     old[3] = math.nan  # a row without a token is left as it is
-    ids = tokens("text", 900, rows, seed=7)
+    ids = tokens("text", count, rows, seed=7)
     ids[ids == 3] = 4
-    g = torch.randint(-60, 61, (900, cols), generator=torch.Generator().manual_seed(8)).to(dtype)
+    g = torch.randint(-60, 61, (count, cols), generator=torch.Generator().manual_seed(8)).to(dtype)
     total, _, n = summed(ids, g, rows)
     out = old.to(DEV)
     at = out.data_ptr()
@@ -138,6 +141,10 @@ def test_special_values_stay_in_their_rows():
     got = ops.embedding_gradient(ids.to(DEV), g.to(DEV), 5).cpu()
     assert got[1, 5] == math.inf and torch.isnan(got[1, 6]) and got[3, 7] == -math.inf
     assert torch.isnan(got).sum() == 1 and torch.isinf(got).sum() == 2
+    ids, g = torch.cat([ids, torch.arange(3000) % 50 + 4]), torch.cat([g, torch.ones(3000, 40)])  # sorted
+    more = ops.embedding_gradient(ids.to(DEV), g.to(DEV), 60).cpu()
+    assert torch.equal(torch.nan_to_num(more[:4], nan=7.5), torch.nan_to_num(got[:4], nan=7.5))
+    assert (more[4:54] == 60).all() and not more[54:].any()
 
 
 def test_offsets_beyond_32_bits():
@@ -151,6 +158,9 @@ def test_offsets_beyond_32_bits():
     wide[1, :8] = 5
     got = ops.embedding_gradient(ids[:2], wide[:, :8], rows)
     assert (got[0] == 5).all() and not got[1:].any()
+    ids = torch.cat([ids[:2], torch.full((2000,), rows, device=DEV)])
+    got = ops.embedding_gradient(ids, wide[1, :8].expand(2002, 8), rows)
+    assert (got[0] == 5).all() and (got[-1] == 5).all() and not got[1:-1].any()
 
 
 def test_captured_beside_eager():
