@@ -486,6 +486,12 @@ int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint
                       const void* dev_w_scales, uint64_t k, void* dev_dx, void* dev_workspace,
                       uint64_t workspace_bytes, void* stream);
 
+/* out[n] = sum over m of x[m][n], in 32 bits in an order that m and n alone decide, rounded once: the gradient of a
+   product's bias.  m and n are up to 2^30; the workspace is as above. */
+uint64_t nz_column_sums_workspace_bytes(uint64_t m, uint64_t n);
+int nz_column_sums(const void* dev_x, int dtype, uint64_t m, uint64_t n, uint64_t stride, void* dev_out,
+                   void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
 /* The gradient of an embedding table of rows x cols that was looked up at dev_indices[0..count) (int64):
    out[v] = scale * sum of g[t] over the t with index v, in 32 bits in an order that the indices alone decide,
    rounded once: the same bits every time.  g has `stride` elements from row to row, out is contiguous.  The row

@@ -36,6 +36,7 @@ EXPORTS = [
     "nz_mx_row_bytes", "nz_mx_scale_bytes", "nz_mx_quantize", "nz_mx_dequantize", "nz_mx_lookup",
     "nz_mx_linear_workspace_bytes", "nz_mx_linear", "nz_mx_linear_rows8",
     "nz_mx_linear_grad_workspace_bytes", "nz_mx_linear_grad",
+    "nz_column_sums_workspace_bytes", "nz_column_sums",
     "nz_embedding_gradient_workspace_bytes", "nz_embedding_gradient",
 ]
 
@@ -156,6 +157,10 @@ def load() -> ctypes.CDLL:
     L.nz_mx_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp, vp, u64, vp]
     L.nz_mx_linear_grad_workspace_bytes.restype = u64
     L.nz_mx_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
+    L.nz_column_sums_workspace_bytes.restype = u64
+    L.nz_column_sums_workspace_bytes.argtypes = [u64, u64]
+    L.nz_column_sums.restype = i32
+    L.nz_column_sums.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, vp]
     L.nz_embedding_gradient_workspace_bytes.restype = u64
     L.nz_embedding_gradient_workspace_bytes.argtypes = [u64, u64]
     L.nz_embedding_gradient.restype = i32

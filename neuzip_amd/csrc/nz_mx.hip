@@ -3,6 +3,7 @@
 // The format is stated in include/neuzip_hip.h.  A row's codes lie in order and are filled up to 128 values, so
 // that a step of the matrix instruction (128 values of a row) never ends inside one; its block scales lie in
 // groups of 16 (512 values) with the four bytes that a lane needs in four successive steps next to each other.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -828,6 +829,40 @@ uint64_t filled(uint64_t cols) { return nz_ceil_div(cols, kStep) * kStep; }
 // rows are counted in 64 bits, the values of one row in 31
 bool cols_ok(uint64_t cols) { return cols <= 0x40000000ull; }
 
+// Sums over rows, the gradient of a bias: 512 columns a workgroup, every fourth of its rows a wavefront, eight of them
+// on their way at a time; the wavefronts' sums are added in their order.  Many rows are cut into parts, whose sums are
+// summed by the same kernel: no atomics, so the order of additions is that of the sizes, and nothing has to be cleared.
+// 8192 x 4096 bf16 values take 17 us, 3.9 TB/s.
+template <class T, class R>
+__global__ __launch_bounds__(256) void nz_mx_column_sums_kernel(const T* x, uint64_t stride, uint32_t m, uint32_t n,
+                                                                uint32_t rows, R* out) {
+  constexpr uint32_t kRows = 8;
+  __shared__ float sums[3][64][9];  // a ninth: lanes apart in their banks
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const uint32_t c = blockIdx.x * 512 + lane * 8, mine = c < n ? min(8u, n - c) : 0;
+  const uint32_t first = blockIdx.y * rows, last = min(m, first + rows);
+  float sum[8] = {};
+  for (uint32_t row = first + wave; row < last; row += 4 * kRows) {
+    float v[kRows][8];
+#pragma unroll
+    for (uint32_t j = 0; j < kRows; ++j) load8_upto(x + min(row + 4 * j, last - 1) * stride + c, mine, v[j]);
+#pragma unroll
+    for (uint32_t j = 0; j < kRows; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = row + 4 * j < last ? sum[e] + v[j][e] : sum[e];
+  }
+  if (wave)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[wave - 1][lane][e] = sum[e];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += sums[w][lane][e];
+  store8_upto(out + (uint64_t)blockIdx.y * n + c, mine, sum);
+}
+
 bool aligned(const void* p, uint64_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 int check_dtype(int dtype, const void* a, const void* b, const void* c) {
@@ -1036,6 +1071,14 @@ void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, cons
 #undef NZ_TILES
 }
 
+// Parts that the rows of a column sum are cut into: workgroups for the whole device, each with 32 rows at least; one
+// where few rows do not pay for a second launch (64 x 4096: 5.7 and 9.9 us).
+uint32_t sum_parts(uint64_t m, uint64_t n) {
+  if (m <= 128) return 1;
+  const uint64_t slices = nz_ceil_div(n, 512);
+  return (uint32_t)std::max<uint64_t>(1, std::min(nz_ceil_div(m, 32), nz_ceil_div(1024, slices)));
+}
+
 // Where a product's workspace holds what: rows in 8 bits, their values for a float32 result, parts.
 struct Room {
   uint64_t xd, xs, values, parts, bytes;
@@ -1239,6 +1282,36 @@ int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint
   }
   return launch_tiles16<true>(cut_product16(m, k, steps * p.count), a, a_stride, m, dev_w_data, dev_w_scales, n, k,
                               steps, p.count, k, nullptr, dev_dx, dtype, (uint8_t*)dev_workspace + p.bytes, st);
+}
+
+uint64_t nz_column_sums_workspace_bytes(uint64_t m, uint64_t n) {
+  const uint32_t parts = sum_parts(m, n);
+  return parts > 1 ? nz_mul(parts, nz_mul(n, 4)) : 0;
+}
+
+int nz_column_sums(const void* dev_x, int dtype, uint64_t m, uint64_t n, uint64_t stride, void* dev_out,
+                   void* dev_workspace, uint64_t workspace_bytes, void* stream) {
+  if (int rc = check_dtype(dtype, dev_x, dev_out, nullptr)) return rc;
+  if (n == 0) return NZ_OK;
+  if (!dev_out || (m && !dev_x)) return nz_fail(NZ_ERR_ARG, "null input or output");
+  if (m > 1u << 30 || n > 1u << 30) return nz_fail(NZ_ERR_ARG, "too many rows or columns");
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, nz_column_sums_workspace_bytes(m, n))) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  const uint32_t parts = sum_parts(m, n), slices = (uint32_t)nz_ceil_div(n, 512);
+  by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const T* x = (const T*)dev_x;
+    T* out = (T*)dev_out;
+    float* part = (float*)dev_workspace;
+    if (parts == 1) {
+      nz_mx_column_sums_kernel<T, T><<<slices, 256, 0, st>>>(x, stride, (uint32_t)m, (uint32_t)n, (uint32_t)m, out);
+    } else {
+      nz_mx_column_sums_kernel<T, float><<<dim3(slices, parts), 256, 0, st>>>(
+          x, stride, (uint32_t)m, (uint32_t)n, (uint32_t)nz_ceil_div(m, parts), part);
+      nz_mx_column_sums_kernel<float, T><<<slices, 256, 0, st>>>(part, n, parts, (uint32_t)n, parts, out);
+    }
+  });
+  return nz_launched();
 }
 
 }  // extern "C"

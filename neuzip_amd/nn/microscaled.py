@@ -28,6 +28,13 @@ class _Microscaled(torch.nn.Module):
         return self.weight_data.numel() + self.weight_scales.numel()
 
 
+def _autocast(x):
+    """``x`` in the type that an autocast region asks for"""
+    if not isinstance(x, MXTensor) and torch.is_autocast_enabled("cuda"):
+        return x.to(torch.get_autocast_dtype("cuda"))
+    return x
+
+
 class MXLinear(_Microscaled):
     def __init__(self, linear: torch.nn.Linear) -> None:
         super().__init__()
@@ -40,8 +47,7 @@ class MXLinear(_Microscaled):
         self._hold(linear.weight.data)
 
     def forward(self, x):
-        if not isinstance(x, MXTensor) and torch.is_autocast_enabled("cuda"):
-            x = x.to(torch.get_autocast_dtype("cuda"))
+        x = _autocast(x)
         bias = self.bias
         if bias is not None:
             dtype = torch.bfloat16 if isinstance(x, MXTensor) else x.dtype
@@ -76,7 +82,7 @@ class MXEmbedding(_Microscaled):
         return mx_embedding(x, self.weight, self.scale, self._like.dtype, self._status)
 
     def linear(self, x):
-        return mx_linear(x, self.weight)
+        return mx_linear(_autocast(x), self.weight)
 
     def check(self) -> None:
         """Raise if a lookup since the last check had an index outside the table (waits for the device)."""

@@ -142,7 +142,8 @@ def mx_quantize(x: torch.Tensor, bits: int = 4) -> MXTensor:
     """``x`` (bfloat16, float16 or float32, on the GPU) in microscaled form:
     blocks of 32 values along the last axis share a power of two, values are
     rounded to the nearest e2m1 (``bits=4``) or e4m3 (``bits=8``) number, ties to
-    the even code.  A block that holds a NaN or an infinity reads as NaN."""
+    the even code.  A block that holds a NaN or an infinity reads as NaN.  Autograd
+    does not record it."""
     if bits not in (4, 8):
         raise ValueError("bits must be 4 or 8")
     code = _dtype_code(x.dtype)
@@ -208,6 +209,16 @@ def _input_gradient(grad: torch.Tensor, weight: MXTensor) -> torch.Tensor:
     return dx
 
 
+def _bias_gradient(grad: torch.Tensor, n: int) -> torch.Tensor:
+    L, index = _lib.load(), _on_gpu(grad=grad)
+    rows, m, stride = _as_rows(grad, n)
+    out = rows.new_empty(n)
+    room = L.nz_column_sums_workspace_bytes(m, n)
+    ws, at = _workspace(room, rows)
+    _call(L.nz_column_sums, index, rows.data_ptr(), _dtype_code(grad.dtype), m, n, stride, out.data_ptr(), at, room)
+    return out
+
+
 class MicroscaledLinear(torch.autograd.Function):
     """``y = x W^T (+ b)`` with a frozen weight in 4 bits.  Backward gives the
     gradients of ``x`` (the rounding of its rows to 8 bits is passed straight
@@ -225,7 +236,7 @@ class MicroscaledLinear(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             grad_x = _input_gradient(grad_output, ctx.weight)
         if ctx.needs_input_grad[2]:
-            grad_b = grad_output.reshape(-1, ctx.weight.shape[0]).sum(0)
+            grad_b = _bias_gradient(grad_output, ctx.weight.shape[0])
         return grad_x, None, grad_b, None
 
 

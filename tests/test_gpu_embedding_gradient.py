@@ -46,7 +46,7 @@ CASES = [("uniform", 1, 1, 1), ("uniform", 5, 7, 3), ("text", 100, 40, 33), ("un
          ("text", 2000, 5003, 129), ("two", 1030, 300, 520), ("descending", 700, 350, 1021), ("text", 4099, 50257, 40),
          ("one", 3000, 2, 513), ("uniform", 9000, 1500, 24), ("text", 20000, 3001, 16), ("one", 70000, 3, 8),
          ("text", 1023, 400, 24), ("text", 1024, 50257, 520), ("one", 1024, 2, 100), ("two", 1025, 30, 17),
-         ("uniform", 17, 1, 40), ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
+         ("uniform", 17, 1, 40), ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("text", 10000, 600000, 9), ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -158,8 +158,8 @@ def test_offsets_beyond_32_bits():
     wide[1, :8] = 5
     got = ops.embedding_gradient(ids[:2], wide[:, :8], rows)
     assert (got[0] == 5).all() and not got[1:].any()
-    ids = torch.cat([ids[:2], torch.full((2000,), rows, device=DEV)])
-    got = ops.embedding_gradient(ids, wide[1, :8].expand(2002, 8), rows)
+    ids = torch.cat([ids[:2], torch.full((9000,), rows, device=DEV)])  # sorted
+    got = ops.embedding_gradient(ids, wide[1, :8].expand(9002, 8), rows)
     assert (got[0] == 5).all() and (got[-1] == 5).all() and not got[1:-1].any()
 
 

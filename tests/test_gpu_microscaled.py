@@ -335,6 +335,33 @@ def test_offsets_beyond_32_bits():
     assert (dx[-1] == 64 * n).all() and not dx[1:-1].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n", [(1, 1), (2, 7), (31, 8), (33, 513), (64, 1024), (100, 3001), (1000, 40), (5000, 1),
+                                 (8192, 1030), (40000, 9), (3, 40001)])
+def test_bias_gradient_of_whole_numbers_is_exact(m, n, dtype):
+    """numbers up to 30 in magnitude: 40000 of them stay below 2^24"""
+    g = whole_numbers(m, n, 30, m + n, dtype)
+    w = ops.mx_quantize(torch.zeros(n, 32, device=DEV), 4)
+    bias = torch.zeros(n, dtype=dtype, device=DEV, requires_grad=True)
+    y = ops.mx_linear(torch.zeros(m, 32, dtype=dtype, device=DEV), w, bias)
+    y.backward(g.to(DEV))
+    same(bias.grad, round_to(g.double().sum(0), dtype))
+    wide = torch.full((m, n + 3), 7.0, dtype=dtype, device=DEV)  # rows that begin between vectors
+    wide[:, 1:n + 1] = g.to(DEV)
+    (gb,) = torch.autograd.grad(ops.mx_linear(torch.zeros(m, 32, dtype=dtype, device=DEV), w, bias), bias,
+                                wide[:, 1:n + 1])
+    same(gb, bias.grad)
+
+
+def test_bias_gradient_of_no_rows_and_one_value():
+    w = ops.mx_quantize(torch.zeros(70, 32, device=DEV), 4)
+    bias = torch.full((70,), 3.0, device=DEV, requires_grad=True)
+    ops.mx_linear(torch.zeros(0, 32, device=DEV), w, bias).sum().backward()
+    same(bias.grad, torch.zeros(70))
+    (gb,) = torch.autograd.grad(ops.mx_linear(torch.zeros(2, 50, 32, device=DEV), w, bias).sum(), bias)  # expanded
+    same(gb, torch.full((70,), 100.0))
+
+
 def test_gradient_strides_shapes_and_no_second_order():
     w = ops.mx_quantize(whole_numbers(24, 96, 6, 1).to(DEV), 4)
     w64 = decoded(w.data.cpu(), w.scales.cpu(), 96, 4)[:, :96]
@@ -430,6 +457,7 @@ def test_layers_hold_compute_and_travel():
     model.embed.check()
     with torch.autocast("cuda", dtype=torch.bfloat16):
         assert model.up(x.float()).dtype == torch.bfloat16
+        assert model.embed.linear(x.float()).dtype == torch.bfloat16
     x8 = ops.mx_quantize(x, 8)
     z = model.up(x8)
     same(z, y)
@@ -518,13 +546,17 @@ def test_captured_calls_replay_beside_eager_ones():
     table = ops.mx_quantize(rnd(100, 640, seed=2).to(DEV), 4)
     ids = torch.zeros(40, dtype=torch.int64, device=DEV)
 
+    bias = torch.ones(w.shape[0], dtype=torch.bfloat16, device=DEV, requires_grad=True)
+
     def work():
         x = ops.mx_embedding(ids, table, 0.5)
         x.requires_grad_(True)
         y = ops.mx_linear(x, w)
         one = ops.mx_linear(x[:1].detach(), w)
         (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
-        return x.detach(), y.detach(), one, gx
+        z = ops.mx_linear(x.detach(), w, bias)
+        (gb,) = torch.autograd.grad(z, bias, z.detach())
+        return x.detach(), y.detach(), one, gx, gb
 
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())

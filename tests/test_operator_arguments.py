@@ -63,12 +63,25 @@ def test_refusals_of_the_abi():
     need = L.nz_mx_linear_grad_workspace_bytes(p + 2, 0, 100, 512, 512, 512)
     refused(L.nz_mx_linear_grad(p + 2, 0, 100, 512, 512, p, p, 512, p, p, need - 1, None), D, "workspace")
     assert L.nz_mx_linear_grad(None, 0, 0, 1, 1, None, None, 1, None, None, 0, None) == _lib.OK
+    sums, need = L.nz_column_sums, L.nz_column_sums_workspace_bytes(5000, 100)
+    assert need and not L.nz_column_sums_workspace_bytes(1, 100)
+    refused(sums(p, 9, 5, 5, 5, p, p, 0, None), C, "Unsupported data type")
+    refused(sums(None, 0, 5, 5, 5, p, p, 0, None), A, "null")
+    refused(sums(p + 1, 0, 5, 5, 5, p, p, 0, None), B, "aligned")
+    refused(sums(p, 0, 1 << 31, 5, 5, p, p, 0, None), A, "too many")
+    refused(sums(p, 0, 5000, 100, 100, p, p, need - 1, None), D, "workspace")
+    refused(sums(p, 0, 5000, 100, 100, p, None, need, None), B, "workspace")
+    assert sums(None, 0, 5, 0, 5, None, None, 0, None) == _lib.OK
     grad = L.nz_embedding_gradient
     refused(grad(p, 1, p, 7, 1, 1, 1, 1.0, -1, 0, p, p, 1 << 30, None), C, "Unsupported data type")
     refused(grad(p, 1, p, 0, 1, 1, 1, 1.0, -1, 4, p, p, 1 << 30, None), A, "unknown flags")
     refused(grad(None, 1, p, 0, 1, 1, 1, 1.0, -1, 0, p, p, 1 << 30, None), A, "null")
     refused(grad(p + 4, 1, p, 0, 1, 1, 1, 1.0, -1, 0, p, p, 1 << 30, None), B, "aligned")
     refused(grad(p, 1 << 32, p, 0, 1, 1, 1, 1.0, -1, 0, p, p, 1 << 30, None), A, "too many")
+    need = L.nz_embedding_gradient_workspace_bytes(5000, 8)
+    assert need and not L.nz_embedding_gradient_workspace_bytes(1000, 8)
+    refused(grad(p, 5000, p, 0, 8, 9, 8, 1.0, -1, 0, p, p, need - 1, None), D, "workspace")
+    refused(grad(p, 5000, p, 0, 8, 9, 8, 1.0, -1, 0, p, p + 8, need, None), B, "workspace")
     assert grad(None, 0, None, 0, 1, 0, 5, 1.0, -1, 0, None, None, 0, None) == _lib.OK
 
 
