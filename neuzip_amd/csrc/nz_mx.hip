@@ -496,10 +496,26 @@ __global__ __launch_bounds__(256) void nz_mx_join_kernel(const float* part, uint
   }
 }
 
+typedef nz_bf16 b8v __attribute__((ext_vector_type(8)));
+typedef nz_bf16 b2v __attribute__((ext_vector_type(2)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+// 8 codes as bf16 numbers.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
+__device__ inline b8v bf16_of_codes(uint32_t codes, uint32_t s) {
+  const float scale = __uint_as_float(s << 23);
+  const b2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
+  const b2v b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+  const b2v c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
+  const b2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+  return b8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
 // Up to 16 rows, where reading the weight is all that counts: no staging and no barrier in the way of it.  The eight
 // wavefronts are kw that share the values of a row (512 at a time, in turn) times 8 / kw with 16 weight rows each;
 // a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
 // (QUANTIZE) as they are: then every workgroup brings them to 8 bits in LDS while its first weights are on their way.
+// Results in float32 are summed by bf16 instructions (why, see below), for which a lane takes both sides to bf16: of
+// the 128 values of a step those of its block, 8 at a time (both sides in the same order, which is all that counts).
 // One row against 14336x4096: 8.4 us, 3.7 TB/s of codes and scales, of which 2 are the launch.
 template <bool QUANTIZE, class T>
 __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t stride, const uint8_t* xs,
@@ -523,7 +539,8 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
   };
   if (kwave < groups) load(a, kwave);
 
-  const uint32_t row = min(r, m - 1);
+  constexpr bool kWide = std::is_same<T, float>::value;
+  const uint32_t row = min(r, m - 1), xg = g * (kWide ? 32 : 16);
   const uint8_t *xp, *xsp;
   if constexpr (QUANTIZE) {
     // rows of groups * 528 bytes: 512 values and their scales per group
@@ -538,10 +555,10 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
       if ((lane & 3) == 0) q[512 + scale_at(lane / 4)] = (uint8_t)s;
     }
     __syncthreads();
-    xp = few_lds + row * groups * 528u + g * 16;
+    xp = few_lds + row * groups * 528u + xg;
     xsp = few_lds + row * groups * 528u + 512 + g * 4;
   } else {
-    xp = (const uint8_t*)x + row * (steps * 128ull) + g * 16;
+    xp = (const uint8_t*)x + row * (steps * 128ull) + xg;
     xsp = xs + row * (groups * 16ull) + g * 4;
   }
   f4 acc = {0, 0, 0, 0};
@@ -551,8 +568,22 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
       constexpr int i = decltype(b4)::value;
       if (group * 4 + i >= steps) return;
       const uint8_t* p = xp + (QUANTIZE ? group * 528 : (uint64_t)group * 512) + i * 128;
-      const i4v x0 = *(const i4v*)p, x1 = *(const i4v*)(p + 64);
-      acc = step(h.w[i], x0, x1, acc, h.s, sx, i);
+      if constexpr (kWide) {
+        const float f = down_factor(sx >> (8 * i) & 255);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+          values8(*(const uint2*)(p + 8 * q), f, v);
+          b8v xv;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) xv[e] = (nz_bf16)v[e];
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(h.w[i][q], h.s >> (8 * i) & 255), xv, acc, 0, 0,
+                                                        0);
+        }
+      } else {
+        const i4v x0 = *(const i4v*)p, x1 = *(const i4v*)(p + 64);
+        acc = step(h.w[i], x0, x1, acc, h.s, sx, i);
+      }
     };
     one(std::integral_constant<int, 0>());
     one(std::integral_constant<int, 1>());
@@ -590,20 +621,6 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
 // largest of its 128 products: 1.5e-5 of a sum, measured, against 6e-8 of this one).  A weight's values are exact in
 // bf16, and so is an activation of 8 bits; a gradient of 16 or 32 bits is the sum of two or three bf16 numbers, laid
 // side by side along the summed axis.
-
-typedef nz_bf16 b8v __attribute__((ext_vector_type(8)));
-typedef nz_bf16 b2v __attribute__((ext_vector_type(2)));
-typedef short s4v __attribute__((ext_vector_type(4)));
-
-// 8 codes as bf16 numbers.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
-__device__ inline b8v bf16_of_codes(uint32_t codes, uint32_t s) {
-  const float scale = __uint_as_float(s << 23);
-  const b2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
-  const b2v b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
-  const b2v c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
-  const b2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
-  return b8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
 
 // Rows cut into P bf16 planes, [m][P][padded]: each plane takes the 8 leading bits that the planes before it left, so
 // three hold all 24 bits of a float32 and two the 11 of a float16.  What is not finite stays in the first.
@@ -944,24 +961,26 @@ struct Cut {
   uint64_t part_bytes(uint64_t m, uint64_t cols) const { return parts > 1 ? align256(parts * m * cols * 4) : 0; }
 };
 
-// What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them do; 256
-// compute units, 64 steps and more, everything else idle.
+// What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them or fewer do, on
+// 256 compute units.  These and the figures of cut_product are fitted to times of 150 products of 17 to 8192 rows with
+// weights of 256 to 16384 rows and columns, each in all tiles and up to 16 parts: the cut chosen by them takes 1.2 %
+// more than the fastest one in the mean (of 16-bit rows 1.4 %), at most 17 %.
 struct Tile {
   uint32_t bm, bn, slots;
   float full, half;
 };
-// Products of 8-bit rows, 128 values a step: 2.6, 2.1, 1.5 and 1.1 PFLOP/s where the device is full.
-constexpr Tile kTiles[] = {{128, 256, 512, 1.72f, 1.38f},
-                           {128, 128, 512, 1.04f, 0.85f},
-                           {64, 128, 256, 0.38f, 0.40f},
-                           {64, 64, 256, 0.25f, 0.31f}};
-// Products of 16-bit rows, 64 values a step: 1.06 and 0.47 PFLOP/s.
-constexpr Tile kTiles16[] = {{256, 128, 256, 1.00f, 0.85f}, {64, 64, 256, 0.29f, 0.38f}};
+// Products of 8-bit rows, 128 values a step: 2.5, 2.1, 1.5 and 1.1 PFLOP/s where the device is full.
+constexpr Tile kTiles[] = {{128, 256, 512, 1.70f, 1.40f},
+                           {128, 128, 512, 1.00f, 1.00f},
+                           {64, 128, 256, 0.36f, 0.38f},
+                           {64, 64, 256, 0.25f, 0.28f}};
+// Products of 16-bit rows, 64 values a step: 1.1 and 0.43 PFLOP/s.
+constexpr Tile kTiles16[] = {{256, 128, 256, 0.95f, 0.86f}, {64, 64, 256, 0.31f, 0.31f}};
 
-// The cut that takes the least time by these figures.  Rounds of workgroups follow each other, a launch and a round's
-// begin and end take some 4 us; parts cost a launch of 3 us and are written, read and joined at 4 bytes each.  With
-// the tiles alone to choose from, 5366 x (576x12736) took 98 us in 420 tiles of 64x128, where two parts of 210 tiles
-// of 128x128 take 75; 64 x (4096x14336) takes 33 us in 64 tiles and 15 in four parts of them.
+// The cut that takes the least time by these figures.  Rounds of workgroups follow each other and begin and end in 1 us
+// that others do not cover; parts cost a launch of 4 us and are written, read and joined at 5 TB/s.
+// 5366 x (576x12736) takes 98 us in 420 tiles of 64x128, 75 in two parts of 210 tiles of 128x128; 64 x (4096x14336)
+// 33 us in 64 tiles and 15 in four parts of them; 17 x (128256x4096) 74 us in tiles of 128x256, 52 in 64x128.
 template <int N>
 Cut cut_product(const Tile (&kinds)[N], uint64_t m, uint64_t cols, uint64_t units_of, uint64_t steps_per_unit,
                 uint64_t least) {
@@ -972,14 +991,16 @@ Cut cut_product(const Tile (&kinds)[N], uint64_t m, uint64_t cols, uint64_t unit
   for (const Tile& t : kinds) {
     const uint64_t mt = nz_ceil_div(m, t.bm), nt = nz_ceil_div(cols, t.bn);
     const float slots = t.slots * scale;
-    for (uint64_t want = 1; want <= 16; ++want) {
-      const uint64_t length = nz_ceil_div(units_of, want), parts = nz_ceil_div(units_of, length);
+    const uint32_t units = (uint32_t)std::min<uint64_t>(units_of, 1u << 30);
+    for (uint32_t want = 1; want <= std::min<uint64_t>(units_of, 16); ++want) {
+      if (want > 1 && (float)(mt * nt * want) > 4 * slots) break;  // enough without parts
+      const uint32_t length = (units + want - 1) / want, parts = (units + length - 1) / length;
       if (parts != want || (parts > 1 && length < least)) continue;
       const float groups = (float)(mt * nt * parts), rounds = floorf(groups / slots), rest = groups - rounds * slots;
       float time = (rounds * t.full + (rest == 0 ? 0.0f : rest <= slots / 2 ? t.half : t.full)) *
                        (float)(length * steps_per_unit) +
-                   4.0f * (rounds + (rest > 0));
-      if (parts > 1) time += 3.0f + (float)parts * (float)m * (float)cols * (12.0f / 5e6f);
+                   rounds + (rest > 0);
+      if (parts > 1) time += 4.0f + (float)parts * (float)m * (float)cols * 2.8e-6f;
       if (best.parts == 0 || time < best_time) {
         best = Cut{t.bm, t.bn, (uint32_t)parts, (uint32_t)length, (uint32_t)mt, (uint32_t)nt};
         best_time = time;
@@ -995,7 +1016,9 @@ Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
 }
 
 // The products of 16-bit rows, in steps of 64.
-Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) { return cut_product(kTiles16, m, cols, steps, 1, 8); }
+Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) {
+  return cut_product(kTiles16, m, cols, steps, 1, 8);
+}
 
 void launch_join(const float* part, const Cut& c, uint64_t m, uint64_t n, const void* bias, void* y, int dtype,
                  hipStream_t st) {
@@ -1032,10 +1055,21 @@ int launch_tiles16(const Cut& c, const void* a, uint64_t a_stride, uint64_t m, c
   return nz_launched();
 }
 
-// Rows that are brought to 8 bits inside the kernel: as many as one workgroup does at little cost.  8 rows against
-// 14336x4096: 12.4 us, in two launches 3.4 + 10.2; against 4096x4096 7.7 and 3.4 + 6.6; 16 rows of 2048 values against
-// 14336 rows 9.9 and 3.3 + 6.4.
-bool few_rows(uint64_t m, uint64_t k) { return m <= 16 && m * nz_ceil_div(k, kGroup) <= 64; }
+// Rows that go to the kernel for few (one tile of the instruction), and those that are brought to 8 bits inside it:
+// every workgroup does that again, which costs more the longer and the more the rows are and the more workgroups there
+// are (`groups` of 512 values in all rows).  Times on the device of quantising inside, before it, and before tiles
+// (with the join of their parts, if any); a launch less is 4 us less for the caller, who often is what takes longest:
+//    2 rows of 12421x14421, 58 groups   22.3 27.7 25.5      8 rows of 50257x4096, 64 groups   30.6 44   23.4
+//    8 of 9505x3706, 64                 11.1 12.7  9.8      4 of 128256x1024, 8               15.0 24   22.7
+//    6 of 1735x7471, 90                  9.9  9.1 12.7     16 of 9498x3995, 128                  - 17.7 10.2
+// Results in float32, whose tiles are slower, are better off there always: 16 rows of 12886x8431 31 against 50 us.
+bool few_inside(uint64_t m, uint64_t n, uint64_t k, int dtype) {
+  const uint64_t groups = m * nz_ceil_div(k, kGroup);
+  return m <= 16 && groups <= 64 && (groups <= 32 || n * k <= 1ull << 26 || dtype == NZ_DTYPE_F32);
+}
+bool few_rows(uint64_t m, uint64_t n, uint64_t k, int dtype) {
+  return few_inside(m, n, k, dtype) || (m <= 16 && (n * k <= 1ull << 25 || dtype == NZ_DTYPE_F32));
+}
 
 template <bool QUANTIZE, class T>
 void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n,
@@ -1082,34 +1116,46 @@ uint32_t sum_parts(uint64_t m, uint64_t n) {
 // Where a product's workspace holds what: rows in 8 bits, their values for a float32 result, parts.
 struct Room {
   uint64_t xd, xs, values, parts, bytes;
+  Cut cut;  // of rows that go to tiles
 };
 Room product_room(uint64_t m, uint64_t n, uint64_t k, int dtype) {
-  Room r;
+  Room r = {};
+  if (few_inside(m, n, k, dtype)) return r;
   r.xd = 0;
   r.xs = align256(nz_mul(m, nz_mx_row_bytes(k, 8)));
   r.values = align256(r.xs + nz_mul(m, nz_mx_scale_bytes(k)));
+  r.bytes = r.values;
+  if (few_rows(m, n, k, dtype)) return r;
   const uint64_t pad = filled(k);
   if (dtype == NZ_DTYPE_F32) {
+    r.cut = cut_product16(m, n, pad / 64);
     r.parts = align256(r.values + nz_mul(m, pad * 2));
-    r.bytes = r.parts + cut_product16(m, n, pad / 64).part_bytes(m, n);
   } else {
+    r.cut = cut_product8(m, n, k);
     r.parts = r.values;
-    r.bytes = r.parts + cut_product8(m, n, k).part_bytes(m, n);
   }
+  r.bytes = r.parts + r.cut.part_bytes(m, n);
   return r;
 }
 
 int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n, uint32_t k,
                    const void* bias, void* y, int dtype, const Room& room, uint8_t* workspace, hipStream_t st) {
+  if (few_rows(m, n, k, dtype)) {
+    by_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      launch_few<false>(xd, 0, xs, m, wd, ws, n, k, (const T*)bias, (T*)y, st);
+    });
+    return nz_launched();
+  }
   if (dtype == NZ_DTYPE_F32) {
     const uint64_t pad = filled(k);
     if (int rc = launch_values(xd, xs, m, pad, 8, nullptr, m, 1.0f, workspace + room.values, NZ_DTYPE_BF16, nullptr,
                                st))
       return rc;
-    return launch_tiles16<false>(cut_product16(m, n, pad / 64), workspace + room.values, pad, m, wd, ws, n, k, pad / 64,
+    return launch_tiles16<false>(room.cut, workspace + room.values, pad, m, wd, ws, n, k, pad / 64,
                                  1, n, bias, y, dtype, workspace + room.parts, st);
   }
-  const Cut c = cut_product8(m, n, k);
+  const Cut& c = room.cut;
   float* part = c.parts > 1 ? (float*)(workspace + room.parts) : nullptr;
   if (dtype == NZ_DTYPE_BF16)
     launch_tiles(c, xd, xs, m, wd, ws, n, k, (const nz_bf16*)bias, (nz_bf16*)y, part, st);
@@ -1190,7 +1236,6 @@ int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, ui
 
 uint64_t nz_mx_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   if (m == 0 || n == 0 || k == 0) return 0;
-  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) return 0;
   return product_room(m, n, k, dtype).bytes;
 }
 
@@ -1201,18 +1246,17 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
   if (m == 0 || n == 0) return NZ_OK;
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
   if (!dev_x || !dev_y) return nz_fail(NZ_ERR_ARG, "null rows or output");
-  if (int rc = check_workspace(dev_workspace, workspace_bytes, nz_mx_linear_workspace_bytes(m, n, k, dtype))) return rc;
+  const Room room = product_room(m, n, k, dtype);
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, room.bytes)) return rc;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) {
-    if (dtype == NZ_DTYPE_BF16)
-      launch_few<true>(dev_x, stride, nullptr, m, dev_w_data, dev_w_scales, n, (uint32_t)k, (const nz_bf16*)dev_bias,
-                       (nz_bf16*)dev_y, st);
-    else
-      launch_few<true>(dev_x, stride, nullptr, m, dev_w_data, dev_w_scales, n, (uint32_t)k, (const nz_f16*)dev_bias,
-                       (nz_f16*)dev_y, st);
+  if (few_inside(m, n, k, dtype)) {
+    by_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      launch_few<true>(dev_x, stride, nullptr, m, dev_w_data, dev_w_scales, n, (uint32_t)k, (const T*)dev_bias,
+                       (T*)dev_y, st);
+    });
     return nz_launched();
   }
-  const Room room = product_room(m, n, k, dtype);
   uint8_t* base = (uint8_t*)dev_workspace;
   if (int rc = launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st)) return rc;
   return launch_product(base + room.xd, base + room.xs, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y,
@@ -1227,19 +1271,11 @@ int nz_mx_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
   if (int rc = check_mx(dev_x_data, dev_x_scales)) return rc;
   if (!dev_y) return nz_fail(NZ_ERR_ARG, "null output");
-  if (int rc = check_workspace(dev_workspace, workspace_bytes, nz_mx_linear_workspace_bytes(m, n, k, dtype))) return rc;
+  const Room room = product_room(m, n, k, dtype);
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, room.bytes)) return rc;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype != NZ_DTYPE_F32 && few_rows(m, k)) {
-    if (dtype == NZ_DTYPE_BF16)
-      launch_few<false>(dev_x_data, 0, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k,
-                        (const nz_bf16*)dev_bias, (nz_bf16*)dev_y, st);
-    else
-      launch_few<false>(dev_x_data, 0, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k,
-                        (const nz_f16*)dev_bias, (nz_f16*)dev_y, st);
-    return nz_launched();
-  }
   return launch_product(dev_x_data, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, dtype,
-                        product_room(m, n, k, dtype), (uint8_t*)dev_workspace, st);
+                        room, (uint8_t*)dev_workspace, st);
 }
 
 uint64_t nz_mx_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
@@ -1257,12 +1293,11 @@ int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint
   if (!dev_dx || !dev_g) return nz_fail(NZ_ERR_ARG, "null gradient or output");
   if (n == 0) return nz_fail(NZ_ERR_ARG, "a weight without rows has no gradient to pass on");
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
-  if (int rc = check_workspace(dev_workspace, workspace_bytes,
-                               nz_mx_linear_grad_workspace_bytes(dev_g, dtype, m, n, stride, k)))
-    return rc;
   const hipStream_t st = (hipStream_t)stream;
   const Planes p = planes_of(dev_g, dtype, m, n, stride);
   const uint64_t steps = p.padded / 64;
+  const Cut cut = cut_product16(m, k, steps * p.count);
+  if (int rc = check_workspace(dev_workspace, workspace_bytes, p.bytes + cut.part_bytes(m, k))) return rc;
   const void* a = dev_g;
   uint64_t a_stride = stride;
   if (p.bytes) {
@@ -1280,7 +1315,7 @@ int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint
       NZ_PLANES(3, float);
 #undef NZ_PLANES
   }
-  return launch_tiles16<true>(cut_product16(m, k, steps * p.count), a, a_stride, m, dev_w_data, dev_w_scales, n, k,
+  return launch_tiles16<true>(cut, a, a_stride, m, dev_w_data, dev_w_scales, n, k,
                               steps, p.count, k, nullptr, dev_dx, dtype, (uint8_t*)dev_workspace + p.bytes, st);
 }
 

@@ -19,7 +19,7 @@ inline int nz_launched() {
   return e == hipSuccess ? NZ_OK : nz_fail(NZ_ERR_HIP, hipGetErrorString(e));
 }
 
-inline uint64_t nz_ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+inline uint64_t nz_ceil_div(uint64_t a, uint64_t b) { return a / b + (a % b != 0); }
 
 inline uint32_t nz_dtype_bytes(int dtype) {
   return dtype == NZ_DTYPE_F32 ? 4u : dtype == NZ_DTYPE_BF16 || dtype == NZ_DTYPE_F16 ? 2u : 0u;

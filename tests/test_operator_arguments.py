@@ -63,6 +63,11 @@ def test_refusals_of_the_abi():
     need = L.nz_mx_linear_grad_workspace_bytes(p + 2, 0, 100, 512, 512, 512)
     refused(L.nz_mx_linear_grad(p + 2, 0, 100, 512, 512, p, p, 512, p, p, need - 1, None), D, "workspace")
     assert L.nz_mx_linear_grad(None, 0, 0, 1, 1, None, None, 1, None, None, 0, None) == _lib.OK
+    for huge in (1 << 24, 1 << 40, (1 << 63) + 5, (1 << 64) - 1):  # sizes beyond the limits: an answer, no harm
+        for m, n, k in ((huge, 5, 5), (5, huge, 5), (5, 5, huge), (huge, huge, huge)):
+            L.nz_mx_linear_workspace_bytes(m, n, k, 0), L.nz_mx_linear_workspace_bytes(m, n, k, 2)
+            L.nz_mx_linear_grad_workspace_bytes(p, 0, m, n, n, k)
+            L.nz_column_sums_workspace_bytes(m, n), L.nz_embedding_gradient_workspace_bytes(m, n)
     sums, need = L.nz_column_sums, L.nz_column_sums_workspace_bytes(5000, 100)
     assert need and not L.nz_column_sums_workspace_bytes(1, 100)
     refused(sums(p, 9, 5, 5, 5, p, p, 0, None), C, "Unsupported data type")
