@@ -457,8 +457,8 @@ int nz_mx_quantize(const void* dev_x, int dtype, uint64_t rows, uint64_t cols, u
 int nz_mx_dequantize(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int bits,
                      void* dev_out, int dtype, void* stream);
 
-/* Rows dev_indices[0..count) (int64) of a table, times `scale`, rounded once.  An index outside the table
-   gives a row of zeros and, when dev_status is not NULL, sets bit 0 of that uint32. */
+/* Rows dev_indices[0..count) (int64) of a table, times `scale` in 32 bits, rounded to dtype.  An index outside the
+   table gives a row of zeros and, when dev_status is not NULL, sets bit 0 of that uint32. */
 int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int bits,
                  const void* dev_indices, uint64_t count, float scale, void* dev_out, int dtype, void* dev_status,
                  void* stream);

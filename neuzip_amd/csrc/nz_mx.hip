@@ -648,6 +648,23 @@ __global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t 
   }
 }
 
+// What the 8 bits of float32 rows stand for, as bf16 numbers, rows filled up to whole steps: the rows' side of a
+// product with a float32 result.
+__global__ __launch_bounds__(256) void nz_mx_rounded_kernel(const float* x, uint64_t stride, uint32_t cols,
+                                                            uint64_t waves, uint32_t groups, nz_bf16* out) {
+  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (wave >= waves) return;
+  const uint64_t row = wave / groups;
+  const uint32_t at = (uint32_t)(wave - row * groups) * kGroup + (threadIdx.x & 63) * 8;
+  float v[8];
+  load8_upto(x + row * stride + at, at < cols ? cols - at : 0, v);
+  const uint32_t s = block_scale<8>(v);
+  const uint2 codes = codes8(v, up_factor(s));
+  values8(codes, down_factor(s), v);
+  const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
+  if (at < filled) store8(out + row * filled + at, v);
+}
+
 // A tile of C[m][cols] = sum over c of A[m][c] B(c, col), c running `planes` times through the summed axis.
 // ROWS: B(c, col) = w[c][col], the gradient; else w[col][c], the product itself.
 //
@@ -961,10 +978,10 @@ struct Cut {
   uint64_t part_bytes(uint64_t m, uint64_t cols) const { return parts > 1 ? align256(parts * m * cols * 4) : 0; }
 };
 
-// What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them or fewer do, on
-// 256 compute units.  These and the figures of cut_product are fitted to times of 150 products of 17 to 8192 rows with
-// weights of 256 to 16384 rows and columns, each in all tiles and up to 16 parts: the cut chosen by them takes 1.2 %
-// more than the fastest one in the mean (of 16-bit rows 1.4 %), at most 17 %.
+// What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them or fewer do,
+// on 256 compute units.  These and the figures of cut_product are fitted to times of 150 products of 17 to 8192 rows
+// with weights of 256 to 16384 rows and columns, each in all tiles and up to 16 parts: the cut chosen by them takes
+// 1.2 % more than the fastest one in the mean (of 16-bit rows 1.4 %), at most 17 %.
 struct Tile {
   uint32_t bm, bn, slots;
   float full, half;
@@ -1129,13 +1146,21 @@ Room product_room(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   const uint64_t pad = filled(k);
   if (dtype == NZ_DTYPE_F32) {
     r.cut = cut_product16(m, n, pad / 64);
-    r.parts = align256(r.values + nz_mul(m, pad * 2));
+    r.values = 0;  // the rows' 8 bits are not kept
+    r.parts = align256(nz_mul(m, pad * 2));
   } else {
     r.cut = cut_product8(m, n, k);
     r.parts = r.values;
   }
   r.bytes = r.parts + r.cut.part_bytes(m, n);
   return r;
+}
+
+// A float32 result of rows whose values lie in the workspace.
+int launch_wide(uint64_t m, const void* wd, const void* ws, uint64_t n, uint32_t k, const void* bias, void* y,
+                const Room& room, uint8_t* workspace, hipStream_t st) {
+  return launch_tiles16<false>(room.cut, workspace + room.values, filled(k), m, wd, ws, n, k, filled(k) / 64, 1, n,
+                               bias, y, NZ_DTYPE_F32, workspace + room.parts, st);
 }
 
 int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, const void* ws, uint64_t n, uint32_t k,
@@ -1148,12 +1173,10 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, c
     return nz_launched();
   }
   if (dtype == NZ_DTYPE_F32) {
-    const uint64_t pad = filled(k);
-    if (int rc = launch_values(xd, xs, m, pad, 8, nullptr, m, 1.0f, workspace + room.values, NZ_DTYPE_BF16, nullptr,
-                               st))
+    if (int rc = launch_values(xd, xs, m, filled(k), 8, nullptr, m, 1.0f, workspace + room.values, NZ_DTYPE_BF16,
+                               nullptr, st))
       return rc;
-    return launch_tiles16<false>(room.cut, workspace + room.values, pad, m, wd, ws, n, k, pad / 64,
-                                 1, n, bias, y, dtype, workspace + room.parts, st);
+    return launch_wide(m, wd, ws, n, k, bias, y, room, workspace, st);
   }
   const Cut& c = room.cut;
   float* part = c.parts > 1 ? (float*)(workspace + room.parts) : nullptr;
@@ -1258,6 +1281,13 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
     return nz_launched();
   }
   uint8_t* base = (uint8_t*)dev_workspace;
+  if (dtype == NZ_DTYPE_F32 && !few_rows(m, n, k, dtype)) {
+    const uint64_t groups = nz_ceil_div(k, kGroup), waves = nz_mul(m, groups);
+    if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
+    nz_mx_rounded_kernel<<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
+        (const float*)dev_x, stride, (uint32_t)k, waves, (uint32_t)groups, (nz_bf16*)(base + room.values));
+    return launch_wide(m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, room, base, st);
+  }
   if (int rc = launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st)) return rc;
   return launch_product(base + room.xd, base + room.xs, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y,
                         dtype, room, base, st);

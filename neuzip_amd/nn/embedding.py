@@ -69,7 +69,7 @@ class Embedding(torch.nn.Module):
 
     def _rows(self, x):
         rows = self._lookup(x)
-        # the table's values are bf16 numbers: this product (in 32 bits) is the only rounding; the rows are the call's own
+        # a product in 32 bits, rounded to bf16; the rows are the call's own
         return rows if self.scale == 1.0 else rows.mul_(self.scale)
 
     def _lookup(self, x):

@@ -274,7 +274,7 @@ def mx_linear(x, weight: MXTensor, bias=None, dtype=None) -> torch.Tensor:
 def mx_embedding(indices: torch.Tensor, table: MXTensor, scale: float = 1.0, dtype: torch.dtype = torch.bfloat16,
                  status=None) -> torch.Tensor:
     """Rows ``indices`` (any integer shape) of a table in microscaled form, times
-    ``scale``, rounded once to ``dtype``.  An index outside the table gives a row
+    ``scale`` in 32 bits, rounded to ``dtype``.  An index outside the table gives a row
     of zeros and sets bit 0 of ``status`` (an int32 tensor of one element)."""
     if not isinstance(table, MXTensor) or len(table.shape) != 2:
         raise ValueError("table must be a matrix in microscaled form (mx_quantize)")

@@ -385,7 +385,7 @@ def test_lookup_scales_and_rounds_once(rows, cols, count, dtype):
     q = ops.mx_quantize(table.to(DEV), 4)
     ids = torch.randint(0, rows, (count,), generator=torch.Generator().manual_seed(1))
     for scale in (1.0, 0.1, math.sqrt(cols)):
-        # a value has 2 bits, the scale is a float32: their product is exact in 32 bits
+        # a value has 2 bits, the scale 24: rounding their product to 24 bits first shows only next to ties
         want = held(table, 4)[ids] * torch.tensor(scale, dtype=torch.float32).double()
         same(ops.mx_embedding(ids.to(DEV), q, scale, dtype), round_to(want, dtype))
     same(ops.mx_embedding(ids.to(DEV).int().view(1, -1), q, 1.0, dtype), round_to(held(table, 4)[ids], dtype)[None])
