@@ -6,7 +6,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from neuzip_amd import _lib
-from neuzip_amd.ops.microscaled import _as_rows, _call, _dtype_code, _on_gpu, _workspace
+from neuzip_amd.ops.microscaled import _as_rows, _call, _dtype_code, _on_gpu, _table_room, _workspace
 
 
 def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings: int, scale: float = 1.0,
@@ -46,7 +46,7 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     idx = idx.contiguous()
     count = idx.numel()
     g, _, stride = _as_rows(grad, cols)
-    room = L.nz_embedding_gradient_workspace_bytes(count, cols)
+    room = _table_room(count, cols)
     ws, at = _workspace(room, g)
     _call(L.nz_embedding_gradient, index, idx.data_ptr(), count, g.data_ptr(), code, stride, num_embeddings, cols,
           float(scale), -1 if padding_idx is None else padding_idx, flags, out.data_ptr(), at, room)

@@ -13,6 +13,7 @@ The kernels are part of libneuzip_hip.so; there is no fallback without a GPU.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -72,6 +73,24 @@ def _as_rows(t: torch.Tensor, width: int):
     return rows, rows.shape[0], rows.stride(0)
 
 
+# What sizes alone decide is asked of the library once.
+@lru_cache(maxsize=1024)
+def _row_sizes(cols: int, bits: int):
+    """Bytes of a row's codes and of its scales."""
+    L = _lib.load()
+    return L.nz_mx_row_bytes(cols, bits), L.nz_mx_scale_bytes(cols)
+
+
+@lru_cache(maxsize=1024)
+def _product_room(m: int, n: int, k: int, code: int) -> int:
+    return _lib.load().nz_mx_linear_workspace_bytes(m, n, k, code)
+
+
+@lru_cache(maxsize=1024)
+def _table_room(count: int, cols: int) -> int:
+    return _lib.load().nz_embedding_gradient_workspace_bytes(count, cols)
+
+
 def _workspace(room: int, like: torch.Tensor):
     """(the tensor that keeps it, its address)"""
     if not room:
@@ -96,9 +115,8 @@ class MXTensor:
             raise ValueError("bits must be 4 or 8")
         if len(shape) < 1:
             raise ValueError("a microscaled tensor has one dimension at least")
-        L, rows = _lib.load(), math.prod(shape[:-1])
-        want = ((rows, L.nz_mx_row_bytes(shape[-1], bits)), (rows, L.nz_mx_scale_bytes(shape[-1])))
-        for name, t, size in (("data", data, want[0]), ("scales", scales, want[1])):
+        rows, sizes = math.prod(shape[:-1]), _row_sizes(shape[-1], bits)
+        for name, t, size in (("data", data, (rows, sizes[0])), ("scales", scales, (rows, sizes[1]))):
             if t.dtype != torch.uint8 or tuple(t.shape) != size or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous uint8 tensor of shape {size}")
         if data.device != scales.device:
@@ -151,11 +169,12 @@ def mx_quantize(x: torch.Tensor, bits: int = 4) -> MXTensor:
     shape = x.shape
     if not shape:
         raise ValueError("x must have one dimension at least")
-    L, cols = _lib.load(), shape[-1]
+    cols = shape[-1]
     rows, n, stride = _as_rows(x, cols)
-    data = x.new_empty((n, L.nz_mx_row_bytes(cols, bits)), dtype=torch.uint8)
-    scales = x.new_empty((n, L.nz_mx_scale_bytes(cols)), dtype=torch.uint8)
-    _call(L.nz_mx_quantize, index, rows.data_ptr(), code, n, cols, stride, bits, data.data_ptr(), scales.data_ptr())
+    sizes = _row_sizes(cols, bits)
+    data = x.new_empty((n, sizes[0]), dtype=torch.uint8)
+    scales = x.new_empty((n, sizes[1]), dtype=torch.uint8)
+    _call(_lib.load().nz_mx_quantize, index, rows.data_ptr(), code, n, cols, stride, bits, data.data_ptr(), scales.data_ptr())
     return MXTensor._of(data, scales, shape, bits)
 
 
@@ -182,7 +201,7 @@ def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
         m = xt.shape[0]
     else:
         xt, m, stride = _as_rows(x, k)
-    room = L.nz_mx_linear_workspace_bytes(m, n, k, code)
+    room = _product_room(m, n, k, code)
     ws, at = _workspace(room, xt)
     if held:
         _call(L.nz_mx_linear_rows8, index, xt.data_ptr(), x.scales.data_ptr(), m, k, wd.data_ptr(),
