@@ -62,6 +62,14 @@ def _call(fn, index: int, *args) -> None:
         _lib.raise_for(rc)
 
 
+def _ask(fn, index: int, *args) -> int:
+    """What a native call answers for device ``index``, whose compute units count."""
+    if index == _current_device():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def _as_rows(t: torch.Tensor, width: int):
     """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it): the
     tensor, its rows, elements from row to row."""
@@ -82,8 +90,8 @@ def _row_sizes(cols: int, bits: int):
 
 
 @lru_cache(maxsize=1024)
-def _product_room(m: int, n: int, k: int, code: int) -> int:
-    return _lib.load().nz_mx_linear_workspace_bytes(m, n, k, code)
+def _product_room(index: int, m: int, n: int, k: int, code: int) -> int:
+    return _ask(_lib.load().nz_mx_linear_workspace_bytes, index, m, n, k, code)
 
 
 @lru_cache(maxsize=1024)
@@ -201,7 +209,7 @@ def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
         m = xt.shape[0]
     else:
         xt, m, stride = _as_rows(x, k)
-    room = _product_room(m, n, k, code)
+    room = _product_room(index, m, n, k, code)
     ws, at = _workspace(room, xt)
     if held:
         _call(L.nz_mx_linear_rows8, index, xt.data_ptr(), x.scales.data_ptr(), m, k, wd.data_ptr(),
@@ -221,7 +229,7 @@ def _input_gradient(grad: torch.Tensor, weight: MXTensor) -> torch.Tensor:
         return dx.zero_()
     rows, m, stride = _as_rows(grad, n)
     args = (rows.data_ptr(), _dtype_code(grad.dtype), m, n, stride)
-    room = L.nz_mx_linear_grad_workspace_bytes(*args, k)
+    room = _ask(L.nz_mx_linear_grad_workspace_bytes, index, *args, k)
     ws, at = _workspace(room, rows)
     _call(L.nz_mx_linear_grad, index, *args, weight.data.data_ptr(), weight.scales.data_ptr(), k, dx.data_ptr(), at,
           room)
