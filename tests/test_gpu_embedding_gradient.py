@@ -42,11 +42,13 @@ def summed(ids, g, rows, skip=None):
     return total, size, torch.bincount(ids[ok], minlength=rows).double()[:, None]
 
 
-CASES = [("uniform", 1, 1, 1), ("uniform", 5, 7, 3), ("text", 100, 40, 33), ("uniform", 64, 1000, 8), ("one", 257, 9, 64),
-         ("text", 2000, 5003, 129), ("two", 1030, 300, 520), ("descending", 700, 350, 1021), ("text", 4099, 50257, 40),
-         ("one", 3000, 2, 513), ("uniform", 9000, 1500, 24), ("text", 20000, 3001, 16), ("one", 70000, 3, 8),
-         ("text", 1023, 400, 24), ("text", 1024, 50257, 520), ("one", 1024, 2, 100), ("two", 1025, 30, 17),
-         ("uniform", 17, 1, 40), ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("text", 10000, 600000, 9), ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
+CASES = [("uniform", 1, 1, 1), ("uniform", 5, 7, 3), ("text", 100, 40, 33), ("uniform", 64, 1000, 8),
+         ("one", 257, 9, 64), ("text", 2000, 5003, 129), ("two", 1030, 300, 520), ("descending", 700, 350, 1021),
+         ("text", 4099, 50257, 40), ("one", 3000, 2, 513), ("uniform", 9000, 1500, 24), ("text", 20000, 3001, 16),
+         ("text", 16385, 900, 40), ("two", 32768, 11, 24), ("one", 70000, 3, 8), ("text", 1023, 400, 24),
+         ("text", 1024, 50257, 520), ("one", 1024, 2, 100), ("two", 1025, 30, 17), ("uniform", 17, 1, 40),
+         ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("text", 10000, 600000, 9),
+         ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
