@@ -108,14 +108,18 @@ __device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t row) {
 }
 
 __global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* tiles, uint32_t count, Place* places) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
+  // eight lanes a token, each for every eighth tile: a bisection is a chain of loads
+  const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t i = (uint32_t)min(id / 8, (uint64_t)count - 1), part = threadIdx.x & 7;
   const Place p = tiles[i];
   const uint32_t own = i / kTile * kTile;
-  uint32_t at = i - own;
-  for (uint32_t base = 0; base < count; base += kTile)  // equal ones of the tiles before stand before
+  uint32_t at = 0;
+  for (uint32_t base = part * kTile; base < count; base += 8 * kTile)  // equal ones of the tiles before stand before
     if (base != own) at += below(tiles + base, min(kTile, count - base), (uint64_t)p.row + (base < own));
-  places[at] = p;
+  at += __shfl_xor(at, 1);
+  at += __shfl_xor(at, 2);
+  at += __shfl_xor(at, 4);
+  if (part == 0 && id / 8 < count) places[i - own + at] = p;
 }
 
 template <class T>
@@ -431,7 +435,7 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
                                                              (uint8_t*)dev_out, bytes);
   }
   if (count > kTile)
-    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 256), 256, 0, st>>>(tiles, (uint32_t)count, places);
+    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 32), 256, 0, st>>>(tiles, (uint32_t)count, places);
   const auto add_up = [&](auto type) {
     using T = decltype(type);
     const T* g = (const T*)dev_g;
