@@ -4,7 +4,7 @@
 // while some of its workgroups sort the tokens (clearing is bound by memory, sorting by arithmetic and latency); the
 // others add up the rows of g.  The launches:
 //
-//   sort   32 tokens a workgroup; a token's place among the 8192 of its tile is the number of smaller keys (index, then
+//   sort   32 tokens a workgroup; a token's place among the up to 8192 of its tile is the number of smaller keys (index, then
 //          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
 //          the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
 //   merge  (more than one tile) the place among all tokens: the same count in the other tiles, by bisection.
@@ -16,11 +16,13 @@
 //
 // 8192 tokens of a text in 50257x1024 (bf16): 16.7 + 11.6 + 5.5 us, where clearing alone takes 15 (6.8 TB/s); 2048 in
 // 128256x4096: 167 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
+#include <type_traits>
+
 #include "nz_operators.h"
 
 namespace {
 
-constexpr uint32_t kTile = 8192;      // tokens that are compared with each other
+constexpr uint32_t kTile = 8192;      // tokens that are compared with each other, at most
 constexpr uint32_t kTileBits = 13;
 constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
 constexpr uint32_t kClear = 1 << 14;  // bytes a workgroup clears
@@ -32,7 +34,7 @@ struct Place {
   uint32_t row, token;
 };
 
-template <class Key>
+template <class Key, uint32_t TILE>
 __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long* index, uint32_t count, uint32_t rows,
                                                                 long long skip, Place* places, uint32_t sorters,
                                                                 uint8_t* out, uint64_t bytes) {
@@ -53,17 +55,17 @@ __global__ __launch_bounds__(512) void nz_embedding_sort_kernel(const long long*
     return;
   }
   typedef Key key4 __attribute__((ext_vector_type(4)));
-  __shared__ __attribute__((aligned(32))) Key keys[kTile];
+  __shared__ __attribute__((aligned(32))) Key keys[TILE];
   __shared__ uint32_t smaller[8][kSorted];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const uint32_t block = blockIdx.x % (kTile / kSorted), base = blockIdx.x / (kTile / kSorted) * kTile;
-  const uint32_t here = min(kTile, count - base), rounds = (here + 255) / 256;
-  long long value[kTile / 512];
+  const uint32_t block = blockIdx.x % (TILE / kSorted), base = blockIdx.x / (TILE / kSorted) * TILE;
+  const uint32_t here = min(TILE, count - base), rounds = (here + 255) / 256;
+  long long value[TILE / 512];
 #pragma unroll
-  for (uint32_t j = 0; j < kTile / 512; ++j)  // all on their way at once
+  for (uint32_t j = 0; j < TILE / 512; ++j)  // all on their way at once
     if (j * 512 < here) value[j] = index[base + min(j * 512 + threadIdx.x, here - 1)];
 #pragma unroll
-  for (uint32_t j = 0; j < kTile / 512; ++j) {
+  for (uint32_t j = 0; j < TILE / 512; ++j) {
     const uint32_t i = j * 512 + threadIdx.x;
     const long long v = i < here ? value[j] : -1;
     const uint32_t row = v >= 0 && v < (long long)rows && v != skip ? (uint32_t)v : rows;
@@ -107,15 +109,16 @@ __device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t row) {
   return lo;
 }
 
-__global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* tiles, uint32_t count, Place* places) {
+__global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* tiles, uint32_t count, uint32_t tile,
+                                                                 Place* places) {
   // eight lanes a token, each for every eighth tile: a bisection is a chain of loads
   const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t i = (uint32_t)min(id / 8, (uint64_t)count - 1), part = threadIdx.x & 7;
   const Place p = tiles[i];
-  const uint32_t own = i / kTile * kTile;
+  const uint32_t own = i / tile * tile;
   uint32_t at = 0;
-  for (uint32_t base = part * kTile; base < count; base += 8 * kTile)  // equal ones of the tiles before stand before
-    if (base != own) at += below(tiles + base, min(kTile, count - base), (uint64_t)p.row + (base < own));
+  for (uint32_t base = part * tile; base < count; base += 8 * tile)  // equal ones of the tiles before stand before
+    if (base != own) at += below(tiles + base, min(tile, count - base), (uint64_t)p.row + (base < own));
   at += __shfl_xor(at, 1);
   at += __shfl_xor(at, 2);
   at += __shfl_xor(at, 4);
@@ -374,6 +377,13 @@ bool unsorted(uint64_t count, uint64_t cols) {
   return count <= kFew && count * count * nz_ceil_div(cols, 512) <= (uint64_t)kFew * kFew;
 }
 
+// Tokens that are sorted among each other.  Up to 8192 need no second launch; above, comparing takes count x tile steps
+// and finding the places among the other tiles count^2 / tile.  Tables of 32000x64, tiles of 8192, 4096 and 2048: 16384
+// tokens 38, 32, 29 us; 65536 82, 70, 70; 131072 137, 124, 140; 262144 302, 310, 408.
+uint32_t tile_of(uint64_t count) {
+  return count <= kTile ? kTile : count <= 65536 ? kTile / 4 : count <= 196608 ? kTile / 2 : kTile;
+}
+
 // Where the workspace holds what: sorted tiles (more than one), places, pieces.
 struct Room {
   uint64_t places, pieces, bytes;
@@ -423,19 +433,30 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   Place *places = (Place*)(ws + room.places), *tiles = (Place*)ws;
   Place* sorted = count > kTile ? tiles : places;
   const dim3 grid((uint32_t)clearers + sorters);
+  const uint32_t tile = tile_of(count);
+  const auto sort = [&](auto key, auto size) {
+    constexpr uint32_t TILE = decltype(size)::value;
+    nz_embedding_sort_kernel<decltype(key), TILE><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
+                                                                        (uint32_t)rows, padding_idx, sorted, sorters,
+                                                                        (uint8_t*)dev_out, bytes);
+  };
+  const auto sort_by = [&](auto key) {
+    if (tile == kTile)
+      sort(key, std::integral_constant<uint32_t, kTile>());
+    else if (tile == kTile / 2)
+      sort(key, std::integral_constant<uint32_t, kTile / 2>());
+    else
+      sort(key, std::integral_constant<uint32_t, kTile / 4>());
+  };
   if (grid.x == 0) {
     // few tokens added to a table: nothing to clear or to sort
   } else if (rows < 1u << (32 - kTileBits)) {
-    nz_embedding_sort_kernel<uint32_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
-                                                             (uint32_t)rows, padding_idx, sorted, sorters,
-                                                             (uint8_t*)dev_out, bytes);
+    sort_by(uint32_t());
   } else {
-    nz_embedding_sort_kernel<uint64_t><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
-                                                             (uint32_t)rows, padding_idx, sorted, sorters,
-                                                             (uint8_t*)dev_out, bytes);
+    sort_by(uint64_t());
   }
   if (count > kTile)
-    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 32), 256, 0, st>>>(tiles, (uint32_t)count, places);
+    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 32), 256, 0, st>>>(tiles, (uint32_t)count, tile, places);
   const auto add_up = [&](auto type) {
     using T = decltype(type);
     const T* g = (const T*)dev_g;
