@@ -7,16 +7,17 @@
 //   sort   32 tokens a workgroup; a token's place among the up to 8192 of its tile is the number of smaller keys (index, then
 //          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
 //          the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
-//   merge  (more than one tile) the place among all tokens: the same count in the other tiles, by bisection.
+//   merge  (more than one tile) 8 or 16 sorted runs become one: the same count in the other runs, by bisection.
 //   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
 //          lie in one window is done; what reaches beyond it is kept as a piece.
 //   join   the pieces of rows that reach over several windows, in their order.
 //
 // Few tokens are not sorted but compared with each other where they are added up.
 //
-// 8192 tokens of a text in 50257x1024 (bf16): 16.7 + 11.6 + 5.5 us, where clearing alone takes 15 (6.8 TB/s); 2048 in
-// 128256x4096: 167 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
+// 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11.4 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
+// 8 + 25 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
 #include <type_traits>
+#include <utility>
 
 #include "nz_operators.h"
 
@@ -27,6 +28,7 @@ constexpr uint32_t kTileBits = 13;
 constexpr uint32_t kSorted = 32;      // tokens that a workgroup places
 constexpr uint32_t kClear = 1 << 14;  // bytes a workgroup clears
 constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
+constexpr uint32_t kJoin = 4;         // wavefronts that join a row's pieces
 constexpr uint32_t kFew = 2048;       // tokens that may go unsorted
 
 // A sorted token: its index (the number of rows if it takes no part) and where it stands.
@@ -109,20 +111,23 @@ __device__ inline uint32_t below(const Place* tile, uint32_t n, uint64_t row) {
   return lo;
 }
 
-__global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* tiles, uint32_t count, uint32_t tile,
-                                                                 Place* places) {
-  // eight lanes a token, each for every eighth tile: a bisection is a chain of loads
+// `fan` sorted runs of `run` places each become one: a place moves up by the number of places of the other runs that
+// stand before it.  Eight lanes a place, each for every eighth run: a bisection is a chain of loads.
+__global__ __launch_bounds__(256) void nz_embedding_merge_kernel(const Place* from, uint32_t count, uint32_t run,
+                                                                 uint32_t fan, Place* to) {
   const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
   const uint32_t i = (uint32_t)min(id / 8, (uint64_t)count - 1), part = threadIdx.x & 7;
-  const Place p = tiles[i];
-  const uint32_t own = i / tile * tile;
+  const Place p = from[i];
+  const uint64_t own = i / run * run, first = i / run / fan * fan * (uint64_t)run;
+  const uint64_t end = min((uint64_t)count, first + fan * (uint64_t)run);
   uint32_t at = 0;
-  for (uint32_t base = part * tile; base < count; base += 8 * tile)  // equal ones of the tiles before stand before
-    if (base != own) at += below(tiles + base, min(tile, count - base), (uint64_t)p.row + (base < own));
+  for (uint64_t base = first + part * (uint64_t)run; base < end; base += 8 * (uint64_t)run)
+    if (base != own)  // equal ones of the runs before stand before
+      at += below(from + base, (uint32_t)min((uint64_t)run, count - base), (uint64_t)p.row + (base < own));
   at += __shfl_xor(at, 1);
   at += __shfl_xor(at, 2);
   at += __shfl_xor(at, 4);
-  if (part == 0 && id / 8 < count) places[i - own + at] = p;
+  if (part == 0 && id / 8 < count) to[first + (i - own) + at] = p;
 }
 
 template <class T>
@@ -239,14 +244,17 @@ __global__ __launch_bounds__(256) void nz_embedding_sum_kernel(const Place* plac
   }
 }
 
-// One wavefront per 512 columns and window: the row that begins in it and goes on behind it, if there is one.
+// One workgroup per 512 columns and window: the row that begins in it and goes on behind it, if there is one.  Its
+// pieces are many where a row has many tokens (those that fill up a batch): the wavefronts take a part each.  32768
+// tokens, half of them the same: 21 us, 57 by one wavefront; eight wavefronts 18, but 13 instead of 9.6 for a text.
 template <class T>
-__global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* places, uint32_t count, uint32_t rows,
-                                                                uint32_t size, uint32_t cols, uint32_t slices,
-                                                                float scale, uint32_t flags, T* out,
-                                                                const float* pieces) {
-  const uint64_t id = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  const uint64_t window = id / slices, first = window * size, next = first + size;
+__global__ __launch_bounds__(64 * kJoin) void nz_embedding_join_kernel(const Place* places, uint32_t count,
+                                                                       uint32_t rows, uint32_t size, uint32_t cols,
+                                                                       uint32_t slices, float scale, uint32_t flags,
+                                                                       T* out, const float* pieces) {
+  __shared__ float sums[kJoin - 1][64][9];  // a ninth: lanes apart in their banks
+  const uint32_t window = blockIdx.x / slices, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint64_t first = (uint64_t)window * size, next = first + size;
   if (next >= count) return;
   // the places around the window's borders, asked for together
   const uint32_t lane = threadIdx.x & 63, row = places[next - 1].row, behind = places[next].row;
@@ -272,20 +280,33 @@ __global__ __launch_bounds__(256) void nz_embedding_join_kernel(const Place* pla
       tokens += __popcll(__ballot(i + lane < size && at < count && places[min(at, (uint64_t)count - 1)].row == row));
     }
   }
-  const Columns k = columns_of((uint32_t)(id - window * slices), lane, cols);
-  float sum[8];
-  load8(pieces + piece_at(window, 1, cols), k, cols, sum);
-  for (uint32_t q = 1; q <= more; q += 16) {
+  const Columns k = columns_of(blockIdx.x - window * slices, lane, cols);
+  const uint32_t share = more <= 16 ? 16 : (more + kJoin - 1) / kJoin, begins = 1 + wave * share;
+  const uint32_t last = min(more, begins + share - 1);
+  float sum[8] = {};
+  if (wave == 0) load8(pieces + piece_at(window, 1, cols), k, cols, sum);
+  for (uint32_t q = begins; q <= last; q += 16) {
     float v[16][8];
 #pragma unroll
     for (uint32_t j = 0; j < 16; ++j)  // the last piece again where there are fewer
-      load8(pieces + piece_at(window + min(q + j, more), 0, cols), k, cols, v[j]);
+      load8(pieces + piece_at(window + min(q + j, last), 0, cols), k, cols, v[j]);
 #pragma unroll
     for (uint32_t j = 0; j < 16; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = q + j <= more ? sum[e] + v[j][e] : sum[e];
+      for (int e = 0; e < 8; ++e) sum[e] = q + j <= last ? sum[e] + v[j][e] : sum[e];
   }
-  if (k.n) put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
+  if (more > 16) {
+    if (wave)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[wave - 1][lane][e] = sum[e];
+    __syncthreads();
+    if (wave == 0)
+#pragma unroll
+      for (uint32_t w = 0; w < kJoin - 1; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += sums[w][lane][e];
+  }
+  if (wave == 0 && k.n) put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
 }
 
 // Few tokens, without sorting them: one workgroup per 512 columns of a token looks for the token's index among
@@ -377,23 +398,19 @@ bool unsorted(uint64_t count, uint64_t cols) {
   return count <= kFew && count * count * nz_ceil_div(cols, 512) <= (uint64_t)kFew * kFew;
 }
 
-// Tokens that are sorted among each other.  Up to 8192 need no second launch; above, comparing takes count x tile steps
-// and finding the places among the other tiles count^2 / tile.  Tables of 32000x64, tiles of 8192, 4096 and 2048: 16384
-// tokens 38, 32, 29 us; 65536 82, 70, 70; 131072 137, 124, 140; 262144 302, 310, 408.
-uint32_t tile_of(uint64_t count) {
-  return count <= kTile ? kTile : count <= 65536 ? kTile / 4 : count <= 196608 ? kTile / 2 : kTile;
-}
+// Tokens that are sorted among each other: up to 8192 need no second launch; above, comparing takes count x tile steps.
+uint32_t tile_of(uint64_t count) { return count <= kTile ? kTile : kTile / 4; }
 
-// Where the workspace holds what: sorted tiles (more than one), places, pieces.
+// Where the workspace holds what: places, once more (if runs of them are merged), pieces.
 struct Room {
-  uint64_t places, pieces, bytes;
+  uint64_t again, pieces, bytes;
 };
 Room room_of(uint64_t count, uint64_t cols) {
   const uint64_t window = window_of(count);
   Room r = {};
   if (unsorted(count, cols)) return r;
-  r.places = count > kTile ? align256(count * sizeof(Place)) : 0;
-  r.pieces = r.places + align256(count * sizeof(Place));
+  r.again = align256(count * sizeof(Place));
+  r.pieces = count > kTile ? 2 * r.again : r.again;
   r.bytes = r.pieces + nz_mul(nz_ceil_div(count, window) * 2 * 4, cols);
   return r;
 }
@@ -430,21 +447,18 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   if (clearers + sorters > 0x7FFFFFFFull) return nz_fail(NZ_ERR_ARG, "table too large for one launch");
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)dev_workspace;
-  Place *places = (Place*)(ws + room.places), *tiles = (Place*)ws;
-  Place* sorted = count > kTile ? tiles : places;
+  Place *places = (Place*)ws, *other = (Place*)(ws + room.again);
   const dim3 grid((uint32_t)clearers + sorters);
   const uint32_t tile = tile_of(count);
   const auto sort = [&](auto key, auto size) {
     constexpr uint32_t TILE = decltype(size)::value;
     nz_embedding_sort_kernel<decltype(key), TILE><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
-                                                                        (uint32_t)rows, padding_idx, sorted, sorters,
+                                                                        (uint32_t)rows, padding_idx, places, sorters,
                                                                         (uint8_t*)dev_out, bytes);
   };
   const auto sort_by = [&](auto key) {
     if (tile == kTile)
       sort(key, std::integral_constant<uint32_t, kTile>());
-    else if (tile == kTile / 2)
-      sort(key, std::integral_constant<uint32_t, kTile / 2>());
     else
       sort(key, std::integral_constant<uint32_t, kTile / 4>());
   };
@@ -455,8 +469,14 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   } else {
     sort_by(uint64_t());
   }
-  if (count > kTile)
-    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 32), 256, 0, st>>>(tiles, (uint32_t)count, tile, places);
+  // 16 runs at a time if that ends it: 51 us for 262144 places, 28 + 28 in two passes of 8 and 2
+  for (uint64_t run = tile; !few && run < count;) {
+    const uint32_t fan = nz_ceil_div(count, run) <= 16 ? 16 : 8;
+    nz_embedding_merge_kernel<<<(uint32_t)nz_ceil_div(count, 32), 256, 0, st>>>(places, (uint32_t)count, (uint32_t)run,
+                                                                               fan, other);
+    std::swap(places, other);
+    run *= fan;
+  }
   const auto add_up = [&](auto type) {
     using T = decltype(type);
     const T* g = (const T*)dev_g;
@@ -472,8 +492,8 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
     const uint32_t waves = (uint32_t)nz_ceil_div(nz_ceil_div(count, window) * slices, 4);
     nz_embedding_sum_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, g, stride,
                                                       (uint32_t)cols, (uint32_t)slices, scale, flags, out, pieces);
-    nz_embedding_join_kernel<T><<<waves, 256, 0, st>>>(places, (uint32_t)count, (uint32_t)rows, window, (uint32_t)cols,
-                                                       (uint32_t)slices, scale, flags, out, pieces);
+    nz_embedding_join_kernel<T><<<(uint32_t)(nz_ceil_div(count, window) * slices), 64 * kJoin, 0, st>>>(
+        places, (uint32_t)count, (uint32_t)rows, window, (uint32_t)cols, (uint32_t)slices, scale, flags, out, pieces);
   };
   if (count == 0) {
   } else if (dtype == NZ_DTYPE_BF16) {

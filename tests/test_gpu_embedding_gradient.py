@@ -49,15 +49,15 @@ CASES = [("uniform", 1, 1, 1), ("uniform", 5, 7, 3), ("text", 100, 40, 33), ("un
          ("text", 1024, 50257, 520), ("one", 1024, 2, 100), ("two", 1025, 30, 17), ("uniform", 17, 1, 40),
          ("two", 1000, 8, 1540), ("text", 70001, 130000, 8), ("text", 10000, 600000, 9),
          ("uniform", 300, 140000, 16), ("uniform", 1, 5, 4096), ("uniform", 200001, 900, 8), ("text", 66000, 600000, 4),
-         ("text", 200000, 700000, 4)]
+         ("text", 200000, 700000, 4), ("text", 1100000, 3000, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("kind,count,rows,cols", CASES)
 def test_whole_numbers_are_exact(kind, count, rows, cols, dtype):
-    """whole numbers up to 100 in magnitude: 70000 of them (60 where there are more) stay below 2^24"""
+    """whole numbers up to 100 in magnitude: 70000 of them (200000 up to 60, 1100000 up to 15) stay below 2^24"""
     ids = tokens(kind, count, rows, seed=count)
-    most = 100 if count <= 70001 else 60
+    most = 100 if count <= 70001 else 60 if count <= 200001 else 15
     g = torch.randint(-most, most + 1, (count, cols), generator=torch.Generator().manual_seed(1)).to(dtype)
     total, _, _ = summed(ids, g, rows)
     got = ops.embedding_gradient(ids.to(DEV), g.to(DEV), rows, 0.5)
