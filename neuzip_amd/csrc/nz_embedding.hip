@@ -15,7 +15,7 @@
 // Few tokens are not sorted but compared with each other where they are added up.
 //
 // 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11.4 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
-// 8 + 25 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
+// 8 + 22 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
 #include <type_traits>
 #include <utility>
 
@@ -30,6 +30,7 @@ constexpr uint32_t kClear = 1 << 14;  // bytes a workgroup clears
 constexpr uint32_t kBatch = 16;       // rows of g that a wavefront has on their way at a time
 constexpr uint32_t kJoin = 4;         // wavefronts that join a row's pieces
 constexpr uint32_t kFew = 2048;       // tokens that may go unsorted
+constexpr uint32_t kFewWaves = 8;     // wavefronts that look for them: 2048 in 30000x512 13 us, by 4 14.5, by 16 19
 
 // A sorted token: its index (the number of rows if it takes no part) and where it stands.
 struct Place {
@@ -211,22 +212,24 @@ __global__ __launch_bounds__(256) void nz_embedding_sum_kernel(const Place* plac
   for (uint32_t at = (uint32_t)first; at < end; at += kBatch) {
     // lanes 0 .. 15: the places of the batch; lanes 1 .. 16 look at the one behind each
     const Place mine = places[min(at + lane, count - 1)];
-    typename Pack<T>::type v[kBatch];
-    float w[kBatch][8];
+    typename Pack<T>::type v[kBatch];  // raw, for all to be on their way before the first is used
+    if (k.whole) {
 #pragma unroll
-    for (uint32_t j = 0; j < kBatch; ++j) {
-      const T* row = g + __builtin_amdgcn_readlane(mine.token, j) * stride;
-      if (k.whole)
-        v[j] = *(const typename Pack<T>::type*)(row + k.c);
-      else
-        load8(row, k, cols, w[j]);
+      for (uint32_t j = 0; j < kBatch; ++j)
+        v[j] = *(const typename Pack<T>::type*)(g + __builtin_amdgcn_readlane(mine.token, j) * stride + k.c);
+    } else {  // narrower than a load
+#pragma unroll
+      for (uint32_t j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+          v[j][e] = e < cols ? g[__builtin_amdgcn_readlane(mine.token, j) * stride + e] : (T)0;
     }
 #pragma unroll
     for (uint32_t j = 0; j < kBatch; ++j) {
       if (at + j >= end) break;
       const uint32_t row = __builtin_amdgcn_readlane(mine.row, j);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += k.whole ? (float)v[j][e] : w[j][e];
+      for (int e = 0; e < 8; ++e) sum[e] += (float)v[j][e];
       ++tokens;
       const bool ends = at + j + 1 == count || __builtin_amdgcn_readlane(mine.row, j + 1) != row;
       if (!ends && at + j + 1 < end) continue;
@@ -246,7 +249,8 @@ __global__ __launch_bounds__(256) void nz_embedding_sum_kernel(const Place* plac
 
 // One workgroup per 512 columns and window: the row that begins in it and goes on behind it, if there is one.  Its
 // pieces are many where a row has many tokens (those that fill up a batch): the wavefronts take a part each.  32768
-// tokens, half of them the same: 21 us, 57 by one wavefront; eight wavefronts 18, but 13 instead of 9.6 for a text.
+// tokens, half of them the same: 18 us, 57 by one wavefront; eight are faster there, but take 13 instead of
+// 9.6 us for a text.
 template <class T>
 __global__ __launch_bounds__(64 * kJoin) void nz_embedding_join_kernel(const Place* places, uint32_t count,
                                                                        uint32_t rows, uint32_t size, uint32_t cols,
@@ -286,10 +290,19 @@ __global__ __launch_bounds__(64 * kJoin) void nz_embedding_join_kernel(const Pla
   float sum[8] = {};
   if (wave == 0) load8(pieces + piece_at(window, 1, cols), k, cols, sum);
   for (uint32_t q = begins; q <= last; q += 16) {
-    float v[16][8];
+    Pack<float>::type v[16];
+    const auto piece = [&](uint32_t j) {  // the last one again where there are fewer
+      return pieces + piece_at(window + min(q + j, last), 0, cols);
+    };
+    if (k.whole) {
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j)  // the last piece again where there are fewer
-      load8(pieces + piece_at(window + min(q + j, last), 0, cols), k, cols, v[j]);
+      for (uint32_t j = 0; j < 16; ++j) v[j] = *(const Pack<float>::type*)(piece(j) + k.c);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j)
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[j][e] = e < cols ? piece(j)[e] : 0.0f;
+    }
 #pragma unroll
     for (uint32_t j = 0; j < 16; ++j)
 #pragma unroll
@@ -309,65 +322,85 @@ __global__ __launch_bounds__(64 * kJoin) void nz_embedding_join_kernel(const Pla
   if (wave == 0 && k.n) put8(out + row * (uint64_t)cols, k, cols, sum, tokens, scale, flags);
 }
 
-// Few tokens, without sorting them: one workgroup per 512 columns of a token looks for the token's index among
-// all of them (a quarter a wavefront).  Where it is the first of its row it adds up the row, again a quarter of the
-// tokens a wavefront if there are many, in their order; else it is done.
+// Few tokens, without sorting them: one workgroup per 512 columns of a token looks for the token's index among all of
+// them, a part a wavefront.  Where it is the first of its row it adds up the row, again a part a wavefront if there are
+// many, in their order; else it is done.
 template <class T>
-__global__ __launch_bounds__(256) void nz_embedding_few_kernel(const long long* index, uint32_t count, uint32_t rows,
-                                                               long long skip, const T* g, uint64_t stride,
-                                                               uint32_t cols, uint32_t slices, float scale,
-                                                               uint32_t flags, T* out) {
-  constexpr uint32_t kQuarter = kFew / 4;
-  __shared__ uint32_t found[4];
-  __shared__ uint16_t list[4][kQuarter];
-  __shared__ float sums[3][64][9];  // a ninth: lanes apart in their banks
+__global__ __launch_bounds__(64 * kFewWaves) void nz_embedding_few_kernel(const long long* index, uint32_t count,
+                                                                          uint32_t rows, long long skip, const T* g,
+                                                                          uint64_t stride, uint32_t cols,
+                                                                          uint32_t slices, float scale, uint32_t flags,
+                                                                          T* out) {
+  constexpr uint32_t W = kFewWaves, kPart = kFew / W;
+  __shared__ uint32_t found[W];
+  __shared__ uint16_t list[kFew];
+  __shared__ float sums[W - 1][64][9];  // a ninth: lanes apart in their banks
   const uint32_t token = blockIdx.x / slices, lane = threadIdx.x & 63;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const long long row = index[token];
   if (row < 0 || row >= (long long)rows || row == skip) return;
-  bool hit[kQuarter / 64];
+  bool hit[kPart / 64];
 #pragma unroll
-  for (uint32_t j = 0; j < kQuarter / 64; ++j) {
-    const uint32_t at = wave * kQuarter + j * 64 + lane;
+  for (uint32_t j = 0; j < kPart / 64; ++j) {
+    const uint32_t at = wave * kPart + j * 64 + lane;
     hit[j] = index[min(at, count - 1)] == row && at < count;
   }
   uint32_t n = 0;
   bool earlier = false;
 #pragma unroll
-  for (uint32_t j = 0; j < kQuarter / 64; ++j) {
-    const uint32_t at = wave * kQuarter + j * 64;
+  for (uint32_t j = 0; j < kPart / 64; ++j) {
     const uint64_t mask = __ballot(hit[j]);
-    earlier |= mask && at + __builtin_ctzll(mask) < token;
-    if (hit[j]) list[wave][n + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(at + lane);
+    earlier |= mask && wave * kPart + j * 64 + __builtin_ctzll(mask) < token;
     n += __popcll(mask);
   }
   if (lane == 0) found[wave] = earlier ? ~0u : n;
   __syncthreads();
-  uint32_t upto[4];
+  uint32_t to = 0;
   n = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < 4; ++w) {
+  for (uint32_t w = 0; w < W; ++w) {
     const uint32_t of = __builtin_amdgcn_readfirstlane(found[w]);
     if (of == ~0u) return;
-    upto[w] = n += of;
+    if (w == wave) to = n;
+    n += of;
   }
-  const auto token_at = [&](uint32_t i) -> uint64_t {
-    const uint32_t w = (i >= upto[0]) + (i >= upto[1]) + (i >= upto[2]);
-    return __builtin_amdgcn_readfirstlane((uint32_t)list[w][w ? i - upto[w - 1] : i]);
-  };
-  const uint32_t share = n <= 16 ? 16 : (n + 3) / 4, first = min(n, wave * share), last = min(n, first + share);
+#pragma unroll
+  for (uint32_t j = 0; j < kPart / 64; ++j) {
+    const uint64_t mask = __ballot(hit[j]);
+    if (hit[j]) list[to + __popcll(mask & ((1ull << lane) - 1))] = (uint16_t)(wave * kPart + j * 64 + lane);
+    to += __popcll(mask);
+  }
+  __syncthreads();
+  const uint32_t share = n <= 16 ? 16 : (n + W - 1) / W, first = min(n, wave * share), last = min(n, first + share);
   const Columns k = columns_of(blockIdx.x - token * slices, lane, cols);
   float sum[8] = {};
-  for (uint32_t i = first; i < last; i += 8) {
-    float v[8][8];
+  const auto row_at = [&](uint32_t i) {
+    return g + (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)list[min(i, last - 1)]) * stride;
+  };
+  const auto add = [&](uint32_t i, auto size) {  // `size` tokens from i on, all on their way before the first is used
+    constexpr uint32_t N = decltype(size)::value;
+    typename Pack<T>::type v[N];
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (i + j < last) load8(g + token_at(i + j) * stride, k, cols, v[j]);
+    for (uint32_t j = 0; j < N; ++j) v[j] = *(const typename Pack<T>::type*)(row_at(i + j) + k.c);
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j)
-      if (i + j < last)
+    for (uint32_t j = 0; j < N; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += v[j][e];
+      for (int e = 0; e < 8; ++e) sum[e] = i + j < last ? sum[e] + (float)v[j][e] : sum[e];
+    return i + N;
+  };
+  for (uint32_t i = first; i < last && !k.whole; ++i) {  // narrower than a load
+    float v[8];
+    load8(row_at(i), k, cols, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += v[e];
+  }
+  for (uint32_t i = first; i < last && k.whole;) {
+    if (last - i > 4)
+      i = add(i, std::integral_constant<uint32_t, 16>());
+    else if (last - i > 1)
+      i = add(i, std::integral_constant<uint32_t, 4>());
+    else
+      i = add(i, std::integral_constant<uint32_t, 1>());
   }
   if (n > 16) {
     if (wave)
@@ -376,7 +409,7 @@ __global__ __launch_bounds__(256) void nz_embedding_few_kernel(const long long* 
     __syncthreads();
     if (wave == 0)
 #pragma unroll
-      for (uint32_t w = 0; w < 3; ++w)
+      for (uint32_t w = 0; w < W - 1; ++w)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += sums[w][lane][e];
   }
@@ -392,8 +425,8 @@ uint32_t window_of(uint64_t count) {
 }
 
 // Whether tokens are few enough to be compared with each other for each 512 columns; what that reads is 8 count^2
-// slices bytes.  (30000x512, bf16, against sorting: 300 tokens 13 and 19 us, 2048 19.4 and 19.4; 8000x256, 1000 tokens
-// 10 and 17, 2048 15 and 18, 3000 22 and 19; with 2048 tokens in eight slices the sums alone take 34 and 16.)
+// slices bytes.  (On the device, bf16, against sorting: 30000x512, 1440 tokens 12 and 19 us, 2048 13 and 20, 4096 21 and
+// 21; 8000x256, 2048 9 and 17; where half of 2048 tokens are the same 26 and 22; 32000x4096, 1440 73 and 50.)
 bool unsorted(uint64_t count, uint64_t cols) {
   return count <= kFew && count * count * nz_ceil_div(cols, 512) <= (uint64_t)kFew * kFew;
 }
@@ -482,7 +515,7 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
     const T* g = (const T*)dev_g;
     T* out = (T*)dev_out;
     if (few) {
-      nz_embedding_few_kernel<T><<<(uint32_t)(count * slices), 256, 0, st>>>(
+      nz_embedding_few_kernel<T><<<(uint32_t)(count * slices), 64 * kFewWaves, 0, st>>>(
           (const long long*)dev_indices, (uint32_t)count, (uint32_t)rows, padding_idx, g, stride, (uint32_t)cols,
           (uint32_t)slices, scale, flags, out);
       return;
