@@ -545,15 +545,31 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
   if constexpr (QUANTIZE) {
     // rows of groups * 528 bytes: 512 values and their scales per group
     const T* xt = (const T*)x;
-    for (uint32_t i = wave; i < m * groups; i += 8) {
-      const uint32_t to = i / groups, group = i - to * groups, at = group * kGroup + lane * 8;
-      float v[8];
-      load8_upto(xt + to * stride + at, at < k ? k - at : 0, v);
-      const uint32_t s = block_scale<8>(v);
-      uint8_t* q = few_lds + i * 528u;
-      *(uint2*)(q + lane * 8) = codes8(v, up_factor(s));
-      if ((lane & 3) == 0) q[512 + scale_at(lane / 4)] = (uint8_t)s;
-    }
+    const auto quantise = [&](uint32_t i, auto size) {  // every eighth from i on, all on their way at once
+      constexpr uint32_t N = decltype(size)::value;
+      typename Pack<T>::type raw[N];
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        const uint32_t to = (i + 8 * j) / groups, at = (i + 8 * j - to * groups) * kGroup + lane * 8;
+        raw[j] = {};
+        if (at + 8 <= k) raw[j] = *(const typename Pack<T>::type*)(xt + to * stride + at);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < N; ++j) {
+        const uint32_t to = (i + 8 * j) / groups, at = (i + 8 * j - to * groups) * kGroup + lane * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)raw[j][e];
+        if (at < k && at + 8 > k) load8_upto(xt + to * stride + at, k - at, v);
+        const uint32_t s = block_scale<8>(v);
+        uint8_t* q = few_lds + (i + 8 * j) * 528u;
+        *(uint2*)(q + lane * 8) = codes8(v, up_factor(s));
+        if ((lane & 3) == 0) q[512 + scale_at(lane / 4)] = (uint8_t)s;
+      }
+    };
+    uint32_t i = wave;
+    for (; i + 24 < m * groups; i += 32) quantise(i, std::integral_constant<uint32_t, 4>());
+    for (; i < m * groups; i += 8) quantise(i, std::integral_constant<uint32_t, 1>());
     __syncthreads();
     xp = few_lds + row * groups * 528u + xg;
     xsp = few_lds + row * groups * 528u + 512 + g * 4;
@@ -866,24 +882,36 @@ bool cols_ok(uint64_t cols) { return cols <= 0x40000000ull; }
 // Sums over rows, the gradient of a bias: 512 columns a workgroup, every fourth of its rows a wavefront, eight of them
 // on their way at a time; the wavefronts' sums are added in their order.  Many rows are cut into parts, whose sums are
 // summed by the same kernel: no atomics, so the order of additions is that of the sizes, and nothing has to be cleared.
-// 8192 x 4096 bf16 values take 17 us, 3.9 TB/s.
+// 8192 x 4096 bf16 values take 18 us, 3.7 TB/s; 8192 x 1021 12.6.
 template <class T, class R>
 __global__ __launch_bounds__(256) void nz_mx_column_sums_kernel(const T* x, uint64_t stride, uint32_t m, uint32_t n,
                                                                 uint32_t rows, R* out) {
   constexpr uint32_t kRows = 8;
   __shared__ float sums[3][64][9];  // a ninth: lanes apart in their banks
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const uint32_t c = blockIdx.x * 512 + lane * 8, mine = c < n ? min(8u, n - c) : 0;
+  // the last columns of a width that is no multiple of 8 are loaded with some before them
+  const uint32_t own = blockIdx.x * 512 + lane * 8, mine = own < n ? min(8u, n - own) : 0;
+  const uint32_t c = n < 8 ? 0 : min(own, n - 8);
   const uint32_t first = blockIdx.y * rows, last = min(m, first + rows);
   float sum[8] = {};
-  for (uint32_t row = first + wave; row < last; row += 4 * kRows) {
-    float v[kRows][8];
+  if (n >= 8) {
+    for (uint32_t row = first + wave; row < last; row += 4 * kRows) {
+      typename Pack<T>::type v[kRows];
 #pragma unroll
-    for (uint32_t j = 0; j < kRows; ++j) load8_upto(x + min(row + 4 * j, last - 1) * stride + c, mine, v[j]);
+      for (uint32_t j = 0; j < kRows; ++j)
+        v[j] = *(const typename Pack<T>::type*)(x + min(row + 4 * j, last - 1) * stride + c);
 #pragma unroll
-    for (uint32_t j = 0; j < kRows; ++j)
+      for (uint32_t j = 0; j < kRows; ++j)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] = row + 4 * j < last ? sum[e] + v[j][e] : sum[e];
+        for (int e = 0; e < 8; ++e) sum[e] = row + 4 * j < last ? sum[e] + (float)v[j][e] : sum[e];
+    }
+  } else {
+    for (uint32_t row = first + wave; row < last; row += 4) {
+      float v[8];
+      load8_upto(x + row * stride, n, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
   }
   if (wave)
 #pragma unroll
@@ -894,7 +922,14 @@ __global__ __launch_bounds__(256) void nz_mx_column_sums_kernel(const T* x, uint
   for (int w = 0; w < 3; ++w)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] += sums[w][lane][e];
-  store8_upto(out + (uint64_t)blockIdx.y * n + c, mine, sum);
+  R* to = out + (uint64_t)blockIdx.y * n;
+  if (mine == 8) {
+    store8_upto(to + own, 8, sum);
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e)
+      if (c + e >= own && c + e < own + mine) to[c + e] = (R)sum[e];
+  }
 }
 
 bool aligned(const void* p, uint64_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -1079,6 +1114,7 @@ int launch_tiles16(const Cut& c, const void* a, uint64_t a_stride, uint64_t m, c
 //    2 rows of 12421x14421, 58 groups   22.3 27.7 25.5      8 rows of 50257x4096, 64 groups   30.6 44   23.4
 //    8 of 9505x3706, 64                 11.1 12.7  9.8      4 of 128256x1024, 8               15.0 24   22.7
 //    6 of 1735x7471, 90                  9.9  9.1 12.7     16 of 9498x3995, 128                  - 17.7 10.2
+// (quantising inside has become faster by up to 1 us since, by loads of four groups on their way at once).
 // Results in float32, whose tiles are slower, are better off there always: 16 rows of 12886x8431 31 against 50 us.
 bool few_inside(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   const uint64_t groups = m * nz_ceil_div(k, kGroup);
@@ -1123,7 +1159,7 @@ void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, cons
 }
 
 // Parts that the rows of a column sum are cut into: workgroups for the whole device, each with 32 rows at least; one
-// where few rows do not pay for a second launch (64 x 4096: 5.7 and 9.9 us).
+// where few rows do not pay for a second launch (64 x 4096: 2.8 us).
 uint32_t sum_parts(uint64_t m, uint64_t n) {
   if (m <= 128) return 1;
   const uint64_t slices = nz_ceil_div(n, 512);
