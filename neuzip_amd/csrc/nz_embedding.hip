@@ -4,9 +4,9 @@
 // while some of its workgroups sort the tokens (clearing is bound by memory, sorting by arithmetic and latency); the
 // others add up the rows of g.  The launches:
 //
-//   sort   32 tokens a workgroup; a token's place among the up to 8192 of its tile is the number of smaller keys (index, then
-//          position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups, and
-//          the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
+//   sort   32 tokens a workgroup; a token's place among the up to 8192 of its tile is the number of smaller keys
+//          (index, then position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups,
+//          and the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
 //   merge  (more than one tile) 8 or 16 sorted runs become one: the same count in the other runs, by bisection.
 //   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
 //          lie in one window is done; what reaches beyond it is kept as a piece.
@@ -14,8 +14,9 @@
 //
 // Few tokens are not sorted but compared with each other where they are added up.
 //
-// 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11.4 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
-// 8 + 22 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the sums, 10 to join.
+// 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
+// 8 + 22 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the
+// sums, 10 to join.
 #include <type_traits>
 #include <utility>
 
@@ -425,8 +426,8 @@ uint32_t window_of(uint64_t count) {
 }
 
 // Whether tokens are few enough to be compared with each other for each 512 columns; what that reads is 8 count^2
-// slices bytes.  (On the device, bf16, against sorting: 30000x512, 1440 tokens 12 and 19 us, 2048 13 and 20, 4096 21 and
-// 21; 8000x256, 2048 9 and 17; where half of 2048 tokens are the same 26 and 22; 32000x4096, 1440 73 and 50.)
+// slices bytes.  (On the device, bf16, against sorting: 30000x512, 1440 tokens 12 and 19 us, 2048 13 and 20, 4096 21
+// and 21; 8000x256, 2048 9 and 17; where half of 2048 tokens are the same 26 and 22; 32000x4096, 1440 73 and 50.)
 bool unsorted(uint64_t count, uint64_t cols) {
   return count <= kFew && count * count * nz_ceil_div(cols, 512) <= (uint64_t)kFew * kFew;
 }

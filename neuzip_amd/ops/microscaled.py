@@ -182,7 +182,8 @@ def mx_quantize(x: torch.Tensor, bits: int = 4) -> MXTensor:
     sizes = _row_sizes(cols, bits)
     data = x.new_empty((n, sizes[0]), dtype=torch.uint8)
     scales = x.new_empty((n, sizes[1]), dtype=torch.uint8)
-    _call(_lib.load().nz_mx_quantize, index, rows.data_ptr(), code, n, cols, stride, bits, data.data_ptr(), scales.data_ptr())
+    _call(_lib.load().nz_mx_quantize, index, rows.data_ptr(), code, n, cols, stride, bits, data.data_ptr(),
+          scales.data_ptr())
     return MXTensor._of(data, scales, shape, bits)
 
 
