@@ -464,7 +464,13 @@ int nz_mx_lookup(const void* dev_data, const void* dev_scales, uint64_t rows, ui
                  void* stream);
 
 /* y[m][n] = sum_k x[m][k] w[n][k] + bias[n]: w holds n rows of k values in 4 bits, the m rows of x are brought to 8
-   bits on the way.  Sums in 32 bits, one rounding to dtype.  bias may be NULL; it, x and y have the same dtype.
+   bits on the way.  bias may be NULL; it, x and y have the same dtype, to which the sum is rounded once.
+   How it is added: NZ_DTYPE_F32 in 32 bits.  The 16-bit types by the scaled matrix instruction, eight values of k at
+   a time (8 j to 8 j + 7): with E the largest of the eight products' exponents (the sum of the two elements' and
+   their blocks'; a subnormal element has its type's smallest), each product is cut toward zero to a multiple of
+   2^(E - 13), so what is lost is below 2^-12 of the largest of the eight.  These sums, the accumulators and the bias
+   are added in 32 bits.  Where large products cancel and the small ones beside them count, nz_mx_linear_rows8 with
+   NZ_DTYPE_F32 keeps them.
    k is 1 to 2^22, n at most 2^21, m at most 2^24.
    The workspace (nz_mx_linear_workspace_bytes bytes, 16-byte aligned, none if that is 0) is free again when the
    call's work has ended. */
