@@ -18,6 +18,7 @@ import math
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from neuzip_amd import _lib
@@ -36,10 +37,25 @@ def _dtype_code(dtype: torch.dtype) -> int:
 # address and the current device are asked for directly, 2 us less a call than through torch.cuda.)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_tracing = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _refuse_unseen(tensors) -> None:
+    """Raise where a native call would be passed by in silence: a trace (of torch.jit or make_fx) would hold the
+    allocation of the result only, and a tangent would end here."""
+    if _tracing() is not None or _modes() and torch._C._get_dispatch_mode(_PROXY) is not None:
+        raise RuntimeError("this call cannot be traced: it writes its result through an address")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("forward-mode differentiation is not supported by this call")
 
 
 def _on_gpu(**tensors) -> int:
     """The index of the device that all of ``tensors`` (None aside) are on, which has to be a GPU."""
+    _refuse_unseen(tensors.values())
     index = None
     for name, t in tensors.items():
         if t is None:
