@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from neuzip_amd import _lib
 from neuzip_amd.ops.microscaled import _as_rows, _call, _dtype_code, _on_gpu, _table_room, _workspace
@@ -20,7 +21,8 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     ``padding_idx`` and indices outside the table take no part;
     ``scale_grad_by_freq`` divides a row's gradient by the number of its tokens.
     With ``out`` the gradient is added to that tensor (contiguous, of the type of
-    ``grad``), which reads and writes the rows of the tokens only."""
+    ``grad``), which reads and writes the rows of the tokens only; autograd takes that for
+    a change in place, but records neither it nor the gradient itself."""
     if indices.dtype not in (torch.int64, torch.int32):
         raise ValueError("indices must be int64 or int32")
     if grad.dim() < 1 or grad.shape[:-1] != indices.shape:
@@ -50,6 +52,8 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     ws, at = _workspace(room, g)
     _call(L.nz_embedding_gradient, index, idx.data_ptr(), count, g.data_ptr(), code, stride, num_embeddings, cols,
           float(scale), -1 if padding_idx is None else padding_idx, flags, out.data_ptr(), at, room)
+    if flags & _lib.GRAD_ACCUMULATE:
+        increment_version(out)
     return out
 
 

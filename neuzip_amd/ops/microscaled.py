@@ -20,6 +20,7 @@ from functools import lru_cache
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from neuzip_amd import _lib
 
@@ -273,6 +274,8 @@ class MicroscaledLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, dtype):
         ctx.weight = weight
+        if ctx.needs_input_grad[0] and not weight.data.is_inference():  # an inference tensor has no version to check
+            ctx.save_for_backward(weight.data, weight.scales)
         return _product(x, weight, bias, dtype)
 
     @staticmethod
@@ -280,7 +283,10 @@ class MicroscaledLinear(torch.autograd.Function):
     def backward(ctx, grad_output):
         grad_x = grad_b = None
         if ctx.needs_input_grad[0]:
-            grad_x = _input_gradient(grad_output, ctx.weight)
+            weight, held = ctx.weight, ctx.saved_tensors  # raises if the weight has been written to since
+            if held:
+                weight = MXTensor(*held, weight.shape, weight.bits)
+            grad_x = _input_gradient(grad_output, weight)
         if ctx.needs_input_grad[2]:
             grad_b = _bias_gradient(grad_output, ctx.weight.shape[0])
         return grad_x, None, grad_b, None
@@ -328,7 +334,8 @@ def mx_embedding(indices: torch.Tensor, table: MXTensor, scale: float = 1.0, dty
                  status=None) -> torch.Tensor:
     """Rows ``indices`` (any integer shape) of a table in microscaled form, times
     ``scale`` in 32 bits, rounded to ``dtype``.  An index outside the table gives a row
-    of zeros and sets bit 0 of ``status`` (an int32 tensor of one element)."""
+    of zeros and sets bit 0 of ``status`` (an int32 tensor of one element).  The table is
+    frozen: autograd has nothing to record."""
     if not isinstance(table, MXTensor) or len(table.shape) != 2:
         raise ValueError("table must be a matrix in microscaled form (mx_quantize)")
     if indices.dtype not in (torch.int64, torch.int32):
@@ -347,4 +354,6 @@ def mx_embedding(indices: torch.Tensor, table: MXTensor, scale: float = 1.0, dty
     out = data.new_empty((*indices.shape, cols), dtype=dtype)
     _call(_lib.load().nz_mx_lookup, index, data.data_ptr(), table.scales.data_ptr(), rows, cols, table.bits,
           idx.data_ptr(), idx.numel(), float(scale), out.data_ptr(), code, at)
+    if status is not None:
+        increment_version(status)
     return out
