@@ -449,7 +449,8 @@ int nz_manager_check(nz_manager* m, void* stream);
 uint64_t nz_mx_row_bytes(uint64_t cols, int bits);
 uint64_t nz_mx_scale_bytes(uint64_t cols);
 
-/* rows x cols values at dev_x, `stride` elements from row to row. */
+/* rows x cols values at dev_x, `stride` elements from row to row.  cols is up to 2^30, rows * ceil(cols / 512) up to
+   2^33, here and below. */
 int nz_mx_quantize(const void* dev_x, int dtype, uint64_t rows, uint64_t cols, uint64_t stride, int bits,
                    void* dev_data, void* dev_scales, void* stream);
 
@@ -503,7 +504,8 @@ int nz_column_sums(const void* dev_x, int dtype, uint64_t m, uint64_t n, uint64_
    rounded once: the same bits every time.  g has `stride` elements from row to row, out is contiguous.  The row
    padding_idx (-1: none) and indices outside the table take no part.  NZ_GRAD_BY_FREQUENCY divides each row by the
    number of its t; NZ_GRAD_ACCUMULATE adds to out (rounded once) instead of setting it, rows without a t are then left as they are.
-   count is up to 2^28, rows below 2^31, cols up to 2^24.  The workspace is as above. */
+   count is up to 2^28 - 32, rows below 2^31, cols up to 2^24, and ceil(count / w) * ceil(cols / 512) below 2^24 with
+   w = 64 (16 up to 16384 indices, 32 up to 32768).  The workspace is as above. */
 #define NZ_GRAD_BY_FREQUENCY 1u
 #define NZ_GRAD_ACCUMULATE 2u
 uint64_t nz_embedding_gradient_workspace_bytes(uint64_t count, uint64_t cols);

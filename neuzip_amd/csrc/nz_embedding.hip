@@ -17,6 +17,7 @@
 // 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
 // 8 + 22 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the
 // sums, 10 to join.
+#include <algorithm>
 #include <type_traits>
 #include <utility>
 
@@ -465,7 +466,9 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
   if (flags & ~(NZ_GRAD_BY_FREQUENCY | NZ_GRAD_ACCUMULATE)) return nz_fail(NZ_ERR_ARG, "unknown flags");
   if (rows == 0 || cols == 0) return NZ_OK;
   const uint64_t slices = nz_ceil_div(cols, 512);
-  if (cols > 1u << 24 || rows > 0x7FFFFFFFull || count > 1u << 28 || count * slices > 1ull << 32)
+  // of the last two launches, which are counted in pieces of windows, and of the sort
+  if (cols > 1u << 24 || rows > 0x7FFFFFFFull || count > nz_most_groups(512) * kSorted ||
+      (!unsorted(count, cols) && nz_ceil_div(count, window_of(count)) * slices > nz_most_groups(64 * kJoin)))
     return nz_fail(NZ_ERR_ARG, "too many rows, columns or indices");
   if (!dev_out || (count && (!dev_indices || !dev_g))) return nz_fail(NZ_ERR_ARG, "null indices, gradient or output");
   if ((uintptr_t)dev_indices % 8 || (uintptr_t)dev_g % size || (uintptr_t)dev_out % size)
@@ -475,20 +478,25 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
     if (workspace_bytes < room.bytes) return nz_fail(NZ_ERR_CAPACITY, "workspace too small");
     if (!dev_workspace || (uintptr_t)dev_workspace % 16) return nz_fail(NZ_ERR_ALIGN, "misaligned workspace");
   }
-  const uint64_t bytes = flags & NZ_GRAD_ACCUMULATE ? 0 : rows * cols * size, clearers = nz_ceil_div(bytes, kClear);
+  const uint64_t bytes = flags & NZ_GRAD_ACCUMULATE ? 0 : rows * cols * size;
   const bool few = unsorted(count, cols);
   const uint32_t sorters = few ? 0 : (uint32_t)nz_ceil_div(count, kSorted);
-  if (clearers + sorters > 0x7FFFFFFFull) return nz_fail(NZ_ERR_ARG, "table too large for one launch");
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)dev_workspace;
   Place *places = (Place*)ws, *other = (Place*)(ws + room.again);
-  const dim3 grid((uint32_t)clearers + sorters);
   const uint32_t tile = tile_of(count);
   const auto sort = [&](auto key, auto size) {
     constexpr uint32_t TILE = decltype(size)::value;
-    nz_embedding_sort_kernel<decltype(key), TILE><<<grid, 512, 0, st>>>((const long long*)dev_indices, (uint32_t)count,
-                                                                        (uint32_t)rows, padding_idx, places, sorters,
-                                                                        (uint8_t*)dev_out, bytes);
+    // the sort and what a launch holds of the clearing besides; the rest of tables beyond 137 GB in further launches
+    uint64_t done = 0;
+    for (uint32_t sorting = sorters; sorting || done < bytes; sorting = 0) {
+      const uint64_t clearers = std::min(nz_ceil_div(bytes - done, kClear), nz_most_groups(512) - sorting);
+      const uint64_t now = std::min(bytes - done, clearers * kClear);
+      nz_embedding_sort_kernel<decltype(key), TILE><<<(uint32_t)clearers + sorting, 512, 0, st>>>(
+          (const long long*)dev_indices, (uint32_t)count, (uint32_t)rows, padding_idx, places, sorting,
+          (uint8_t*)dev_out + done, now);
+      done += now;
+    }
   };
   const auto sort_by = [&](auto key) {
     if (tile == kTile)
@@ -496,9 +504,7 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
     else
       sort(key, std::integral_constant<uint32_t, kTile / 4>());
   };
-  if (grid.x == 0) {
-    // few tokens added to a table: nothing to clear or to sort
-  } else if (rows < 1u << (32 - kTileBits)) {
+  if (rows < 1u << (32 - kTileBits)) {
     sort_by(uint32_t());
   } else {
     sort_by(uint64_t());

@@ -962,8 +962,9 @@ int check_bits(int bits) {
   return bits == 4 || bits == 8 ? NZ_OK : nz_fail(NZ_ERR_ARG, "bits must be 4 or 8");
 }
 
-int check_grid(uint64_t blocks) {
-  return blocks <= 0x7FFFFFFFull ? NZ_OK : nz_fail(NZ_ERR_ARG, "too many rows for one launch");
+// groups of 512 values in all rows, beyond any memory
+int check_groups(uint64_t rows, uint64_t groups) {
+  return nz_mul(rows, groups) <= 1ull << 33 ? NZ_OK : nz_fail(NZ_ERR_ARG, "too many rows");
 }
 
 template <class F>
@@ -979,17 +980,21 @@ void by_dtype(int dtype, F f) {
 int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint64_t stride, int bits, void* data,
                     void* scales, hipStream_t st) {
   const uint32_t groups = (cols + kGroup - 1) / kGroup;
-  const uint64_t waves = nz_mul(rows, groups);
-  if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
-  const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
-  by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (bits == 4)
-      nz_mx_quantize_kernel<4, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups,
-                                                        (uint8_t*)data, (uint8_t*)scales);
-    else
-      nz_mx_quantize_kernel<8, T><<<grid, 256, 0, st>>>((const T*)x, stride, cols, waves, groups,
-                                                        (uint8_t*)data, (uint8_t*)scales);
+  if (int rc = check_groups(rows, groups)) return rc;
+  const uint64_t row_bytes = nz_mx_row_bytes(cols, bits);
+  nz_in_pieces(rows, groups * 64ull, [&](uint64_t first, uint64_t count) {
+    const uint64_t waves = count * groups;
+    const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
+    uint8_t* d = (uint8_t*)data + first * row_bytes;
+    uint8_t* s = (uint8_t*)scales + first * groups * 16;
+    by_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      const T* from = (const T*)x + first * stride;
+      if (bits == 4)
+        nz_mx_quantize_kernel<4, T><<<grid, 256, 0, st>>>(from, stride, cols, waves, groups, d, s);
+      else
+        nz_mx_quantize_kernel<8, T><<<grid, 256, 0, st>>>(from, stride, cols, waves, groups, d, s);
+    });
   });
   return nz_launched();
 }
@@ -997,19 +1002,26 @@ int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint
 int launch_values(const void* data, const void* scales, uint64_t rows, uint64_t cols, int bits, const void* index,
                   uint64_t count, float scale, void* out, int dtype, void* status, hipStream_t st) {
   const uint32_t groups = (uint32_t)nz_ceil_div(cols, kGroup);
-  const uint64_t waves = nz_mul(count, groups);
-  if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
-  const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
-  by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (bits == 4)
-      nz_mx_values_kernel<4, T><<<grid, 256, 0, st>>>((const uint8_t*)data, (const uint8_t*)scales, rows,
-                                                      (uint32_t)cols, (const long long*)index, waves, groups,
-                                                      scale, (T*)out, (uint32_t*)status);
-    else
-      nz_mx_values_kernel<8, T><<<grid, 256, 0, st>>>((const uint8_t*)data, (const uint8_t*)scales, rows,
-                                                      (uint32_t)cols, (const long long*)index, waves, groups,
-                                                      scale, (T*)out, (uint32_t*)status);
+  if (int rc = check_groups(count, groups)) return rc;
+  const uint64_t row_bytes = nz_mx_row_bytes(cols, bits);
+  nz_in_pieces(count, groups * 64ull, [&](uint64_t first, uint64_t piece) {
+    const uint64_t waves = piece * groups;
+    const dim3 grid((uint32_t)nz_ceil_div(waves, 4));
+    // rows that no index names begin at the piece's first
+    const uint64_t skip = index ? 0 : first;
+    const uint8_t* d = (const uint8_t*)data + skip * row_bytes;
+    const uint8_t* s = (const uint8_t*)scales + skip * groups * 16;
+    const long long* ids = index ? (const long long*)index + first : nullptr;
+    by_dtype(dtype, [&](auto t) {
+      using T = decltype(t);
+      T* to = (T*)out + first * cols;
+      if (bits == 4)
+        nz_mx_values_kernel<4, T><<<grid, 256, 0, st>>>(d, s, rows - skip, (uint32_t)cols, ids, waves, groups, scale,
+                                                        to, (uint32_t*)status);
+      else
+        nz_mx_values_kernel<8, T><<<grid, 256, 0, st>>>(d, s, rows - skip, (uint32_t)cols, ids, waves, groups, scale,
+                                                        to, (uint32_t*)status);
+    });
   });
   return nz_launched();
 }
@@ -1237,9 +1249,13 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const void* wd, c
 int check_product(uint64_t m, uint64_t n, uint64_t k, const void* wd, const void* ws) {
   if (k == 0 || k > 1ull << 22 || n > 1ull << 21)
     return nz_fail(NZ_ERR_ARG, "a weight must have 1 to 2^22 columns and up to 2^21 rows");
-  if (m > 1ull << 24 || nz_ceil_div(m, 64) * nz_ceil_div(n > k ? n : k, 64) > 0x7FFFFFFFull)
-    return nz_fail(NZ_ERR_ARG, "too many rows for one launch");
+  if (m > 1ull << 24) return nz_fail(NZ_ERR_ARG, "too many rows");
   return check_mx(wd, ws);
+}
+
+// Tiles of the largest products are counted by the grid: workgroups have up to 512 threads.
+int check_cut(const Cut& c) {
+  return (uint64_t)c.mt * c.nt <= nz_most_groups(512) ? NZ_OK : nz_fail(NZ_ERR_ARG, "too many rows for one launch");
 }
 
 int check_workspace(const void* workspace, uint64_t bytes, uint64_t need) {
@@ -1315,6 +1331,7 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
   if (int rc = check_product(m, n, k, dev_w_data, dev_w_scales)) return rc;
   if (!dev_x || !dev_y) return nz_fail(NZ_ERR_ARG, "null rows or output");
   const Room room = product_room(m, n, k, dtype);
+  if (int rc = check_cut(room.cut)) return rc;
   if (int rc = check_workspace(dev_workspace, workspace_bytes, room.bytes)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   if (few_inside(m, n, k, dtype)) {
@@ -1327,10 +1344,12 @@ int nz_mx_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t 
   }
   uint8_t* base = (uint8_t*)dev_workspace;
   if (dtype == NZ_DTYPE_F32 && !few_rows(m, n, k, dtype)) {
-    const uint64_t groups = nz_ceil_div(k, kGroup), waves = nz_mul(m, groups);
-    if (int rc = check_grid(nz_ceil_div(waves, 4))) return rc;
-    nz_mx_rounded_kernel<<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
-        (const float*)dev_x, stride, (uint32_t)k, waves, (uint32_t)groups, (nz_bf16*)(base + room.values));
+    const uint64_t groups = nz_ceil_div(k, kGroup);
+    nz_in_pieces(m, groups * 64, [&](uint64_t first, uint64_t count) {
+      nz_mx_rounded_kernel<<<(uint32_t)nz_ceil_div(count * groups, 4), 256, 0, st>>>(
+          (const float*)dev_x + first * stride, stride, (uint32_t)k, count * groups, (uint32_t)groups,
+          (nz_bf16*)(base + room.values) + first * filled(k));
+    });
     return launch_wide(m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, room, base, st);
   }
   if (int rc = launch_quantize(dev_x, dtype, m, (uint32_t)k, stride, 8, base + room.xd, base + room.xs, st)) return rc;
@@ -1347,6 +1366,7 @@ int nz_mx_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_
   if (int rc = check_mx(dev_x_data, dev_x_scales)) return rc;
   if (!dev_y) return nz_fail(NZ_ERR_ARG, "null output");
   const Room room = product_room(m, n, k, dtype);
+  if (int rc = check_cut(room.cut)) return rc;
   if (int rc = check_workspace(dev_workspace, workspace_bytes, room.bytes)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   return launch_product(dev_x_data, dev_x_scales, m, dev_w_data, dev_w_scales, n, (uint32_t)k, dev_bias, dev_y, dtype,
@@ -1372,16 +1392,18 @@ int nz_mx_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint
   const Planes p = planes_of(dev_g, dtype, m, n, stride);
   const uint64_t steps = p.padded / 64;
   const Cut cut = cut_product16(m, k, steps * p.count);
+  if (int rc = check_cut(cut)) return rc;
   if (int rc = check_workspace(dev_workspace, workspace_bytes, p.bytes + cut.part_bytes(m, k))) return rc;
   const void* a = dev_g;
   uint64_t a_stride = stride;
   if (p.bytes) {
     a = dev_workspace, a_stride = p.padded * p.count;
-    const uint64_t blocks = nz_ceil_div(m * (p.padded / 8), 256);
-    if (int rc = check_grid(blocks)) return rc;
 #define NZ_PLANES(P, T)                                                                                           \
-  nz_mx_planes_kernel<P, T><<<(uint32_t)blocks, 256, 0, st>>>((const T*)dev_g, stride, m, (uint32_t)n,            \
-                                                              (uint32_t)p.padded, (nz_bf16*)dev_workspace)
+  nz_in_pieces(m, p.padded / 8, [&](uint64_t first, uint64_t count) {                                             \
+    nz_mx_planes_kernel<P, T><<<(uint32_t)nz_ceil_div(count * (p.padded / 8), 256), 256, 0, st>>>(                \
+        (const T*)dev_g + first * stride, stride, count, (uint32_t)n, (uint32_t)p.padded,                         \
+        (nz_bf16*)dev_workspace + first * a_stride);                                                              \
+  })
     if (dtype == NZ_DTYPE_BF16)
       NZ_PLANES(1, nz_bf16);
     else if (dtype == NZ_DTYPE_F16)

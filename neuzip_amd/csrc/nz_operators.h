@@ -31,5 +31,17 @@ inline uint64_t nz_mul(uint64_t a, uint64_t b) {
   return __builtin_mul_overflow(a, b, &r) ? ~0ull : r;
 }
 
+// Workgroups of `threads` threads that one launch may have along an axis: its threads are counted in 32 bits.  (Beyond
+// that a launch is no error here, it leaves workgroups out.)
+inline uint64_t nz_most_groups(uint32_t threads) { return 0xFFFFFFFFull / threads; }
+
+// f(first, count) for pieces of `rows` rows, each as many as a launch of workgroups of 256 threads takes with `threads`
+// threads to a row: one piece, but for tens of millions of rows.
+template <class F>
+inline void nz_in_pieces(uint64_t rows, uint64_t threads, F f) {
+  const uint64_t most = nz_most_groups(256) * 256 / threads;
+  for (uint64_t first = 0; first < rows; first += most) f(first, rows - first < most ? rows - first : most);
+}
+
 using nz_bf16 = __bf16;
 using nz_f16 = _Float16;
