@@ -81,17 +81,36 @@ def _convert(manager, module: torch.nn.Module, prefix: str = "") -> torch.nn.Mod
     return module
 
 
-def mx_convert(module: torch.nn.Module, prefix: str = "", _made=None) -> torch.nn.Module:
+def _heads(module: torch.nn.Module) -> set:
+    """The modules that stand in or below a child whose name contains ``lm_head``."""
+    heads, pending, seen = set(), [module], set()
+    while pending:
+        parent = pending.pop()
+        if parent in seen:
+            continue
+        seen.add(parent)
+        for name, child in parent._modules.items():  # every name: named_children gives a module once
+            if child is None:
+                continue
+            if "lm_head" in name:
+                heads.update(child.modules())
+            else:
+                pending.append(child)
+    return heads
+
+
+def mx_convert(module: torch.nn.Module, prefix: str = "", _made=None, _kept=None) -> torch.nn.Module:
     """In place: the ``nn.Linear`` layers that ``Manager.convert`` would compress
-    (those whose attribute name contains ``lm_head`` are left alone) are held in
-    microscaled 4 bits instead, with their weights frozen.  A layer that stands in
-    several places is converted once."""
+    (those whose attribute name contains ``lm_head`` are left alone, wherever else
+    they stand too) are held in microscaled 4 bits instead, with their weights
+    frozen.  A layer that stands in several places is converted once."""
     from neuzip_amd.nn import MXLinear
 
     made = {} if _made is None else _made
+    kept = _heads(module) if _kept is None else _kept
     for name, child in list(module._modules.items()):
         dotted = f"{prefix}.{name}" if prefix else name
-        if child is None or "lm_head" in name:
+        if child is None or child in kept:
             continue
         if isinstance(child, torch.nn.Linear):
             if child not in made:
@@ -100,5 +119,5 @@ def mx_convert(module: torch.nn.Module, prefix: str = "", _made=None) -> torch.n
                 _delete_module(child)
             setattr(module, name, made[child])
         else:
-            mx_convert(child, dotted, made)
+            mx_convert(child, dotted, made, kept)
     return module
