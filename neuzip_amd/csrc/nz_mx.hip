@@ -244,14 +244,13 @@ __device__ inline f4 step(i4v w, i4v x0, i4v x1, f4 acc, uint32_t sw, uint32_t s
 // 16 (4) bytes of every lane to LDS: lane l's to `to` (an LDS address, the same for all lanes) + 16 l (4 l), from
 // `from`, the same for all lanes, + `offset`.  In assembly because the compiler, where it knows of such loads, waits
 // for all of them in front of other reads of LDS, the next steps' loads among them.  It has no register to give to
-// anything else too early, the kernels count these loads themselves (wait_loads), and nothing else here uses m0.
+// anything else too early, and the kernels count these loads themselves (wait_loads).  The address goes in through m0
+// as an operand, so the compiler knows what is in that register; s_nop stands between its write and the load.
 __device__ inline void to_lds16(const uint8_t* from, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(from)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
 }
 __device__ inline void to_lds4(const uint8_t* from, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to), "v"(offset), "s"(from)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, %2" ::"{m0}"(to), "v"(offset), "s"(from) : "memory");
 }
 
 __device__ inline uint32_t lds_address(uint8_t* p) {
