@@ -94,7 +94,7 @@ def _as_rows(t: torch.Tensor, width: int):
     tensor, its rows, elements from row to row."""
     if t.is_contiguous():
         return t, t.numel() // width if width else math.prod(t.shape[:-1]), width
-    rows = t.reshape(-1, width)
+    rows = t.resolve_neg().reshape(-1, width)  # its memory may hold the values with the other sign
     if rows.stride(1) != 1 and width > 1:
         rows = rows.contiguous()
     return rows, rows.shape[0], rows.stride(0)

@@ -37,6 +37,16 @@ def test_forward_mode_differentiation_is_refused(call, t):
             call(t)  # without a tangent there is none to lose
 
 
+def test_rows_whose_sign_is_held_back():
+    """imag of a conjugate: its memory holds the values with the other sign"""
+    z = torch.arange(12.0).view(4, 3).to(torch.complex64) * 1j
+    for width in (3, 1):
+        t = z[:, :width].conj().imag
+        assert t.is_neg()
+        rows, n, stride = ops.microscaled._as_rows(t, width)
+        assert not rows.is_neg() and torch.equal(rows, t) and (n, stride) == (4, rows.stride(0))
+
+
 @pytest.mark.gpu
 def test_compiled_functions_make_the_calls():
     w = ops.mx_quantize(torch.randn(40, 64, device="cuda"), 4)
