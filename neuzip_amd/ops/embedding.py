@@ -40,7 +40,8 @@ def embedding_gradient(indices: torch.Tensor, grad: torch.Tensor, num_embeddings
     if out is None:
         out = grad.new_empty((num_embeddings, cols))
     else:
-        if tuple(out.shape) != (num_embeddings, cols) or out.dtype != grad.dtype or not out.is_contiguous():
+        if (tuple(out.shape) != (num_embeddings, cols) or out.dtype != grad.dtype or not out.is_contiguous()
+                or out.is_neg()):
             raise ValueError(f"out must be a contiguous {grad.dtype} tensor of shape {(num_embeddings, cols)}")
         flags |= _lib.GRAD_ACCUMULATE
     L = _lib.load()

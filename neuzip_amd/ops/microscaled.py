@@ -92,7 +92,7 @@ def _ask(fn, index: int, *args) -> int:
 def _as_rows(t: torch.Tensor, width: int):
     """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it): the
     tensor, its rows, elements from row to row."""
-    if t.is_contiguous():
+    if t.is_contiguous() and not t.is_neg():
         return t, t.numel() // width if width else math.prod(t.shape[:-1]), width
     rows = t.resolve_neg().reshape(-1, width)  # its memory may hold the values with the other sign
     if rows.stride(1) != 1 and width > 1:
@@ -223,7 +223,7 @@ def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
         return y.copy_(bias) if bias is not None else y.zero_()
     b = None
     if bias is not None:
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
         b = bias.data_ptr()
     if held:
         m = xt.shape[0]
