@@ -284,7 +284,7 @@ class MicroscaledLinear(torch.autograd.Function):
         grad_x = grad_b = None
         if ctx.needs_input_grad[0]:
             weight, held = ctx.weight, ctx.saved_tensors  # raises if the weight has been written to since
-            if held:
+            if held and (held[0] is not weight.data or held[1] is not weight.scales):  # a hook's
                 weight = MXTensor(*held, weight.shape, weight.bits)
             grad_x = _input_gradient(grad_output, weight)
         if ctx.needs_input_grad[2]:
