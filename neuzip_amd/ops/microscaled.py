@@ -46,17 +46,18 @@ _PROXY = torch._C._TorchDispatchModeKey.PROXY
 def _refuse_unseen(tensors) -> None:
     """Raise where a native call would be passed by in silence: a trace (of torch.jit or make_fx) would hold the
     allocation of the result only, and a tangent would end here."""
-    if _tracing() is not None or _modes() and torch._C._get_dispatch_mode(_PROXY) is not None:
+    if _tracing() is not None or torch._C._get_dispatch_mode(_PROXY) is not None:
         raise RuntimeError("this call cannot be traced: it writes its result through an address")
     if forward_ad._current_level >= 0:
-        for t in tensors:
+        for t in tensors.values():
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError("forward-mode differentiation is not supported by this call")
 
 
 def _on_gpu(**tensors) -> int:
     """The index of the device that all of ``tensors`` (None aside) are on, which has to be a GPU."""
-    _refuse_unseen(tensors.values())
+    if forward_ad._current_level >= 0 or _modes() or _tracing() is not None:
+        _refuse_unseen(tensors)
     index = None
     for name, t in tensors.items():
         if t is None:
@@ -92,8 +93,10 @@ def _ask(fn, index: int, *args) -> int:
 def _as_rows(t: torch.Tensor, width: int):
     """``t`` as rows of ``width`` elements that lie next to each other (a copy only where no view does it): the
     tensor, its rows, elements from row to row."""
-    if t.is_contiguous() and not t.is_neg():
-        return t, t.numel() // width if width else math.prod(t.shape[:-1]), width
+    if t.is_contiguous():
+        n = t.numel()
+        if n != 1 or not t.is_neg():
+            return t, n // width if width else math.prod(t.shape[:-1]), width
     rows = t.resolve_neg().reshape(-1, width)  # its memory may hold the values with the other sign
     if rows.stride(1) != 1 and width > 1:
         rows = rows.contiguous()
@@ -223,7 +226,9 @@ def _product(x, weight: MXTensor, bias, dtype: torch.dtype) -> torch.Tensor:
         return y.copy_(bias) if bias is not None else y.zero_()
     b = None
     if bias is not None:
-        bias = bias.resolve_neg().contiguous()
+        bias = bias.contiguous()
+        if n == 1:
+            bias = bias.resolve_neg()
         b = bias.data_ptr()
     if held:
         m = xt.shape[0]
