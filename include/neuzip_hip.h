@@ -503,7 +503,8 @@ int nz_column_sums(const void* dev_x, int dtype, uint64_t m, uint64_t n, uint64_
    out[v] = scale * sum of g[t] over the t with index v, in 32 bits in an order that the indices alone decide,
    rounded once: the same bits every time.  g has `stride` elements from row to row, out is contiguous.  The row
    padding_idx (-1: none) and indices outside the table take no part.  NZ_GRAD_BY_FREQUENCY divides each row by the
-   number of its t; NZ_GRAD_ACCUMULATE adds to out (rounded once) instead of setting it, rows without a t are then left as they are.
+   number of its t; NZ_GRAD_ACCUMULATE adds to out (rounded once) instead of setting it, rows without a t are then
+   left as they are.
    count is up to 2^28 - 32, rows below 2^31, cols up to 2^24, and ceil(count / w) * ceil(cols / 512) below 2^24 with
    w = 64 (16 up to 16384 indices, 32 up to 32768).  The workspace is as above. */
 #define NZ_GRAD_BY_FREQUENCY 1u

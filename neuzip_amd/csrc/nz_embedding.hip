@@ -5,8 +5,9 @@
 // others add up the rows of g.  The launches:
 //
 //   sort   32 tokens a workgroup; a token's place among the up to 8192 of its tile is the number of smaller keys
-//          (index, then position), counted by comparing with all of them from LDS: no passes, no exchange between workgroups,
-//          and the same place every time.  Four tokens a lane, so that reading the keys does not take the longest.
+//          (index, then position), counted by comparing with all of them from LDS: no passes, no exchange between
+//          workgroups, and the same place every time.  Four tokens a lane, so that reading the keys does not take the
+//          longest.
 //   merge  (more than one tile) 8 or 16 sorted runs become one: the same count in the other runs, by bisection.
 //   sum    one wavefront per 512 columns of a window of places, added in float32 in their order.  A row whose tokens
 //          lie in one window is done; what reaches beyond it is kept as a piece.
@@ -14,9 +15,9 @@
 //
 // Few tokens are not sorted but compared with each other where they are added up.
 //
-// 8192 tokens of a text in 50257x1024 (bf16): 15.5 + 11 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768: 19 +
-// 8 + 22 + 9.6; 2048 in 128256x4096: 165 + 11 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us for the
-// sums, 10 to join.
+// 8192 tokens of a text in 50257x1024 (bf16): 16.6 + 11 + 5 us, where clearing alone takes 15 (6.8 TB/s); 32768:
+// 19 + 8 + 22 + 9.6; 2048 in 128256x4096: 167 + 15 + 5 us, bound by clearing.  Windows of 8 places instead of 16: 9 us
+// for the sums, 10 to join.
 #include <algorithm>
 #include <type_traits>
 #include <utility>

@@ -310,8 +310,8 @@ def mx_linear(x, weight: MXTensor, bias=None, dtype=None) -> torch.Tensor:
     largest of the eight consecutive products that it is added with: usually far
     below its own rounding, but not where large products cancel.  A float32 result is
     summed in 32 bits throughout, from the same rows with
-    ``mx_linear(mx_quantize(x, 8), weight, dtype=torch.float32)`` (1.2 times the time
-    for a few rows, 2.4 times for thousands)."""
+    ``mx_linear(mx_quantize(x, 8), weight, dtype=torch.float32)`` (1.3 to 1.6 times the
+    time of a few such rows, 2.5 times that of many)."""
     _check_weight(weight)
     n, k = weight.shape
     if isinstance(x, MXTensor):
