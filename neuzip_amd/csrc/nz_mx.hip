@@ -650,7 +650,8 @@ __global__ __launch_bounds__(512) void nz_mx_few_kernel(const void* x, uint64_t 
 // side by side along the summed axis.
 
 // Rows cut into P bf16 planes, [m][P][padded]: each plane takes the 8 leading bits that the planes before it left, so
-// three hold all 24 bits of a float32 and two the 11 of a float16.  What is not finite stays in the first.
+// three hold all 24 bits of a float32 (of one below 2^-110 those down to 2^-133) and two the 11 of a float16.  What is not
+// finite stays in the first.
 template <int P, class T>
 __global__ __launch_bounds__(256) void nz_mx_planes_kernel(const T* g, uint64_t stride, uint64_t m, uint32_t n,
                                                            uint32_t padded, nz_bf16* out) {

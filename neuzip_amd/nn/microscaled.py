@@ -3,6 +3,9 @@
 reaches them, the gradients of a Linear's input and bias do.
 
 The stored tensors are buffers, so they travel with ``state_dict`` and ``.to``.
+Whatever writes to them between a forward pass and its backward makes that an
+error; ``DistributedDataParallel`` does so at every forward, unless it is told
+``broadcast_buffers=False``.
 """
 from __future__ import annotations
 
