@@ -279,7 +279,7 @@ def _held(x, block):
 
 def _exact_function(kind, x):
     if kind == "gelu":
-        p = torch.special.ndtr(x)
+        p = torch.exp(torch.special.log_ndtr(x))  # (ndtr itself loses its digits below -5)
         return x * p, p + x * torch.exp(-0.5 * x * x) / math.sqrt(2 * math.pi)
     if kind == "gelu_tanh":
         u = math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
