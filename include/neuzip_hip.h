@@ -514,6 +514,81 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
                           uint64_t rows, uint64_t cols, float scale, int64_t padding_idx, uint32_t flags,
                           void* dev_out, void* dev_workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- tensors in 8 bits with a scale for each block of 128 -----------------
+ *
+ * No counterpart in the reference.  Weights that are multiplied as they are, and
+ * activations that a training step keeps for its backward pass.  The calls hold
+ * no state, as above.
+ *
+ * The format.  A block is 128 values of a row (block_rows = 1) or 128 rows of 128
+ * columns (block_rows = 128), counted from the first row and column; the last
+ * ones may be smaller.  A block shares a power of two X = 2^(s - 127), s the
+ * smallest, not below 0, with which its largest magnitude is at most 448 X; a
+ * value v is held as v / X rounded to an e4m3 number, to the nearest, ties to the
+ * even code.  A block with a NaN or an infinity has s = 255 and reads as NaN.
+ * Data: rows of nz_fp8_row_bytes(cols), values in order, filled up to 128 values
+ * with zeros.  Scales: a row of nz_fp8_scale_bytes(cols) for each row (or 128
+ * rows), one byte s per block in order, filled up to 4 bytes with zeros.  Both are
+ * 16-byte aligned. */
+uint64_t nz_fp8_row_bytes(uint64_t cols);
+uint64_t nz_fp8_scale_bytes(uint64_t cols);
+
+/* rows x cols values at dev_x, `stride` elements from row to row, and the values back, rows contiguous, rounded to
+   dtype.  cols is up to 2^30, rows * ceil(cols / 512) up to 2^33, here and below. */
+int nz_fp8_quantize(const void* dev_x, int dtype, uint64_t rows, uint64_t cols, uint64_t stride, int block_rows,
+                    void* dev_data, void* dev_scales, void* stream);
+int nz_fp8_dequantize(const void* dev_data, const void* dev_scales, uint64_t rows, uint64_t cols, int block_rows,
+                      void* dev_out, int dtype, void* stream);
+
+/* y[m][n] = sum_k x[m][k] w[n][k] + bias[n]: w holds n rows of k values in 8 bits (in blocks of block_rows rows), the m
+   rows of x are brought to 8 bits (blocks of one row) on the way.  bias may be NULL; it, x and y have the same dtype,
+   to which the sum is rounded once.
+   How it is added: as nz_mx_linear states, NZ_DTYPE_F32 in 32 bits, the 16-bit types by the scaled matrix instruction,
+   which cuts each of eight consecutive products 13 places behind the largest exponent of the eight.
+   k is 1 to 2^22, n at most 2^21, m at most 2^24.  The workspace is as above. */
+uint64_t nz_fp8_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype);
+int nz_fp8_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t stride, const void* dev_w_data,
+                  const void* dev_w_scales, uint64_t n, int block_rows, const void* dev_bias, void* dev_y,
+                  void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
+/* The same for rows that are held in 8 bits already (blocks of one row). */
+int nz_fp8_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64_t m, uint64_t k,
+                        const void* dev_w_data, const void* dev_w_scales, uint64_t n, int block_rows,
+                        const void* dev_bias, void* dev_y, int dtype, void* dev_workspace, uint64_t workspace_bytes,
+                        void* stream);
+
+/* dx[m][k] = sum_n g[m][n] w[n][k]: the gradient of that product's rows (their rounding to 8 bits is passed straight
+   through), in 32 bits.  n is 1 at least. */
+uint64_t nz_fp8_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
+                                            uint64_t k);
+int nz_fp8_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
+                       const void* dev_w_scales, uint64_t k, int block_rows, void* dev_dx, void* dev_workspace,
+                       uint64_t workspace_bytes, void* stream);
+
+/* out[n][k] = sum_m g[m][n] x[m][k], the gradient of a weight of n rows whose input was kept as m rows of k values in 8
+   bits, in 32 bits, in an order that the sizes alone decide.  NZ_GRAD_ACCUMULATE adds to out (rounded once) instead of
+   setting it.  m is 1 to 2^24, n at most 2^21, k at most 2^22. */
+uint64_t nz_fp8_weight_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
+                                            uint64_t k);
+int nz_fp8_weight_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_x_data,
+                       const void* dev_x_scales, uint64_t k, int block_rows, uint32_t flags, void* dev_out,
+                       void* dev_workspace, uint64_t workspace_bytes, void* stream);
+
+/* y = f(x), times `up` where dev_up is not NULL (rows and columns as x), rows contiguous, rounded once; x (and up) are
+   kept in 8 bits (blocks of one row; not where dev_x_data is NULL) for
+   dx = g f'(x) (times up), dup = g f(x), with x and up as the 8 bits hold them.
+   f: x times the normal distribution's integral up to x; the same by its approximation with a hyperbolic tangent,
+   x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3))); x / (1 + exp(-x)). */
+#define NZ_ACTIVATION_GELU 0
+#define NZ_ACTIVATION_GELU_TANH 1
+#define NZ_ACTIVATION_SILU 2
+int nz_fp8_activation(int kind, const void* dev_x, int dtype, uint64_t rows, uint64_t cols, uint64_t stride,
+                      const void* dev_up, uint64_t up_stride, void* dev_y, void* dev_x_data, void* dev_x_scales,
+                      void* dev_up_data, void* dev_up_scales, void* stream);
+int nz_fp8_activation_grad(int kind, const void* dev_g, int dtype, uint64_t rows, uint64_t cols, uint64_t stride,
+                           const void* dev_x_data, const void* dev_x_scales, const void* dev_up_data,
+                           const void* dev_up_scales, void* dev_dx, void* dev_dup, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

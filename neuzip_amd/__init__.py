@@ -10,10 +10,10 @@ from neuzip_amd import nn, ops
 from neuzip_amd.binding import Algorithm, Manager
 from neuzip_amd.fused import FusedGemv
 from neuzip_amd.prefetch import DecompressAhead
-from neuzip_amd.utils import mx_convert
+from neuzip_amd.utils import fp8_activations, fp8_convert, mx_convert
 
 __all__ = ["ops", "nn", "Algorithm", "Manager", "DecompressAhead", "FusedGemv", "lomo_hook", "compressed_lomo_hook",
-           "mx_convert"]
+           "mx_convert", "fp8_convert", "fp8_activations"]
 
 
 def _current_lr(scheduler) -> float:

@@ -2,9 +2,10 @@
 
 Nine translation units of the codec: nz_launch.hip twice per precision (the
 encode kernels and the decode kernels of one kept-mantissa setting) and
-nz_api.hip (the C ABI and the kernels all precisions share); two more hold the
-operators on microscaled weights (nz_mx.hip) and on embedding gradients
-(nz_embedding.hip).  They compile side by side and are linked into one library.
+nz_api.hip (the C ABI and the kernels all precisions share); three more hold the
+operators on microscaled weights (nz_mx.hip), on embedding gradients
+(nz_embedding.hip) and on tensors in 8 bits (nz_fp8.hip).  They compile side by
+side and are linked into one library.
 """
 from __future__ import annotations
 
@@ -52,7 +53,7 @@ def units(objdir: str):
 def operator_units(objdir: str):
     """The same of the translation units beside the codec."""
     return [(os.path.join(CSRC, f"{stem}.hip"), [], os.path.join(objdir, f"{stem}.o"))
-            for stem in ("nz_mx", "nz_embedding")]
+            for stem in ("nz_mx", "nz_embedding", "nz_fp8")]
 
 
 def run(cmd, verbose: bool) -> None:

@@ -22,7 +22,8 @@ DEFAULT_CHUNK = 131072
 DEFAULT_LANE_SYMS = 256
 DEFAULT_SIZE_BUDGET = 1.01
 LANE_SYMS_AUTO = 0xFFFFFFFF
-GRAD_BY_FREQUENCY, GRAD_ACCUMULATE = 1, 2  # nz_embedding_gradient flags
+GRAD_BY_FREQUENCY, GRAD_ACCUMULATE = 1, 2  # nz_embedding_gradient flags, the second nz_fp8_weight_grad's too
+ACTIVATION_GELU, ACTIVATION_GELU_TANH, ACTIVATION_SILU = 0, 1, 2  # nz_fp8_activation kinds
 DECODE_CHECK, DECODE_STREAM_OUT, DECODE_RESIDENT_OUT = 1, 2, 4  # nz_decode flags
 
 EXPORTS = [
@@ -38,6 +39,10 @@ EXPORTS = [
     "nz_mx_linear_grad_workspace_bytes", "nz_mx_linear_grad",
     "nz_column_sums_workspace_bytes", "nz_column_sums",
     "nz_embedding_gradient_workspace_bytes", "nz_embedding_gradient",
+    "nz_fp8_row_bytes", "nz_fp8_scale_bytes", "nz_fp8_quantize", "nz_fp8_dequantize",
+    "nz_fp8_linear_workspace_bytes", "nz_fp8_linear", "nz_fp8_linear_rows8",
+    "nz_fp8_linear_grad_workspace_bytes", "nz_fp8_linear_grad",
+    "nz_fp8_weight_grad_workspace_bytes", "nz_fp8_weight_grad", "nz_fp8_activation", "nz_fp8_activation_grad",
 ]
 
 _lib = None
@@ -166,6 +171,32 @@ def load() -> ctypes.CDLL:
     L.nz_embedding_gradient.restype = i32
     L.nz_embedding_gradient.argtypes = [vp, u64, vp, i32, u64, u64, u64, ctypes.c_float, ctypes.c_int64, u32, vp, vp,
                                         u64, vp]
+    L.nz_fp8_row_bytes.restype = u64
+    L.nz_fp8_row_bytes.argtypes = [u64]
+    L.nz_fp8_scale_bytes.restype = u64
+    L.nz_fp8_scale_bytes.argtypes = [u64]
+    L.nz_fp8_quantize.restype = i32
+    L.nz_fp8_quantize.argtypes = [vp, i32, u64, u64, u64, i32, vp, vp, vp]
+    L.nz_fp8_dequantize.restype = i32
+    L.nz_fp8_dequantize.argtypes = [vp, vp, u64, u64, i32, vp, i32, vp]
+    L.nz_fp8_linear_workspace_bytes.restype = u64
+    L.nz_fp8_linear_workspace_bytes.argtypes = [u64, u64, u64, i32]
+    L.nz_fp8_linear.restype = i32
+    L.nz_fp8_linear.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, i32, vp, vp, vp, u64, vp]
+    L.nz_fp8_linear_rows8.restype = i32
+    L.nz_fp8_linear_rows8.argtypes = [vp, vp, u64, u64, vp, vp, u64, i32, vp, vp, i32, vp, u64, vp]
+    L.nz_fp8_linear_grad_workspace_bytes.restype = u64
+    L.nz_fp8_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
+    L.nz_fp8_linear_grad.restype = i32
+    L.nz_fp8_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, i32, vp, vp, u64, vp]
+    L.nz_fp8_weight_grad_workspace_bytes.restype = u64
+    L.nz_fp8_weight_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
+    L.nz_fp8_weight_grad.restype = i32
+    L.nz_fp8_weight_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, i32, u32, vp, vp, u64, vp]
+    L.nz_fp8_activation.restype = i32
+    L.nz_fp8_activation.argtypes = [i32, vp, i32, u64, u64, u64, vp, u64, vp, vp, vp, vp, vp, vp]
+    L.nz_fp8_activation_grad.restype = i32
+    L.nz_fp8_activation_grad.argtypes = [i32, vp, i32, u64, u64, u64, vp, vp, vp, vp, vp, vp, vp]
     _lib = L
     return L
 

@@ -8,10 +8,15 @@ Behaviour follows the reference's ``CompressedLinear`` (neuzip/ops/linear.py:11-
   on the parameter's ``_gradient`` slot (not in ``.grad``), and hand autograd a
   zero-size tensor for the placeholder so that post-accumulate-grad hooks of
   the compressed parameter still fire.
+
+:class:`CompressedLinearHeld8` does the same, but keeps the activation in 8 bits
+(``fp8_quantize``) for ``dL/dW``, which is then that of the kept values.
 """
 from __future__ import annotations
 
 import torch
+
+from neuzip_amd.ops.blocks8 import FP8Tensor, _saved, _unsaved, fp8_quantize, fp8_weight_gradient
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -49,4 +54,38 @@ class CompressedLinear(torch.autograd.Function):
             _p._gradient.add_(grad_w)
 
         grad_b = go2d.sum(0) if bias is not None else None
+        return grad_x, torch.empty_like(_p.data), grad_b
+
+
+class CompressedLinearHeld8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, inputs, _p, bias):
+        ctx._inputs_dtype = inputs.dtype
+        x = inputs
+        if torch.is_autocast_enabled():
+            x = x.to(torch.get_autocast_gpu_dtype())
+        held = fp8_quantize(x)
+        ctx.carry = (_p, held, bias is not None)
+        _saved(ctx, held)
+        return _p.linear(x, bias)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        _p, held, has_bias = ctx.carry
+        (held,) = _unsaved(ctx, held)
+        go2d = _as_rows(grad_output)
+        dense_w = _p.shared()
+
+        grad_x = torch.mm(go2d, dense_w).reshape(held.shape).to(ctx._inputs_dtype)
+        del dense_w
+        held = FP8Tensor._of(held.data, held.scales, (go2d.shape[0], held.shape[-1]), 1)
+        into = _p._gradient
+        if into is None:
+            _p._gradient = fp8_weight_gradient(go2d, held)
+        elif into.dtype == go2d.dtype and into.is_contiguous():
+            fp8_weight_gradient(go2d, held, out=into)
+        else:
+            into.add_(fp8_weight_gradient(go2d, held))
+
+        grad_b = go2d.sum(0) if has_bias else None
         return grad_x, torch.empty_like(_p.data), grad_b

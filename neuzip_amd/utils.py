@@ -81,8 +81,9 @@ def _convert(manager, module: torch.nn.Module, prefix: str = "") -> torch.nn.Mod
     return module
 
 
-def _heads(module: torch.nn.Module) -> set:
-    """The modules that stand in or below a child whose name contains ``lm_head``."""
+def _heads(module: torch.nn.Module, *marks: str) -> set:
+    """The modules that stand in or below a child whose name contains one of ``marks`` (``lm_head``)."""
+    marks = marks or ("lm_head",)
     heads, pending, seen = set(), [module], set()
     while pending:
         parent = pending.pop()
@@ -92,32 +93,71 @@ def _heads(module: torch.nn.Module) -> set:
         for name, child in parent._modules.items():  # every name: named_children gives a module once
             if child is None:
                 continue
-            if "lm_head" in name:
+            if any(mark in name for mark in marks):
                 heads.update(child.modules())
             else:
                 pending.append(child)
     return heads
 
 
-def mx_convert(module: torch.nn.Module, prefix: str = "", _made=None, _kept=None) -> torch.nn.Module:
+def _replace(module: torch.nn.Module, prefix: str, make, made, kept) -> torch.nn.Module:
+    """In place: children (at any depth) for which ``make(child)`` is not None become what it gives, those in ``kept``
+    aside.  A module that stands in several places is replaced once."""
+    for name, child in list(module._modules.items()):
+        dotted = f"{prefix}.{name}" if prefix else name
+        if child is None or child in kept:
+            continue
+        if child not in made:
+            new = make(child)
+            if new is not None:
+                logger.debug("Converting %s: %s", dotted, child)
+                made[child] = new
+                _delete_module(child)
+        if child in made:
+            setattr(module, name, made[child])
+        else:
+            _replace(child, dotted, make, made, kept)
+    return module
+
+
+def mx_convert(module: torch.nn.Module, prefix: str = "") -> torch.nn.Module:
     """In place: the ``nn.Linear`` layers that ``Manager.convert`` would compress
     (those whose attribute name contains ``lm_head`` are left alone, wherever else
     they stand too) are held in microscaled 4 bits instead, with their weights
     frozen.  A layer that stands in several places is converted once."""
     from neuzip_amd.nn import MXLinear
 
-    made = {} if _made is None else _made
-    kept = _heads(module) if _kept is None else _kept
-    for name, child in list(module._modules.items()):
-        dotted = f"{prefix}.{name}" if prefix else name
-        if child is None or child in kept:
-            continue
-        if isinstance(child, torch.nn.Linear):
-            if child not in made:
-                logger.debug("Converting %s: %s", dotted, child)
-                made[child] = MXLinear(child)
-                _delete_module(child)
-            setattr(module, name, made[child])
-        else:
-            mx_convert(child, dotted, made, kept)
-    return module
+    return _replace(module, prefix, lambda m: MXLinear(m) if isinstance(m, torch.nn.Linear) else None, {},
+                    _heads(module))
+
+
+def fp8_convert(module: torch.nn.Module, prefix: str = "", block_rows: int = 128) -> torch.nn.Module:
+    """The same with weights in 8 bits: 128 rows of 128 columns share a scale, or with
+    ``block_rows=1`` 128 values of a row."""
+    from neuzip_amd.nn import FP8Linear
+
+    return _replace(module, prefix, lambda m: FP8Linear(m, block_rows) if isinstance(m, torch.nn.Linear) else None, {},
+                    _heads(module))
+
+
+def fp8_activations(module: torch.nn.Module, skip=(), prefix: str = "") -> torch.nn.Module:
+    """In place: what a training step keeps of activations is kept in 8 bits.  Compressed
+    Linear layers (``neuzip_amd.nn.Linear``) get ``saved_bits = 8``; ``nn.GELU`` and
+    ``nn.SiLU`` become ``neuzip_amd.nn.FP8Activation``.  Modules whose attribute name
+    contains one of ``skip`` are left as they are, and so is what stands below them:
+    layers that share their input keep one of 16 bits together, but 8 bits each, so for
+    three of them (q, k and v) 16 bits are less."""
+    from neuzip_amd.nn import FP8Activation, Linear
+
+    kept = _heads(module, *skip) if skip else set()
+
+    def make(m):
+        if isinstance(m, Linear):
+            m.saved_bits = 8
+        elif isinstance(m, torch.nn.GELU):
+            return FP8Activation("gelu" if m.approximate == "none" else "gelu_tanh")
+        elif isinstance(m, torch.nn.SiLU):
+            return FP8Activation("silu")
+        return None
+
+    return _replace(module, prefix, make, {}, kept)
