@@ -396,6 +396,216 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU
   finish_tile<WM, WN, TM, TN, LDS>(acc, lds, m, n, m0, n0, bias, y, part);
 }
 
+__device__ inline i8v both(i4v a, i4v b) { return i8v{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}; }
+
+// `step` in assembly: the sum stays in the registers it is in, of the kind that only such instructions use.  (Where sums
+// fill half of all registers the compiler, which may choose others for each instruction's result, moves them about.)
+// What reads a sum, and the first instruction behind a write of its registers, has to wait: `settle`.
+template <int BYTE>
+__device__ inline void step_in_place(i8v w, i8v x, f4& acc, uint32_t sw, uint32_t sx) {
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0]"
+               : "+a"(acc)
+               : "v"(w), "v"(x), "v"(sw), "v"(sx), "n"(BYTE & 1), "n"(BYTE >> 1));
+}
+__device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+// The same for the largest products, whose results are of 16 bits: tiles of 256x256, four wavefronts of 128x128 each, a
+// compute unit's own, and every workgroup goes through several of them.  k is a multiple of 512.
+//
+// What a wavefront reads of LDS for its matrix instructions is the less the larger its tile: 32 KB a step for 64
+// instructions (2048 cycles), where 64x64 take 16 KB for 16.  A step's 64 squares are multiplied a row of x at a time, in
+// four places that are read again as soon as they are used up; w's eight follow beside the last row.  From the sixth row
+// on what is read is of the next step: before it is the step's only barrier, which tells that the stage behind has
+// arrived and that this one has been read, so that the loads of the stage after the next go there.  Steps follow each
+// other across tiles: the loads run ahead into the next tile, whose first operands are there when the result has been
+// stored.  It goes through a part of LDS that is each wavefront's own, 16 rows at a time.
+//
+// 8192 x (14336x4096): 363 to 378 us, 2.55 to 2.65 PFLOP/s (the tiles of 128x256 above 520 beside them; a library's
+// 8-bit product of 8192^3 reaches 2.75).  Of that some 50 are the stores of the results, in which all compute units meet
+// seven times; letting them start apart by up to half a tile gained nothing.
+template <class T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void nz_fp8_wide_kernel(
+    const uint8_t* xd, const uint8_t* xs, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t shift, uint32_t n,
+    uint32_t k, const T* bias, T* y, uint32_t mt, uint32_t nt) {
+  constexpr int SIDE = 256, XB = SIDE * 128, STAGE = 2 * XB, S_AT = 2 * STAGE, OUT_AT = S_AT + 2 * SIDE * 4;
+  constexpr int PITCH = 128 * (int)sizeof(T) + 16;  // a row of a wavefront's part of the result
+  static_assert(sizeof(T) == 2 && OUT_AT + 4 * 16 * PITCH <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[OUT_AT + 4 * 16 * PITCH];
+  const uint32_t base = lds_address(lds);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t r = lane & 15, g = lane / 16, wm = wave & 1, wn = wave / 2;
+  const uint32_t groups = k / kGroup, pitch = groups * 4, tiles = mt * nt;
+
+  // Where a lane loads a tile from: bases of the workgroup, moved from step to step, and offsets.  Rows behind the last
+  // one are read as the last.
+  const uint8_t *xb, *wb, *sb;
+  uint32_t xo[8], wo[8], so[2];
+  const auto column = [](uint32_t row) {  // of the tile, for a staged weight row: a lane ends with 32 consecutive ones
+    return row / 128 * 128 + row % 16 / 4 * 32 + row / 16 % 8 * 4 + row % 4;
+  };
+  const auto aim = [&](uint32_t tile, uint32_t group) {
+    uint32_t tm, tn;
+    tile_of(tile, mt, nt, tm, tn);
+    const uint32_t m0 = tm * SIDE, n0 = tn * SIDE;
+    const uint32_t m_last = min((uint32_t)SIDE, m - m0) - 1, n_last = min((uint32_t)SIDE, n - n0) - 1;
+    xb = xd + (uint64_t)m0 * k + group * kGroup, wb = wd + (uint64_t)n0 * k + group * kGroup;
+    const uint32_t chunk = ((lane & 7) ^ (lane / 8)) * 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t row = (wave * 8 + i) * 8 + lane / 8;
+      xo[i] = __umul24(min(row, m_last), k) + chunk;
+      wo[i] = __umul24(min(column(row), n_last), k) + chunk;
+    }
+    // wavefronts 0 and 1 load the scales of x, the others those of w
+    sb = wave < 2 ? xs + (uint64_t)m0 * pitch : ws + (uint64_t)(n0 >> shift) * pitch;
+    sb += group * 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t row = (wave % 2 * 2 + i) * 64 + lane;
+      so[i] = (wave < 2 ? min(row, m_last) : ((min(column(row), n_last) + n0) >> shift) - (n0 >> shift)) * pitch;
+    }
+  };
+  const auto load_x = [&](uint32_t buf, int i) { to_lds16(xb, xo[i], base + buf * STAGE + (wave * 8 + i) * 1024); };
+  const auto load_w = [&](uint32_t buf, int i) { to_lds16(wb, wo[i], base + buf * STAGE + XB + (wave * 8 + i) * 1024); };
+  const auto load_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) to_lds4(sb, so[i], base + S_AT + (wave * 2 + i) * 256);
+  };
+
+  f4 acc[8][8];
+  i8v x[4], w[8];
+  uint32_t sx[8], sw[8];
+  const uint32_t c0 = (g ^ (r & 7)) * 16, c1 = c0 ^ 64;
+  const uint32_t xr = (wm * 128 + r) * 128, wr = XB + (wn * 128 + r) * 128;
+  const auto read_x = [&](uint32_t buf, int i) {
+    x[i % 4] = both(*(const i4v*)(lds + buf * STAGE + xr + i * 2048 + c0),
+                    *(const i4v*)(lds + buf * STAGE + xr + i * 2048 + c1));
+  };
+  const auto read_w = [&](uint32_t buf, int j) {
+    w[j] = both(*(const i4v*)(lds + buf * STAGE + wr + j * 2048 + c0),
+                *(const i4v*)(lds + buf * STAGE + wr + j * 2048 + c1));
+  };
+  const auto read_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sx[i] = *(const uint32_t*)(lds + S_AT + (wm * 128 + i * 16 + r) * 4);
+      sw[i] = *(const uint32_t*)(lds + S_AT + SIDE * 4 + (wn * 128 + i * 16 + r) * 4);
+    }
+  };
+
+  uint32_t tile = blockIdx.x;
+  aim(tile, 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load_x(0, i), load_w(0, i);
+  load_scales();
+  xb += 128, wb += 128;
+  wait_loads<0>();
+  block_barrier();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) read_w(0, i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read_x(0, i);
+  read_scales();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load_x(1, i), load_w(1, i);
+  xb += 128, wb += 128;
+
+  // A step, s % 4 of a tile; stage s is in buffer s % 2.  An empty statement that could change a result holds each
+  // instruction in its place among the reads and loads.
+  const auto body = [&](auto b4) {
+    constexpr int byte = decltype(b4)::value, buf = byte % 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i == 5) {
+        wait_loads<0>();  // the next stage
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        block_barrier();
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        step_in_place<byte>(w[j], x[i % 4], acc[i][j], sw[j], sx[i]);
+        if (i == 7) read_w(buf ^ 1, j);
+        if (i == 5 || i == 6) {
+          if (i == 5) load_x(buf, j);
+          else load_w(buf, j);
+        }
+        if (j == 7 && i < 4) read_x(buf, i + 4);
+        if (j == 7 && i == 5) read_x(buf ^ 1, 0), read_x(buf ^ 1, 1);
+        if (j == 7 && i > 5) read_x(buf ^ 1, i - 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (byte == 2) load_scales();
+    if (byte == 3) read_scales();
+    xb += 128, wb += 128;
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  using B2 = std::integral_constant<int, 2>;
+  using B3 = std::integral_constant<int, 3>;
+  for (;;) {
+    uint32_t tm, tn;
+    tile_of(tile, mt, nt, tm, tn);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[i][j] = f4{0, 0, 0, 0};
+        asm volatile("" : "+a"(acc[i][j]));
+      }
+    settle();
+    const bool more = tile + gridDim.x < tiles;
+    const uint32_t next = more ? tile + gridDim.x : tile;  // behind the last tile its own begin, which is not used
+    uint32_t i = 0;
+    do {
+      body(B0());
+      body(B1());
+      ++i;
+      aim(i == groups ? next : tile, i == groups ? 0 : i);
+      body(B2());
+      body(B3());
+    } while (i != groups);
+    tile = next;
+    settle();
+
+    const uint32_t row0 = tm * SIDE + wm * 128, col0 = tn * SIDE + wn * 128;
+    uint8_t* mine = lds + OUT_AT + wave * 16 * PITCH;
+    typedef T whole __attribute__((ext_vector_type(8)));
+    typedef T piece __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) asm volatile("" : "+a"(acc[i][j]));  // they stay in their registers until here
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        float v[8], b[8] = {};
+        const uint32_t c = col0 + g * 32 + j * 4;
+        if (bias && c < n) load8_upto(bias + c, n - c, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][j + e / 4][e % 4] + b[e];
+        store8((T*)(mine + r * PITCH) + g * 32 + j * 4, v);
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t at = q * 4 + lane / 16, row = row0 + i * 16 + at, c = col0 + lane % 16 * 8;
+        const whole v = *(const whole*)(mine + at * PITCH + lane % 16 * 16);
+        if (row >= m || c >= n) continue;
+        T* to = y + (uint64_t)row * n + c;
+        if (c + 8 <= n)
+          *(piece*)to = v;
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c + e < n) to[e] = v[e];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (!more) break;
+  }
+  wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
+}
+
 // Up to 16 rows, where reading the weight is all that counts: no staging and no barrier in the way of it.  The eight
 // wavefronts are kw that share the values of a row (512 at a time, in turn) times 8 / kw with 16 weight rows each;
 // a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
@@ -857,17 +1067,21 @@ int launch_values(const void* data, const void* scales, uint32_t shift, uint64_t
   return nz_launched();
 }
 
+// Figures of the tiles, and of those of 16-bit rows: fitted to times of 60 products of 17 to 8192 rows with weights of 256
+// to 16384 rows and columns, each in all tiles and up to 16 parts.  The cut chosen by them takes 1.2 % more than the
+// fastest one in the mean.
 // Products of 8-bit rows, 128 values a step.
-constexpr Tile kTiles[] = {{128, 256, 256, 0.90f, 0.90f},
-                           {128, 128, 512, 1.00f, 1.00f},
-                           {64, 128, 256, 0.36f, 0.38f},
-                           {64, 64, 256, 0.25f, 0.28f}};
+constexpr Tile kTiles[] = {{256, 256, 256, 1.31f, 0.94f, 4.0f, true},
+                           {128, 256, 256, 0.72f, 0.74f, 3.2f},
+                           {128, 128, 512, 0.78f, 0.76f, 2.4f},
+                           {64, 128, 256, 0.30f, 0.28f, 1.1f},
+                           {64, 64, 256, 0.21f, 0.13f, 0.8f}};
 // Products of 16-bit rows, 64 values a step.
 constexpr Tile kTiles16[] = {{256, 128, 256, 0.95f, 0.86f}, {64, 64, 256, 0.31f, 0.31f}};
 
 // The product of 8-bit rows, cut along k by groups of four steps, two at least.
 Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
-  return cut_product(kTiles, m, n, nz_ceil_div(k, kGroup), 4, 2);
+  return cut_product(kTiles, m, n, nz_ceil_div(k, kGroup), 4, 2, k % kGroup == 0);
 }
 
 // The products of 16-bit rows, in steps of 64.
@@ -883,7 +1097,12 @@ void launch_tiles(const Cut& c, const void* xd, const void* xs, uint64_t m, cons
   nz_fp8_tiles_kernel<WM, WN, TM, TN, NS, EU, T><<<grid, 64 * WM * WN, 0, st>>>(                                   \
       (const uint8_t*)xd, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, shift,          \
       (uint32_t)n, k, bias, y, c.mt, c.nt, c.part_length, part)
-  if (c.bn == 256)
+  const uint32_t cus = nz_compute_units();
+  if (c.bm == 256)
+    nz_fp8_wide_kernel<T><<<std::min(c.mt * c.nt, cus ? cus : 256), 256, 0, st>>>(
+        (const uint8_t*)xd, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, shift, (uint32_t)n,
+        k, bias, y, c.mt, c.nt);
+  else if (c.bn == 256)
     NZ_TILES(2, 4, 4, 4, 3, 2);
   else if (c.bm == 128)
     NZ_TILES(2, 2, 4, 4, 2, 2);

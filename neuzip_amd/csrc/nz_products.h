@@ -293,36 +293,39 @@ struct Cut {
 };
 
 // What a step takes (us) of a kernel with this tile while `slots` workgroups run, and while half of them or fewer do,
-// on 256 compute units.
+// on 256 compute units; the begin and end of a round of workgroups, which others do not cover; and whether it takes whole
+// products of whole steps only.
 struct Tile {
   uint32_t bm, bn, slots;
-  float full, half;
+  float full, half, ends = 1.0f;
+  bool whole = false;
 };
 
-// The cut that takes the least time by these figures.  Rounds of workgroups follow each other and begin and end in 1 us
-// that others do not cover; parts cost a launch of 4 us and are written, read and joined at 5 TB/s.
+// The cut that takes the least time by these figures.  Rounds of workgroups follow each other; parts cost a launch of
+// 4 us and are written, read and joined at 5 TB/s.  `whole`: the product is one of whole steps.
 // From rows in 8 bits, 64 x (4096x14336) takes 24 us in 64 tiles of 64x64 and 12.5 in four parts of them; 17 x
 // (128256x4096) 71 us in tiles of 128x256, 51 in 64x128.  Where the figures are off: 5366 x (576x12736) takes 64 us in
 // the 420 tiles of 64x128 that are chosen, 60 in two parts of 210 tiles of 128x128.
 template <int N>
 Cut cut_product(const Tile (&kinds)[N], uint64_t m, uint64_t cols, uint64_t units_of, uint64_t steps_per_unit,
-                uint64_t least) {
+                uint64_t least, bool whole = false) {
   const uint32_t cus = nz_compute_units();
   const float scale = cus ? cus / 256.0f : 1.0f;
   Cut best = {};
   float best_time = 0;
   for (const Tile& t : kinds) {
+    if (t.whole && !whole) continue;
     const uint64_t mt = nz_ceil_div(m, t.bm), nt = nz_ceil_div(cols, t.bn);
     const float slots = t.slots * scale;
     const uint32_t units = (uint32_t)std::min<uint64_t>(units_of, 1u << 30);
     for (uint32_t want = 1; want <= std::min<uint64_t>(units_of, 16); ++want) {
-      if (want > 1 && (float)(mt * nt * want) > 4 * slots) break;  // enough without parts
+      if (want > 1 && (t.whole || (float)(mt * nt * want) > 4 * slots)) break;  // enough without parts
       const uint32_t length = (units + want - 1) / want, parts = (units + length - 1) / length;
       if (parts != want || (parts > 1 && length < least)) continue;
       const float groups = (float)(mt * nt * parts), rounds = floorf(groups / slots), rest = groups - rounds * slots;
       float time = (rounds * t.full + (rest == 0 ? 0.0f : rest <= slots / 2 ? t.half : t.full)) *
                        (float)(length * steps_per_unit) +
-                   rounds + (rest > 0);
+                   t.ends * rounds + t.ends * (rest > 0);
       if (parts > 1) time += 4.0f + (float)parts * (float)m * (float)cols * 2.8e-6f;
       if (best.parts == 0 || time < best_time) {
         best = Cut{t.bm, t.bn, (uint32_t)parts, (uint32_t)length, (uint32_t)mt, (uint32_t)nt};

@@ -147,6 +147,21 @@ def test_large_products_of_whole_numbers_are_exact(m, n):
         same(ops.fp8_linear(x, ops.fp8_quantize(wd, block_rows)), round_to(want.cpu(), torch.bfloat16))
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 1024), (4097, 4101, 512), (8100, 6000, 1536), (3900, 5003, 2048)])
+def test_products_of_whole_steps_are_exact(m, n, k, dtype):
+    """rows of a multiple of 512 values: the tiles that workgroups go through one after the other, their ends, a scale of
+    its own in every block, a bias"""
+    up = torch.exp2(torch.arange(k) // 128 % 5 - 2.0).to(DEV)
+    x, wd = (whole_numbers(rows, k, 7, seed).to(DEV) for rows, seed in ((m, 1), (n, 2)))
+    rows = torch.exp2(torch.arange(m, device=DEV) % 3 - 1.0)[:, None]
+    bias = whole_numbers(1, n, 99, 5, dtype)[0].to(DEV)
+    want = (x * rows).double() @ wd.double().t() + bias.double()
+    for block_rows in (1, 128):
+        got = ops.fp8_linear((x * rows * up).to(dtype), ops.fp8_quantize(wd / up, block_rows), bias)
+        same(got, round_to(want.cpu(), dtype))
+
+
 @pytest.mark.parametrize("block_rows", (1, 128))
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("m,n,k", [(1, 200, 1024), (4, 131, 1001), (50, 60, 640), (70, 130, 300), (260, 48, 300)])
