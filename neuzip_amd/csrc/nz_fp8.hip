@@ -46,25 +46,39 @@ __device__ inline uint32_t block_scale(float (&v)[8]) {
 //
 // One wavefront per 512 values of a row: 8 values a lane, 16 lanes a block.
 
+// Division of the number of a wavefront, below 2^26 in one launch, by the groups of 512 values in a row: n / d is
+// n mul >> shift with mul = floor(2^shift / d) + 1 and 2^shift >= 2^26 d, for then n (mul d - 2^shift) < 2^shift.
+// (In 64 bits as it is, it takes more instructions than what follows.)
+struct Groups {
+  uint32_t count, mul, shift;
+};
+struct Place {
+  uint64_t row;
+  uint32_t at;  // column of the lane's first value
+};
+__device__ inline Place place_of(uint32_t wave, const Groups& g) {
+  const uint32_t n = __builtin_amdgcn_readfirstlane(wave);
+  const uint32_t row = (uint32_t)((uint64_t)n * g.mul >> g.shift);
+  return Place{row, (n - row * g.count) * kGroup + (threadIdx.x & 63) * 8};
+}
+
 // Codes and scale of 8 values of a row (`at` its first one's column, a multiple of 8) by a lane of such a wavefront.
-__device__ inline void hold(float (&v)[8], uint64_t row, uint32_t at, uint32_t cols, uint32_t groups, uint8_t* data,
-                            uint8_t* scales) {
+__device__ inline void hold(float (&v)[8], Place at, uint32_t cols, uint32_t groups, uint8_t* data, uint8_t* scales) {
   const uint32_t s = block_scale(v), filled = (cols + kStep - 1) / kStep * kStep;
-  if (at < filled) *reinterpret_cast<uint2*>(data + row * filled + at) = codes8(v, up_factor(s));
-  if (at % kStep == 0) scales[row * (groups * 4ull) + at / kStep] = (uint8_t)s;
+  if (at.at < filled) *reinterpret_cast<uint2*>(data + at.row * filled + at.at) = codes8(v, up_factor(s));
+  if (at.at % kStep == 0) scales[at.row * (groups * 4ull) + at.at / kStep] = (uint8_t)s;
 }
 
 template <class T>
 __global__ __launch_bounds__(256) void nz_fp8_quantize_kernel(const T* x, uint64_t stride, uint32_t cols,
-                                                              uint64_t waves, uint32_t groups, uint8_t* data,
+                                                              uint32_t waves, Groups groups, uint8_t* data,
                                                               uint8_t* scales) {
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const uint32_t wave = blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
-  const uint64_t row = wave / groups;
-  const uint32_t at = (uint32_t)(wave - row * groups) * kGroup + (threadIdx.x & 63) * 8;
+  const Place p = place_of(wave, groups);
   float v[8];
-  load8_upto(x + row * stride + at, at < cols ? cols - at : 0, v);
-  hold(v, row, at, cols, groups, data, scales);
+  load8_upto(x + p.row * stride + p.at, p.at < cols ? cols - p.at : 0, v);
+  hold(v, p, cols, groups.count, data, scales);
 }
 
 // A workgroup per block of 128 x 128 values, which stay in registers between the search for the largest and the
@@ -76,15 +90,25 @@ __global__ __launch_bounds__(256) void nz_fp8_quantize_blocks_kernel(const T* x,
   const uint32_t down = blockIdx.x / blocks, across = blockIdx.x - down * blocks;
   const uint32_t at = across * kStep + threadIdx.x % 16 * 8, n = at < cols ? cols - at : 0;
   const uint64_t first = down * 128ull + threadIdx.x / 16;
-  float v[8][8];
-  uint32_t top = 0;
+  typename Pack<T>::type raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint64_t row = first + i * 16;
-    load8_upto(x + min(row, rows - 1) * stride + at, row < rows ? n : 0, v[i]);
-  }
+    const T* p = x + min(first + i * 16, rows - 1) * stride + at;
+    if (n >= 8) {
+      raw[i] = *(const typename Pack<T>::type*)p;
+    } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, top8(v[i]));
+      for (int e = 0; e < 8; ++e) raw[i][e] = (uint32_t)e < n ? p[e] : (T)0.0f;
+    }
+  }
+  uint32_t top = 0;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)raw[i][e];
+    top = max(top, top8(v));  // a row behind the last is the last one once more
+  }
   top = max16(top);
   top = max(top, (uint32_t)__shfl_xor((int)top, 16));
   top = max(top, (uint32_t)__shfl_xor((int)top, 32));
@@ -96,10 +120,10 @@ __global__ __launch_bounds__(256) void nz_fp8_quantize_blocks_kernel(const T* x,
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint64_t row = first + i * 16;
-    if (s == 255)
+    asm volatile("" : "+v"(raw[i]));  // converted again instead of kept in 32 bits: twice the wavefronts
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-    if (row < rows) *reinterpret_cast<uint2*>(data + row * (blocks * 128ull) + at) = codes8(v[i], up);
+    for (int e = 0; e < 8; ++e) v[e] = s == 255 ? 0.0f : (float)raw[i][e];
+    if (row < rows) *reinterpret_cast<uint2*>(data + row * (blocks * 128ull) + at) = codes8(v, up);
   }
   uint8_t* to = scales + (uint64_t)down * pitch + across;
   if (threadIdx.x == 0) *to = (uint8_t)s;
@@ -108,17 +132,18 @@ __global__ __launch_bounds__(256) void nz_fp8_quantize_blocks_kernel(const T* x,
 
 template <class T>
 __global__ __launch_bounds__(256) void nz_fp8_values_kernel(const uint8_t* data, const uint8_t* scales, uint32_t shift,
-                                                            uint64_t first, uint32_t cols, uint64_t waves,
-                                                            uint32_t groups, T* out) {
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+                                                            uint64_t first, uint32_t cols, uint32_t waves,
+                                                            Groups groups, T* out) {
+  const uint32_t wave = blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
-  const uint64_t row = first + wave / groups;
-  const uint32_t at = (uint32_t)(wave % groups) * kGroup + (threadIdx.x & 63) * 8;
+  const Place p = place_of(wave, groups);
+  const uint64_t row = first + p.row;
+  const uint32_t at = p.at;
   if (at >= cols) return;
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
   float v[8];
   values8(*reinterpret_cast<const uint2*>(data + row * filled + at),
-          down_factor(scales[(row >> shift) * (groups * 4ull) + at / kStep]), v);
+          down_factor(scales[(row >> shift) * (groups.count * 4ull) + at / kStep]), v);
   store8_upto(out + row * cols + at, cols - at, v);
 }
 
@@ -144,17 +169,26 @@ template <int KIND, bool FINE, bool SLOPE>
 __device__ inline float gate(float x, float& slope) {
   if constexpr (KIND == NZ_ACTIVATION_GELU) {
     // p is the normal distribution's integral.  Below zero it is exp(-x^2 / 2) r(t), r(t) = t times a polynomial in
-    // t = 1 / (1 + 0.35 |x|), fitted to the least relative error from 0 to -14 (3.2e-8; the integral is below 2^-126
-    // from -13 on).
-    const float a = fminf(fabsf(x), 30.0f), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
+    // t = 1 / (1 + c |x|), fitted to the least relative error from 0 to -14 (3.2e-8, for results of 16 bits 1.5e-07; the
+    // integral is below 2^-126 from -13 on).
     constexpr float k[9] = {0.139621407f,  0.139861897f,  0.119832724f, 0.105508536f, -0.0231109783f,
                             0.159175649f, -0.25571543f, 0.143972203f, -0.0291460212f};
-    float r = k[8];
+    constexpr float k16[8] = {0.119629294f, 0.120754004f, 0.0999131426f, 0.128562927f,
+                              -0.0536863729f, 0.206356779f, -0.15720515f, 0.0356753133f};
+    // (FINE subtracts squares, which must not overflow)
+    const float a = FINE ? fminf(fabsf(x), 30.0f) : fabsf(x);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(FINE ? 0.35f : 0.3f, a, 1.0f));
+    float r = FINE ? k[8] : k16[7];
 #pragma unroll
-    for (int i = 7; i >= 0; --i) r = __builtin_fmaf(r, t, k[i]);
+    for (int i = FINE ? 7 : 6; i >= 0; --i) r = __builtin_fmaf(r, t, FINE ? k[i] : k16[i]);
     const float square = a * a;
-    float e = exp_of<FINE>(-0.5f * square);
-    if constexpr (FINE) e = __builtin_fmaf(e, -0.5f * __builtin_fmaf(a, a, -square), e);
+    float e;
+    if constexpr (FINE) {
+      e = exp_of<true>(-0.5f * square);
+      e = __builtin_fmaf(e, -0.5f * __builtin_fmaf(a, a, -square), e);
+    } else {
+      e = __builtin_amdgcn_exp2f(square * (-0.5f * kLog2E));
+    }
     const float tail = e * (r * t), p = x > 0.0f ? 1.0f - tail : tail;
     if constexpr (SLOPE) slope = __builtin_fmaf(x * e, 0.398942280f, p);
     return p;
@@ -178,14 +212,15 @@ __device__ inline float gate(float x, float& slope) {
 // row, as above.
 template <int KIND, bool GATED, class T>
 __global__ __launch_bounds__(256) void nz_fp8_activation_kernel(const T* x, uint64_t stride, const T* up,
-                                                                uint64_t up_stride, uint32_t cols, uint64_t waves,
-                                                                uint32_t groups, T* y, uint8_t* x_data,
+                                                                uint64_t up_stride, uint32_t cols, uint32_t waves,
+                                                                Groups groups, T* y, uint8_t* x_data,
                                                                 uint8_t* x_scales, uint8_t* up_data,
                                                                 uint8_t* up_scales) {
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const uint32_t wave = blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
-  const uint64_t row = wave / groups;
-  const uint32_t at = (uint32_t)(wave - row * groups) * kGroup + (threadIdx.x & 63) * 8, n = at < cols ? cols - at : 0;
+  const Place p = place_of(wave, groups);
+  const uint64_t row = p.row;
+  const uint32_t at = p.at, n = at < cols ? cols - at : 0;
   float v[8], u[8], f[8], none;
   load8_upto(x + row * stride + at, n, v);
   if constexpr (GATED) load8_upto(up + row * up_stride + at, n, u);
@@ -196,24 +231,25 @@ __global__ __launch_bounds__(256) void nz_fp8_activation_kernel(const T* x, uint
   }
   if (n) store8_upto(y + row * cols + at, n, f);
   if (!x_data) return;
-  hold(v, row, at, cols, groups, x_data, x_scales);
-  if constexpr (GATED) hold(u, row, at, cols, groups, up_data, up_scales);
+  hold(v, p, cols, groups.count, x_data, x_scales);
+  if constexpr (GATED) hold(u, p, cols, groups.count, up_data, up_scales);
 }
 
 // dx = g f'(x), times `up` where GATED, and dup = g f(x).
 template <int KIND, bool GATED, class T>
 __global__ __launch_bounds__(256) void nz_fp8_activation_grad_kernel(const T* g, uint64_t stride, uint32_t cols,
-                                                                     uint64_t waves, uint32_t groups,
+                                                                     uint32_t waves, Groups groups,
                                                                      const uint8_t* x_data, const uint8_t* x_scales,
                                                                      const uint8_t* up_data, const uint8_t* up_scales,
                                                                      T* dx, T* dup) {
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  const uint32_t wave = blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
-  const uint64_t row = wave / groups;
-  const uint32_t at = (uint32_t)(wave - row * groups) * kGroup + (threadIdx.x & 63) * 8;
+  const Place p = place_of(wave, groups);
+  const uint64_t row = p.row;
+  const uint32_t at = p.at;
   if (at >= cols) return;
   const uint32_t n = cols - at, filled = (cols + kStep - 1) / kStep * kStep;
-  const uint64_t code = row * filled + at, scale = row * (groups * 4ull) + at / kStep;
+  const uint64_t code = row * filled + at, scale = row * (groups.count * 4ull) + at / kStep;
   float v[8], u[8], d[8], a[8], b[8];
   load8_upto(g + row * stride + at, n, d);
   values8(*reinterpret_cast<const uint2*>(x_data + code), down_factor(x_scales[scale]), v);
@@ -221,10 +257,10 @@ __global__ __launch_bounds__(256) void nz_fp8_activation_grad_kernel(const T* g,
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float slope;
-    const float p = gate<KIND, std::is_same<T, float>::value, true>(v[i], slope);
+    const float f = gate<KIND, std::is_same<T, float>::value, true>(v[i], slope);
     if constexpr (GATED) {
       a[i] = d[i] * u[i] * slope;
-      b[i] = d[i] * (v[i] * p);
+      b[i] = d[i] * (v[i] * f);
     } else {
       a[i] = d[i] * slope;
     }
@@ -734,17 +770,17 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
 // What 8 bits of float32 rows stand for, as bf16 numbers, rows filled up to whole steps: the rows' side of a product
 // with a float32 result.
 __global__ __launch_bounds__(256) void nz_fp8_rounded_kernel(const float* x, uint64_t stride, uint32_t cols,
-                                                             uint64_t waves, uint32_t groups, nz_bf16* out) {
-  const uint64_t wave = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64;
+                                                             uint32_t waves, Groups groups, nz_bf16* out) {
+  const uint32_t wave = blockIdx.x * 4 + threadIdx.x / 64;
   if (wave >= waves) return;
-  const uint64_t row = wave / groups;
-  const uint32_t at = (uint32_t)(wave - row * groups) * kGroup + (threadIdx.x & 63) * 8;
+  const Place p = place_of(wave, groups);
+  const uint32_t at = p.at;
   float v[8];
-  load8_upto(x + row * stride + at, at < cols ? cols - at : 0, v);
+  load8_upto(x + p.row * stride + at, at < cols ? cols - at : 0, v);
   const uint32_t s = block_scale(v);
   values8(codes8(v, up_factor(s)), down_factor(s), v);
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
-  if (at < filled) store8(out + row * filled + at, v);
+  if (at < filled) store8(out + p.row * filled + at, v);
 }
 
 // Which product: x wT (a float32 result), g w (the gradient of the rows), gT x (the gradient of a weight).
@@ -1010,6 +1046,16 @@ int check_groups(uint64_t rows, uint64_t groups) {
   return nz_mul(rows, groups) <= 1ull << 33 ? NZ_OK : nz_fail(NZ_ERR_ARG, "too many rows");
 }
 
+Groups groups_of(uint64_t cols) {
+  Groups g;
+  g.count = (uint32_t)nz_ceil_div(cols, kGroup);
+  uint32_t up = 0;  // 2^up is d at least
+  while ((1ull << up) < g.count) ++up;
+  g.shift = 26 + up;
+  g.mul = (uint32_t)((1ull << g.shift) / g.count + 1);
+  return g;
+}
+
 int check_fp8(const void* data, const void* scales) {
   if (!data || !scales) return nz_fail(NZ_ERR_ARG, "null data or scales");
   if (!aligned(data, 16) || !aligned(scales, 16))
@@ -1029,14 +1075,15 @@ int check_rows(uint64_t rows, uint64_t cols) {
 
 int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint64_t stride, int block_rows,
                     void* data, void* scales, hipStream_t st) {
-  const uint32_t groups = (cols + kGroup - 1) / kGroup, blocks = (cols + kStep - 1) / kStep;
+  const Groups g = groups_of(cols);
+  const uint32_t groups = g.count, blocks = (cols + kStep - 1) / kStep;
   if (block_rows == 1) {
     nz_in_pieces(rows, groups * 64ull, [&](uint64_t first, uint64_t count) {
       const uint64_t waves = count * groups;
       by_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         nz_fp8_quantize_kernel<T><<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
-            (const T*)x + first * stride, stride, cols, waves, groups, (uint8_t*)data + first * filled(cols),
+            (const T*)x + first * stride, stride, cols, (uint32_t)waves, g, (uint8_t*)data + first * filled(cols),
             (uint8_t*)scales + first * groups * 4);
       });
     });
@@ -1055,9 +1102,9 @@ int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint
 
 int launch_values(const void* data, const void* scales, uint32_t shift, uint64_t rows, uint64_t cols, void* out,
                   int dtype, hipStream_t st) {
-  const uint32_t groups = (uint32_t)nz_ceil_div(cols, kGroup);
-  nz_in_pieces(rows, groups * 64ull, [&](uint64_t first, uint64_t count) {
-    const uint64_t waves = count * groups;
+  const Groups groups = groups_of(cols);
+  nz_in_pieces(rows, groups.count * 64ull, [&](uint64_t first, uint64_t count) {
+    const uint32_t waves = (uint32_t)(count * groups.count);
     by_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       nz_fp8_values_kernel<T><<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
@@ -1075,7 +1122,7 @@ constexpr Tile kTiles[] = {{256, 256, 256, 1.31f, 0.94f, 4.0f, true},
                            {128, 256, 256, 0.72f, 0.74f, 3.2f},
                            {128, 128, 512, 0.78f, 0.76f, 2.4f},
                            {64, 128, 256, 0.30f, 0.28f, 1.1f},
-                           {64, 64, 256, 0.21f, 0.13f, 0.8f}};
+                           {64, 64, 256, 0.21f, 0.15f, 0.8f}};
 // Products of 16-bit rows, 64 values a step.
 constexpr Tile kTiles16[] = {{256, 128, 256, 0.95f, 0.86f}, {64, 64, 256, 0.31f, 0.31f}};
 
@@ -1350,10 +1397,11 @@ int nz_fp8_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t
   }
   uint8_t* base = (uint8_t*)dev_workspace;
   if (dtype == NZ_DTYPE_F32 && !few_rows(m, n, k, dtype)) {
-    const uint64_t groups = nz_ceil_div(k, kGroup);
-    nz_in_pieces(m, groups * 64, [&](uint64_t first, uint64_t count) {
-      nz_fp8_rounded_kernel<<<(uint32_t)nz_ceil_div(count * groups, 4), 256, 0, st>>>(
-          (const float*)dev_x + first * stride, stride, (uint32_t)k, count * groups, (uint32_t)groups,
+    const Groups groups = groups_of(k);
+    nz_in_pieces(m, groups.count * 64ull, [&](uint64_t first, uint64_t count) {
+      const uint32_t waves = (uint32_t)(count * groups.count);
+      nz_fp8_rounded_kernel<<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
+          (const float*)dev_x + first * stride, stride, (uint32_t)k, waves, groups,
           (nz_bf16*)(base + room.values) + first * filled(k));
     });
     return launch_wide(m, w, dev_bias, dev_y, room, base, st);
@@ -1448,9 +1496,10 @@ int nz_fp8_activation(int kind, const void* dev_x, int dtype, uint64_t rows, uin
   if (keep && dev_up)
     if (int rc = check_fp8(dev_up_data, dev_up_scales)) return rc;
   const hipStream_t st = (hipStream_t)stream;
-  const uint32_t groups = (uint32_t)nz_ceil_div(cols, kGroup);
-  nz_in_pieces(rows, groups * 64ull, [&](uint64_t first, uint64_t count) {
-    const uint64_t waves = count * groups, d = first * filled(cols), s = first * groups * 4;
+  const Groups groups = groups_of(cols);
+  nz_in_pieces(rows, groups.count * 64ull, [&](uint64_t first, uint64_t count) {
+    const uint32_t waves = (uint32_t)(count * groups.count);
+    const uint64_t d = first * filled(cols), s = first * groups.count * 4;
     by_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       by_kind(kind, dev_up != nullptr, [&](auto k, auto gated) {
@@ -1480,9 +1529,10 @@ int nz_fp8_activation_grad(int kind, const void* dev_g, int dtype, uint64_t rows
     if (!dev_dup) return nz_fail(NZ_ERR_ARG, "null output");
   }
   const hipStream_t st = (hipStream_t)stream;
-  const uint32_t groups = (uint32_t)nz_ceil_div(cols, kGroup);
-  nz_in_pieces(rows, groups * 64ull, [&](uint64_t first, uint64_t count) {
-    const uint64_t waves = count * groups, d = first * filled(cols), s = first * groups * 4;
+  const Groups groups = groups_of(cols);
+  nz_in_pieces(rows, groups.count * 64ull, [&](uint64_t first, uint64_t count) {
+    const uint32_t waves = (uint32_t)(count * groups.count);
+    const uint64_t d = first * filled(cols), s = first * groups.count * 4;
     by_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       by_kind(kind, dev_up_data != nullptr, [&](auto k, auto gated) {
