@@ -42,6 +42,16 @@ __device__ inline uint32_t block_scale(float (&v)[8]) {
   return s;
 }
 
+// Values of 8 codes.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
+__device__ inline void values_of(uint2 codes, uint32_t s, float (&v)[8]) {
+  const float scale = __uint_as_float(s << 23);
+  const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.x, scale, false);
+  const f2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.x, scale, true);
+  const f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.y, scale, false);
+  const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.y, scale, true);
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+}
+
 // ---- quantisation and values -----------------------------------------------------------------------------------
 //
 // One wavefront per 512 values of a row: 8 values a lane, 16 lanes a block.
@@ -142,8 +152,8 @@ __global__ __launch_bounds__(256) void nz_fp8_values_kernel(const uint8_t* data,
   if (at >= cols) return;
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
   float v[8];
-  values8(*reinterpret_cast<const uint2*>(data + row * filled + at),
-          down_factor(scales[(row >> shift) * (groups.count * 4ull) + at / kStep]), v);
+  values_of(*reinterpret_cast<const uint2*>(data + row * filled + at),
+            scales[(row >> shift) * (groups.count * 4ull) + at / kStep], v);
   store8_upto(out + row * cols + at, cols - at, v);
 }
 
@@ -252,8 +262,8 @@ __global__ __launch_bounds__(256) void nz_fp8_activation_grad_kernel(const T* g,
   const uint64_t code = row * filled + at, scale = row * (groups.count * 4ull) + at / kStep;
   float v[8], u[8], d[8], a[8], b[8];
   load8_upto(g + row * stride + at, n, d);
-  values8(*reinterpret_cast<const uint2*>(x_data + code), down_factor(x_scales[scale]), v);
-  if constexpr (GATED) values8(*reinterpret_cast<const uint2*>(up_data + code), down_factor(up_scales[scale]), u);
+  values_of(*reinterpret_cast<const uint2*>(x_data + code), x_scales[scale], v);
+  if constexpr (GATED) values_of(*reinterpret_cast<const uint2*>(up_data + code), up_scales[scale], u);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float slope;
@@ -290,7 +300,7 @@ __device__ inline f4 step(i4v w0, i4v w1, i4v x0, i4v x1, f4 acc, uint32_t sw, u
   }
 }
 
-// 8 codes as bf16 numbers.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
+// 8 codes as bf16 numbers, by such a conversion too.
 __device__ inline b8v bf16_of_codes(uint2 codes, uint32_t s) {
   const float scale = __uint_as_float(s << 23);
   const b2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.x, scale, false);
@@ -778,7 +788,7 @@ __global__ __launch_bounds__(256) void nz_fp8_rounded_kernel(const float* x, uin
   float v[8];
   load8_upto(x + p.row * stride + at, at < cols ? cols - at : 0, v);
   const uint32_t s = block_scale(v);
-  values8(codes8(v, up_factor(s)), down_factor(s), v);
+  values_of(codes8(v, up_factor(s)), s, v);
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
   if (at < filled) store8(out + p.row * filled + at, v);
 }
