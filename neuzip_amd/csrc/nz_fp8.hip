@@ -654,13 +654,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
 // Up to 16 rows, where reading the weight is all that counts: no staging and no barrier in the way of it.  The eight
 // wavefronts are kw that share the values of a row (512 at a time, in turn) times 8 / kw with 16 weight rows each;
-// a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits, or
-// (QUANTIZE) as they are: then every workgroup brings them to 8 bits in LDS while its first weights are on their way.
+// a lane loads its operand of the matrix instruction straight from memory.  The rows come in 8 bits (N = 0), or
+// as they are, at most 8 N groups of 512 values: then every workgroup brings them to 8 bits in LDS while its first weights
+// are on their way.
 // Results in float32 are summed by bf16 instructions (why, see `step`), for which a lane takes both sides to bf16: of
 // the 128 values of a step those it holds, 8 at a time (both sides in the same order, which is all that counts).
 constexpr uint32_t kHeld = 528;  // bytes of 512 values of a row and their scales in LDS
 
-template <bool QUANTIZE, class T>
+template <int N, class T>
 __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t stride, const uint8_t* xs, uint32_t m,
                                                          const uint8_t* wd, const uint8_t* ws, uint32_t shift,
                                                          uint32_t n, uint32_t k, const T* bias, T* y, uint32_t kw) {
@@ -688,33 +689,28 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
   constexpr bool kWide = std::is_same<T, float>::value;
   const uint32_t row = min(r, m - 1);
   const uint8_t *xp, *xsp;
-  if constexpr (QUANTIZE) {
+  if constexpr (N > 0) {
     const T* xt = (const T*)x;
-    const auto quantise = [&](uint32_t i, auto size) {  // every eighth from i on, all on their way at once
-      constexpr uint32_t N = decltype(size)::value;
-      typename Pack<T>::type raw[N];
+    typename Pack<T>::type raw[N];  // every eighth group of values of a wavefront, all on their way at once
 #pragma unroll
-      for (uint32_t j = 0; j < N; ++j) {
-        const uint32_t to = (i + 8 * j) / groups, at = (i + 8 * j - to * groups) * kGroup + lane * 8;
-        raw[j] = {};
-        if (at + 8 <= k) raw[j] = *(const typename Pack<T>::type*)(xt + to * stride + at);
-      }
+    for (uint32_t j = 0; j < N; ++j) {
+      const uint32_t i = wave + 8 * j, to = i / groups, at = (i - to * groups) * kGroup + lane * 8;
+      raw[j] = {};
+      if (i < m * groups && at + 8 <= k) raw[j] = *(const typename Pack<T>::type*)(xt + to * stride + at);
+    }
 #pragma unroll
-      for (uint32_t j = 0; j < N; ++j) {
-        const uint32_t to = (i + 8 * j) / groups, at = (i + 8 * j - to * groups) * kGroup + lane * 8;
-        float v[8];
+    for (uint32_t j = 0; j < N; ++j) {
+      const uint32_t i = wave + 8 * j, to = i / groups, at = (i - to * groups) * kGroup + lane * 8;
+      if (i >= m * groups) break;
+      float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (float)raw[j][e];
-        if (at < k && at + 8 > k) load8_upto(xt + to * stride + at, k - at, v);
-        const uint32_t s = block_scale(v);
-        uint8_t* q = few_lds + (i + 8 * j) * kHeld;
-        *(uint2*)(q + lane * 8) = codes8(v, up_factor(s));
-        if ((lane & 15) == 0) q[kGroup + lane / 16] = (uint8_t)s;
-      }
-    };
-    uint32_t i = wave;
-    for (; i + 24 < m * groups; i += 32) quantise(i, std::integral_constant<uint32_t, 4>());
-    for (; i < m * groups; i += 8) quantise(i, std::integral_constant<uint32_t, 1>());
+      for (int e = 0; e < 8; ++e) v[e] = (float)raw[j][e];
+      if (at < k && at + 8 > k) load8_upto(xt + to * stride + at, k - at, v);
+      const uint32_t s = block_scale(v);
+      uint8_t* q = few_lds + i * kHeld;
+      *(uint2*)(q + lane * 8) = codes8(v, up_factor(s));
+      if ((lane & 15) == 0) q[kGroup + lane / 16] = (uint8_t)s;
+    }
     __syncthreads();
     xp = few_lds + row * groups * kHeld + g * 16;
     xsp = few_lds + row * groups * kHeld + kGroup;
@@ -724,11 +720,11 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
   }
   f4 acc = {0, 0, 0, 0};
   const auto multiply = [&](const Held& h, uint32_t group) {
-    const uint32_t sx = *(const uint32_t*)(xsp + group * (QUANTIZE ? kHeld : 4));
+    const uint32_t sx = *(const uint32_t*)(xsp + group * (N ? kHeld : 4));
     const auto one = [&](auto b4) {
       constexpr int i = decltype(b4)::value;
       if (group * 4 + i >= steps) return;
-      const uint8_t* p = xp + (QUANTIZE ? group * kHeld : (uint64_t)group * 512) + i * 128;
+      const uint8_t* p = xp + (N ? group * kHeld : (uint64_t)group * 512) + i * 128;
       const i4v x0 = *(const i4v*)p, x1 = *(const i4v*)(p + 64);
       if constexpr (kWide) {
         const uint32_t s = sx >> (8 * i) & 255, sw = h.s >> (8 * i) & 255;
@@ -1217,7 +1213,7 @@ bool few_rows(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   return few_inside(m, n, k, dtype) || (m <= 16 && (n * k <= 1ull << 25 || dtype == NZ_DTYPE_F32));
 }
 
-template <bool QUANTIZE, class T>
+template <int N, class T>
 void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, const void* wd, const void* ws,
                 uint32_t shift, uint64_t n, uint32_t k, const T* bias, T* y, hipStream_t st) {
   const uint32_t groups = (k + kGroup - 1) / kGroup;
@@ -1225,8 +1221,8 @@ void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, cons
   const uint64_t t = nz_ceil_div(n, 16);
   const uint32_t cus = nz_compute_units();
   if (t > 2 * (cus ? cus : 256)) kw = kw < 4 ? kw : m >= 4 ? 2 : 4;
-  const uint32_t lds = QUANTIZE ? (uint32_t)m * groups * kHeld : 0;
-  nz_fp8_few_kernel<QUANTIZE, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
+  const uint32_t lds = N ? (uint32_t)m * groups * kHeld : 0;
+  nz_fp8_few_kernel<N, T><<<(uint32_t)nz_ceil_div(t, 8 / kw), 512, lds > 8192 ? lds : 8192, st>>>(
       x, stride, (const uint8_t*)xs, (uint32_t)m, (const uint8_t*)wd, (const uint8_t*)ws, shift, (uint32_t)n, k, bias,
       y, kw);
 }
@@ -1271,7 +1267,7 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const Held8& w, c
   if (few_rows(m, n, k, dtype)) {
     by_dtype(dtype, [&](auto t) {
       using T = decltype(t);
-      launch_few<false>(xd, 0, xs, m, w.data, w.scales, w.shift, n, k, (const T*)bias, (T*)y, st);
+      launch_few<0>(xd, 0, xs, m, w.data, w.scales, w.shift, n, k, (const T*)bias, (T*)y, st);
     });
     return nz_launched();
   }
@@ -1400,8 +1396,17 @@ int nz_fp8_linear(const void* dev_x, int dtype, uint64_t m, uint64_t k, uint64_t
   if (few_inside(m, n, k, dtype)) {
     by_dtype(dtype, [&](auto t) {
       using T = decltype(t);
-      launch_few<true>(dev_x, stride, nullptr, m, w.data, w.scales, w.shift, n, (uint32_t)k, (const T*)dev_bias,
-                       (T*)dev_y, st);
+      const auto launch = [&](auto held) {
+        launch_few<decltype(held)::value>(dev_x, stride, nullptr, m, w.data, w.scales, w.shift, n, (uint32_t)k,
+                                          (const T*)dev_bias, (T*)dev_y, st);
+      };
+      const uint64_t groups = m * nz_ceil_div(k, kGroup);
+      if (groups <= 8)
+        launch(std::integral_constant<int, 1>());
+      else if (groups <= 32)
+        launch(std::integral_constant<int, 4>());
+      else
+        launch(std::integral_constant<int, 8>());
     });
     return nz_launched();
   }
