@@ -822,33 +822,37 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   uint32_t tm, tn;
   tile_of(blockIdx.x, mt, nt, tm, tn);
   const uint32_t m0 = tm * BM, n0 = tn * BN, m_last = min((uint32_t)BM, m - m0) - 1;
-  const uint32_t last_rows = b_rows - (steps_1 - 1) * 64;  // ROWS: of the last step of a plane
+  // ROWS: the last step of a plane may have fewer than 64 rows of its own.  TURN: it begins earlier, so that it has 64, of
+  // which those that the step before had count as zeros.
+  const uint32_t last_rows = b_rows - (steps_1 - 1) * 64, last_at = b_rows > 64 ? b_rows - 64 : 0;
 
-  // Loads: a base of the workgroup, moved from step to step, and an offset of the lane.  The last rows along the summed
-  // axis have offsets of their own, so that none behind the last is read.
+  // Loads: a base of the workgroup, moved from step to step, and an offset of the lane.
   const auto turned = [](uint32_t row) { return ((row & 3) | (row >> 1 & 4)) * 2 % (BM / 8); };
   const uint8_t* ab = (const uint8_t*)a;
   if constexpr (!TURN) ab += (uint64_t)m0 * a_stride * 2 + from * 128ull;
-  uint32_t ao[XI], ao_last[XI];
+  uint32_t ao[XI];
 #pragma unroll
   for (int i = 0; i < XI; ++i) {
     if constexpr (TURN) {
       const uint32_t id = (wave * XI + i) * 64 + lane, row = id / (BM / 8), c = id % (BM / 8) ^ turned(row);
       const uint32_t col = min(m0 + c * 8, a_width - 8);
-      ao[i] = (row * (uint32_t)a_stride + col) * 2;
-      ao_last[i] = (min(row, last_rows - 1) * (uint32_t)a_stride + col) * 2;
+      ao[i] = (min(row, b_rows - 1) * (uint32_t)a_stride + col) * 2;
     } else {
       ao[i] = min((wave * XI + i) * 8 + lane / 8, m_last) * (uint32_t)(a_stride * 2) + ((lane & 7) ^ (lane / 8)) * 16;
     }
   }
-  uint32_t a_step = from % steps_1, a_at = from / steps_1;  // TURN: of the stage that is loaded next, its plane
+  uint32_t a_step = from % steps_1, plane = from / steps_1;  // TURN: of the stage that is loaded next
+  const auto a_base = [&]() { return ab + (plane * a_plane + min(a_step * 64, last_at) * a_stride) * 2; };
+  const uint8_t* a_at = TURN ? a_base() : nullptr;
   const auto load_a = [&](uint32_t s, uint32_t buf, int i) {  // the i-th of XI
     const uint32_t to = base + buf * AB + (wave * XI + i) * 1024;
     // past the end the last stage is loaded again, into a buffer that is not read
     if constexpr (TURN) {
-      to_lds16(ab + (a_at * a_plane + a_step * 64ull * a_stride) * 2, a_step + 1 == steps_1 ? ao_last[i] : ao[i], to);
+      to_lds16(a_at, ao[i], to);
       if (i == XI - 1 && s + 1 < steps) {
-        if (++a_step == steps_1) a_step = 0, ++a_at;
+        const bool turn = a_step + 1 == steps_1;
+        a_step = turn ? 0 : a_step + 1, plane += turn;
+        a_at = a_base();
       }
     } else {
       to_lds16(ab + min(s, steps - 1) * 128ull, ao[i], to);
@@ -864,8 +868,10 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
     const uint32_t s_row = wave * OWN + min(lane, OWN - 1u);
     if constexpr (ROWS) {
       const uint32_t chunk = min(n0 / 16 + c, b_steps * 8 - 1), group = n0 / kGroup * 4;
-      co = row * b_bytes + chunk * 16, co_last = min(row, last_rows - 1) * b_bytes + chunk * 16;
-      so = (s_row >> shift) * pitch + group, so_last = (min(s_row, last_rows - 1) >> shift) * pitch + group;
+      const uint32_t end = TURN ? b_rows : last_rows;
+      co = (TURN ? min(row, end - 1) : row) * b_bytes + chunk * 16, co_last = min(row, end - 1) * b_bytes + chunk * 16;
+      so = (s_row >> shift) * pitch + group, so_last = (min(s_row, end - 1) >> shift) * pitch + group;
+      if constexpr (TURN) so = min(s_row, end - 1), so_last = group;
     } else {
       const auto place = [&](uint32_t id) {
         const uint32_t col = id / (TN * 16) * (TN * 16) + id % 16 / 4 * (TN * 4) + id / 16 % TN * 4 + id % 4;
@@ -878,12 +884,14 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   }
   uint32_t w_step = from % steps_1;  // of the codes that are loaded next
   const auto load_b = [&](uint32_t buf) {
+    const uint32_t row = TURN ? min(w_step * 64, last_at) : w_step * 64;
+    const uint8_t* c = bd + (ROWS ? (uint64_t)row * b_bytes : w_step * 64ull);
+    // steps begin at multiples of 64, so with a scale for 128 rows all of one have the same; TURN: not the last
+    const uint8_t* s = bs + (ROWS ? (uint64_t)(row >> shift) * pitch : w_step / 8 * 4ull);
     const bool last = ROWS && w_step + 1 == steps_1;
-    const uint8_t* c = bd + (ROWS ? (uint64_t)w_step * 64 * b_bytes : w_step * 64ull);
-    // with a scale for 128 rows, steps 2 i and 2 i + 1 have the same
-    const uint8_t* s = bs + (ROWS ? (uint64_t)(w_step * 64 >> shift) * pitch : w_step / 8 * 4ull);
-    to_lds16(c, last ? co_last : co, base + C_AT + buf * CB + wave * 1024);
-    to_lds4(s, last ? so_last : so, base + S_AT + buf * SB + wave * 256);
+    to_lds16(c, !TURN && last ? co_last : co, base + C_AT + buf * CB + wave * 1024);
+    to_lds4(s, TURN ? (((row + so) >> shift) - (row >> shift)) * pitch + so_last : last ? so_last : so,
+            base + S_AT + buf * SB + wave * 256);
     w_step = w_step + 1 == steps_1 ? 0 : w_step + 1;
   };
   // To bf16: 16 codes of a lane, neighbours' from eight rows.  Rows exchange 16-byte pieces (piece c of row r at
@@ -907,12 +915,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
         bf16_of_codes(swap ? make_uint2(codes.w, codes.z) : make_uint2(codes.z, codes.w), scale);
     c_step = c_step + 1 == steps_1 ? 0 : c_step + 1;
   };
-  // TURN: rows of A behind the last of a plane were read as the last; they count as zeros.
+  // TURN: rows of A that a plane's last step has once more count as zeros.
   uint32_t z_step = from % steps_1;  // of the rows that are looked at next
   const auto clear = [&](uint32_t buf) {
     if constexpr (TURN) {
       if (z_step + 1 == steps_1 && last_rows < 64) {
-        for (uint32_t at = last_rows * (BM * 2) + threadIdx.x * 16; at < AB; at += 64 * W * 16)
+        const uint32_t begin = b_rows < 64 ? b_rows : 0, end = b_rows < 64 ? 64 : 64 - last_rows;
+        for (uint32_t at = begin * (BM * 2) + threadIdx.x * 16; at < end * (BM * 2); at += 64 * W * 16)
           *(i4v*)(lds + buf * AB + at) = i4v{0, 0, 0, 0};
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         block_barrier();
