@@ -1046,7 +1046,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   }
   if (s < steps) body(s, std::integral_constant<uint32_t, 0>());
   wait_loads<0>();  // nothing may arrive in this memory once it is another workgroup's
-  finish_tile<WM, WN, TM, TN, S_AT + 3 * SB, ADD>(acc, lds, m, cols, m0, n0, bias, y, part);
+  finish_tile<WM, WN, TM, TN, S_AT + 3 * SB, ADD, true>(acc, lds, m, cols, m0, n0, bias, y, part);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------

@@ -137,32 +137,15 @@ __device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& 
 // Add the bias (ADD: what y holds) to a workgroup's tile and store it, or store it as it is among the parts.  A lane (r, g) of wavefront
 // (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], 4 TN consecutive columns.
 //
-// The tile goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold
+// The tile (PARTS_TOO: one of the parts as well) goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold
 // pieces of 16 rows, 8192 x (4096x1024) takes 53 us in tiles of 128x256 instead of 37, 8192 x (14336x4096) 434 instead
 // of 409. (In tiles of 128x128 39 instead of 37 and 462 instead of 466.)
-template <int WM, int WN, int TM, int TN, int LDS, bool ADD = false, class T>
-__device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
-                                   const T* bias, T* y, float* part) {
+template <int WM, int WN, int TM, int TN, int LDS, bool ADD, class T>
+__device__ inline void store_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+                                  const T* bias, T* y) {
   constexpr int W = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
   const uint32_t wm = wave % WM, wn = wave / WM, c0 = wn * TN * 16 + g * TN * 4;
-  if (part) {
-    part += (uint64_t)blockIdx.y * m * n;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const uint32_t row = m0 + (wm * TM + i) * 16 + r;
-      if (row >= m) break;
-#pragma unroll
-      for (int j = 0; j < TN; j += 2) {
-        const uint32_t c = n0 + c0 + j * 4;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[i][j + e / 4][e % 4];
-        if (c < n) store8_upto(part + (uint64_t)row * n + c, n - c, v);
-      }
-    }
-    return;
-  }
   constexpr int PITCH = BN * sizeof(T) + 16;  // eight lanes in turn write to all banks
   static_assert(BM * PITCH <= LDS, "a tile of the result");
   block_barrier();
@@ -200,6 +183,35 @@ __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, 
       for (int e = 0; e < V; ++e)
         if (n0 + c + e < n) q[e] = v[e];
   }
+}
+
+template <int WM, int WN, int TM, int TN, int LDS, bool ADD = false, bool PARTS_TOO = false, class T>
+__device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
+                                   const T* bias, T* y, float* part) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, r = lane & 15, g = lane / 16;
+  const uint32_t wm = wave % WM, wn = wave / WM, c0 = wn * TN * 16 + g * TN * 4;
+  if (part) {
+    part += (uint64_t)blockIdx.y * m * n;
+    if constexpr (PARTS_TOO) {
+      store_tile<WM, WN, TM, TN, LDS, false>(acc, lds, m, n, m0, n0, (const float*)nullptr, part);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const uint32_t row = m0 + (wm * TM + i) * 16 + r;
+      if (row >= m) break;
+#pragma unroll
+      for (int j = 0; j < TN; j += 2) {
+        const uint32_t c = n0 + c0 + j * 4;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][j + e / 4][e % 4];
+        if (c < n) store8_upto(part + (uint64_t)row * n + c, n - c, v);
+      }
+    }
+    return;
+  }
+  store_tile<WM, WN, TM, TN, LDS, ADD>(acc, lds, m, n, m0, n0, bias, y);
 }
 
 // The parts of a product whose rows were cut, added in their order (ADD: to what y holds).
