@@ -560,7 +560,7 @@ int nz_fp8_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64
 /* dx[m][k] = sum_n g[m][n] w[n][k]: the gradient of that product's rows (their rounding to 8 bits is passed straight
    through), in 32 bits.  n is 1 at least. */
 uint64_t nz_fp8_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
-                                            uint64_t k);
+                                            uint64_t k, int block_rows);
 int nz_fp8_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
                        const void* dev_w_scales, uint64_t k, int block_rows, void* dev_dx, void* dev_workspace,
                        uint64_t workspace_bytes, void* stream);

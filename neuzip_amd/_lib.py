@@ -186,7 +186,7 @@ def load() -> ctypes.CDLL:
     L.nz_fp8_linear_rows8.restype = i32
     L.nz_fp8_linear_rows8.argtypes = [vp, vp, u64, u64, vp, vp, u64, i32, vp, vp, i32, vp, u64, vp]
     L.nz_fp8_linear_grad_workspace_bytes.restype = u64
-    L.nz_fp8_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64]
+    L.nz_fp8_linear_grad_workspace_bytes.argtypes = [vp, i32, u64, u64, u64, u64, i32]
     L.nz_fp8_linear_grad.restype = i32
     L.nz_fp8_linear_grad.argtypes = [vp, i32, u64, u64, u64, vp, vp, u64, i32, vp, vp, u64, vp]
     L.nz_fp8_weight_grad_workspace_bytes.restype = u64

@@ -1049,6 +1049,204 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   finish_tile<WM, WN, TM, TN, S_AT + 3 * SB, ADD, true>(acc, lds, m, cols, m0, n0, bias, y, part);
 }
 
+// `mfma` of bf16 in assembly, as step_in_place.
+__device__ inline void step16_in_place(b8v b, b8v a, f4& acc) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(b), "v"(a));
+}
+
+// The gradient of the rows where 128 rows of the weight share a scale: tiles of 256 x 32 TN, four wavefronts of 128 x
+// 16 TN each, a compute unit's own.
+//
+// What bounds the kernel above is LDS: its wavefronts' tiles of 64x64 read 128 KB a step, and the codes pass it twice
+// more, 40 % of its time in addition to the rows' way in.  Here a wavefront's tile is as large as its registers allow
+// (96 KB a step of 256x128, 128 KB of 256x256), and codes are read as they are, eight of a column by the instruction that
+// transposes 8 x 16 bytes on the way, and converted in the wavefront that multiplies them: a step has one scale.
+//
+// Steps of 64 values in two halves, whose operands are read while the other half's are multiplied.  In the middle is the
+// step's barrier: the next step has arrived and this one has been read, so that the third behind it goes there, two steps
+// ahead of its use.
+template <int TN, class T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void nz_fp8_input_kernel(
+    const nz_bf16* a, uint64_t a_stride, uint32_t m, const uint8_t* bd, const uint8_t* bs, uint32_t b_rows,
+    uint32_t b_cols, uint32_t steps_1, uint32_t planes, T* y, uint32_t mt, uint32_t nt, uint32_t part_steps,
+    float* part) {
+  constexpr int TM = 8, BM = 256, BN = TN * 32, M = TM * TN, CI = TN / 2;
+  constexpr int AB = BM * 128, CB = BN * 64, S_AT = AB + CB, STAGE = S_AT + 1024, NS = 3, LOADS = 8 + CI + 1;
+  static_assert(NS * STAGE <= 160 * 1024, "LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE];
+  const uint32_t base = lds_address(lds);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t r = lane & 15, g = lane / 16, wm = wave & 1, wn = wave / 2;
+  const uint32_t from = blockIdx.y * part_steps, steps = min(steps_1 * planes - from, part_steps);
+  const uint32_t b_bytes = (b_cols + kStep - 1) / kStep * 128, pitch = (b_cols + kGroup - 1) / kGroup * 4;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, mt, nt, tm, tn);
+  const uint32_t m0 = tm * BM, n0 = tn * BN;
+
+  // Loads: a base of the workgroup, moved from step to step, and offsets of the lane.  Rows and columns behind the last
+  // are read as that; the last rows along the summed axis, beside which A has zeros, have offsets of their own.  16-byte
+  // chunk c of a row of A lies at c ^ (row & 7), of a row of codes at c ^ mixed(row): what 32 lanes read is in all banks.
+  const auto mixed = [](uint32_t row) { return BN == 256 ? row & 15 : row >> 1 & 7; };
+  const uint8_t* ab = (const uint8_t*)a + (uint64_t)m0 * a_stride * 2 + from * 128ull;
+  uint32_t ao[8], co[CI], co_last[CI];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t row = min((wave * 8 + i) * 8 + lane / 8, m - m0 - 1);
+    ao[i] = row * (uint32_t)(a_stride * 2) + ((lane & 7) ^ (lane / 8)) * 16;
+  }
+  const uint32_t last_rows = b_rows - (steps_1 - 1) * 64;
+#pragma unroll
+  for (int i = 0; i < CI; ++i) {
+    const uint32_t id = (wave * CI + i) * 64 + lane, row = id / (BN / 16), c = id % (BN / 16) ^ mixed(row);
+    const uint32_t at = min(n0 + c * 16, b_bytes - 16);
+    co[i] = row * b_bytes + at, co_last[i] = min(row, last_rows - 1) * b_bytes + at;
+  }
+  // the block of columns that the wavefront has, among four of which a load takes the scales
+  const uint32_t block = min((n0 + wn * TN * 16) / kStep, pitch - 1);
+  uint32_t left = steps, b_step = from % steps_1;
+  const auto load = [&](uint32_t at, int i) {  // the i-th of LOADS; `at`: the stage's place in LDS
+    if (i < 8) {
+      to_lds16(ab, ao[i], base + at + (wave * 8 + i) * 1024);
+    } else if (i < 8 + CI) {
+      to_lds16(bd + (uint64_t)b_step * 64 * b_bytes, b_step + 1 == steps_1 ? co_last[i - 8] : co[i - 8],
+               base + at + AB + (wave * CI + i - 8) * 1024);
+    } else {
+      to_lds4(bs + (uint64_t)(b_step / 2) * pitch + (block & ~3u), 0, base + at + S_AT + wave * 256);
+      const uint32_t more = left > 1;  // behind the last step it is loaded again, into a place that is not read
+      left -= more, ab += more * 128;
+      b_step = more ? (b_step + 1 == steps_1 ? 0 : b_step + 1) : b_step;
+    }
+  };
+
+  uint32_t ra[2], rc[TN];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) ra[h] = (wm * 128 + r) * 128 + ((h * 4 + g) ^ (r & 7)) * 16;
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const uint32_t row = g * 8 + r / 2;
+    rc[j] = base + AB + row * BN + (wn * TN + j ^ mixed(row)) * 16 + r % 2 * 8;
+  }
+  b8v x[2][TM], w[2][TN];
+  typedef int i2v __attribute__((ext_vector_type(2)));
+  i2v codes[TN];
+  uint32_t scale;
+  const auto read_x = [&](uint32_t at, int h, int i) { x[h][i] = *(const b8v*)(lds + at + ra[h] + i * 2048); };
+  const auto read_codes = [&](uint32_t at, int h, int j) {
+    codes[j] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (__attribute__((address_space(3))) i2v*)(uintptr_t)(rc[j] + at + h * 32 * BN));
+  };
+  const auto read_scale = [&](uint32_t at) {
+    scale = *(const uint32_t*)(lds + at + S_AT + wave * 256) >> (block & 3) * 8 & 255;
+  };
+  const auto convert = [&](int h, int j) {
+    w[h][j] = bf16_of_codes(make_uint2((uint32_t)codes[j].x, (uint32_t)codes[j].y), scale);
+  };
+
+  f4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      acc[i][j] = f4{0, 0, 0, 0};
+      asm volatile("" : "+a"(acc[i][j]));
+    }
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load(s * STAGE, i);
+  wait_loads<(NS - 1) * LOADS>();
+  block_barrier();
+  read_scale(0);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) read_codes(0, 0, j);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) read_x(0, 0, i);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) convert(0, j);
+  settle();
+
+  const auto multiply = [&](int h, auto beside) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        step16_in_place(w[h][j], x[h][i], acc[i][j]);
+        beside(i * TN + j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  // half h of the stage at `at` is read beside the other's instructions: its codes first, which are converted later
+  const auto read_beside = [&](uint32_t at, int h, int t) {
+    constexpr int C = M / 2 / TN;  // instructions between two conversions
+    if (t < TN) read_codes(at, h, t);
+    if (t >= TN && t < TN + 2 * TM && (t - TN) % 2 == 0) read_x(at, h, (t - TN) / 2);
+    if (t >= M / 2 && (t - M / 2) % C == 0) convert(h, (t - M / 2) / C);
+  };
+  uint32_t at = 0;
+  for (uint32_t s = 0; s < steps; ++s) {
+    const uint32_t next = at == (NS - 1) * STAGE ? 0 : at + STAGE;
+    multiply(0, [&](int t) { read_beside(at, 1, t); });
+    // a stage is asked for in the second half of a step: one is on its way, that of the step before
+    wait_loads<LOADS>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();
+    read_scale(next);
+    multiply(1, [&](int t) {
+      read_beside(next, 0, t);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        if (i * M / LOADS == t) load(at, i);
+    });
+    at = next;
+  }
+  wait_loads<0>();  // nothing may arrive in this memory once it is used for something else
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  block_barrier();
+  settle();
+
+  // The result through a part of LDS of the wavefront's own, 16 rows at a time.
+  const uint32_t row0 = m0 + wm * 128, col0 = n0 + wn * TN * 16;
+  const auto finish = [&](auto* out) {
+    using O = std::remove_reference_t<decltype(*out)>;
+    constexpr int PITCH = TN * 16 * (int)sizeof(O) + 16, V = 16 / sizeof(O), ACROSS = TN * 16 / V;
+    static_assert(4 * 16 * PITCH <= (int)sizeof(lds), "four parts");
+    typedef O four __attribute__((ext_vector_type(4)));
+    typedef O whole __attribute__((ext_vector_type(V)));
+    typedef O piece __attribute__((ext_vector_type(V), aligned(sizeof(O))));
+    uint8_t* mine = lds + wave * 16 * PITCH;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        asm volatile("" : "+a"(acc[i][j]));  // it stays where it is until here
+        four v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (O)acc[i][j][e];
+        *(four*)(mine + r * PITCH + (j * 16 + g * 4) * sizeof(O)) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int q = 0; q < 16 * ACROSS / 64; ++q) {
+        const uint32_t id = q * 64 + lane, row = row0 + i * 16 + id / ACROSS, c = col0 + id % ACROSS * V;
+        const whole v = *(const whole*)(mine + id / ACROSS * PITCH + id % ACROSS * 16);
+        if (row >= m || c >= b_cols) continue;
+        O* p = out + (uint64_t)row * b_cols + c;
+        if (c + V <= b_cols)
+          *(piece*)p = v;
+        else
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (c + e < b_cols) p[e] = v[e];
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  if (part)
+    finish(part + (uint64_t)blockIdx.y * m * b_cols);
+  else
+    finish(y);
+}
+
 // ---- host side -------------------------------------------------------------------------------------------------
 
 uint64_t filled(uint64_t cols) { return nz_ceil_div(cols, kStep) * kStep; }
@@ -1129,9 +1327,9 @@ int launch_values(const void* data, const void* scales, uint32_t shift, uint64_t
   return nz_launched();
 }
 
-// Figures of the tiles, and of those of 16-bit rows: fitted to times of 60 products of 17 to 8192 rows with weights of 256
-// to 16384 rows and columns, each in all tiles and up to 16 parts.  The cut chosen by them takes 1.2 % more than the
-// fastest one in the mean.
+// Figures of the tiles, fitted to times of 60 products of 17 to 8192 rows with weights of 256 to 16384 rows and columns,
+// each in all tiles and up to 16 parts, and of 45 gradients of either kind.  The cut chosen by them takes 1.2 % more than
+// the fastest one in the mean (of gradients of rows 2.3 %, of a weight 0.2 %).
 // Products of 8-bit rows, 128 values a step.
 constexpr Tile kTiles[] = {{256, 256, 256, 1.31f, 0.94f, 4.0f, true},
                            {128, 256, 256, 0.72f, 0.74f, 3.2f},
@@ -1139,7 +1337,11 @@ constexpr Tile kTiles[] = {{256, 256, 256, 1.31f, 0.94f, 4.0f, true},
                            {64, 128, 256, 0.30f, 0.28f, 1.1f},
                            {64, 64, 256, 0.21f, 0.15f, 0.8f}};
 // Products of 16-bit rows, 64 values a step.
-constexpr Tile kTiles16[] = {{256, 128, 256, 0.95f, 0.86f}, {64, 64, 256, 0.31f, 0.31f}};
+constexpr Tile kTiles16[] = {{256, 128, 256, 0.86f, 0.94f, 0.9f}, {64, 64, 256, 0.40f, 0.44f, 0.5f}};
+// The gradient of the rows where 128 rows of the weight share a scale.
+constexpr Tile kTilesInput[] = {{256, 256, 256, 1.07f, 0.92f, 3.9f},
+                                {256, 128, 256, 0.80f, 0.83f, 1.1f},
+                                {64, 64, 256, 0.34f, 0.33f, 0.9f}};
 
 // The product of 8-bit rows, cut along k by groups of four steps, two at least.
 Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
@@ -1149,6 +1351,9 @@ Cut cut_product8(uint64_t m, uint64_t n, uint64_t k) {
 // The products of 16-bit rows, in steps of 64.
 Cut cut_product16(uint64_t m, uint64_t cols, uint64_t steps) {
   return cut_product(kTiles16, m, cols, steps, 1, 8);
+}
+Cut cut_input(uint64_t m, uint64_t cols, uint64_t steps, uint32_t shift) {
+  return shift ? cut_product(kTilesInput, m, cols, steps, 1, 8) : cut_product16(m, cols, steps);
 }
 
 template <class T>
@@ -1202,11 +1407,26 @@ int launch_tiles16(const Cut& c, const Rows16& a, uint64_t m, const Held8& b, ui
       (const nz_bf16*)a.data, a.stride, (uint32_t)a.width, a.plane, (uint32_t)m, (const uint8_t*)b.data,            \
       (const uint8_t*)b.scales, b.shift, (uint32_t)b.rows, (uint32_t)b.cols, (uint32_t)steps_1, a.planes,           \
       (uint32_t)cols, (const T*)bias, (T*)y, c.mt, c.nt, c.part_length, p)
+#define NZ_INPUT(TN)                                                                                                \
+  nz_fp8_input_kernel<TN, T><<<grid, 256, 0, st>>>((const nz_bf16*)a.data, a.stride, (uint32_t)m,                   \
+                                                   (const uint8_t*)b.data, (const uint8_t*)b.scales,                \
+                                                   (uint32_t)b.rows, (uint32_t)b.cols, (uint32_t)steps_1, a.planes, \
+                                                   (T*)y, c.mt, c.nt, c.part_length, p)
+      if constexpr (P == kInput) {
+        if (b.shift && c.bm == 256) {
+          if (c.bn == 256)
+            NZ_INPUT(8);
+          else
+            NZ_INPUT(4);
+          return;
+        }
+      }
       if (c.bm == 256)
         NZ_TILES16(4, 2, 4, 4);
       else
         NZ_TILES16(2, 2, 2, 2);
 #undef NZ_TILES16
+#undef NZ_INPUT
     }
   });
   if (p) launch_join<ADD>(p, c, m, cols, bias, y, dtype, st);
@@ -1451,10 +1671,10 @@ int nz_fp8_linear_rows8(const void* dev_x_data, const void* dev_x_scales, uint64
 }
 
 uint64_t nz_fp8_linear_grad_workspace_bytes(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride,
-                                            uint64_t k) {
+                                            uint64_t k, int block_rows) {
   if (m == 0 || n == 0 || k == 0) return 0;
   const Planes p = planes_of(dev_g, dtype, m, n, stride);
-  return p.bytes + cut_product16(m, k, p.padded / 64 * p.count).part_bytes(m, k);
+  return p.bytes + cut_input(m, k, p.padded / 64 * p.count, shift_of(block_rows)).part_bytes(m, k);
 }
 
 int nz_fp8_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uint64_t stride, const void* dev_w_data,
@@ -1468,7 +1688,7 @@ int nz_fp8_linear_grad(const void* dev_g, int dtype, uint64_t m, uint64_t n, uin
   const hipStream_t st = (hipStream_t)stream;
   const Planes p = planes_of(dev_g, dtype, m, n, stride);
   const uint64_t steps = p.padded / 64;
-  const Cut cut = cut_product16(m, k, steps * p.count);
+  const Cut cut = cut_input(m, k, steps * p.count, shift_of(block_rows));
   if (int rc = check_cut(cut)) return rc;
   if (int rc = check_workspace(dev_workspace, workspace_bytes, p.bytes + cut.part_bytes(m, k))) return rc;
   const Rows16 a = launch_planes(dev_g, dtype, m, n, stride, p, dev_workspace, st);

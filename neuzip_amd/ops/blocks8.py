@@ -165,7 +165,7 @@ def _input_gradient(grad: torch.Tensor, weight: FP8Tensor) -> torch.Tensor:
         return dx.zero_()
     rows, m, stride = _as_rows(grad, n)
     args = (rows.data_ptr(), _dtype_code(grad.dtype), m, n, stride)
-    room = _ask(L.nz_fp8_linear_grad_workspace_bytes, index, *args, k)
+    room = _ask(L.nz_fp8_linear_grad_workspace_bytes, index, *args, k, weight.block_rows)
     ws, at = _workspace(room, rows)
     _call(L.nz_fp8_linear_grad, index, *args, weight.data.data_ptr(), weight.scales.data_ptr(), k, weight.block_rows,
           dx.data_ptr(), at, room)

@@ -70,7 +70,7 @@ def test_refusals_of_the_products():
     refused(g(None, 0, 1, 1, 1, P, P, 1, 1, P, P, 1 << 30, None), A, "null gradient")
     refused(g(P, 0, 1, 0, 1, P, P, 1, 1, P, P, 1 << 30, None), A, "without rows")
     refused(g(P, 0, 1, 1 << 22, 1 << 22, P, P, 1, 1, P, P, 1 << 30, None), A, "2^21")
-    need = L.nz_fp8_linear_grad_workspace_bytes(P + 2, 0, 100, 512, 512, 512)
+    need = L.nz_fp8_linear_grad_workspace_bytes(P + 2, 0, 100, 512, 512, 512, 1)
     refused(g(P + 2, 0, 100, 512, 512, P, P, 512, 1, P, P, need - 1, None), D, "workspace")
     assert g(None, 0, 0, 1, 1, None, None, 1, 1, None, None, 0, None) == _lib.OK
 
@@ -114,7 +114,7 @@ def test_sizes_beyond_the_limits_have_an_answer():
     for huge in (1 << 24, 1 << 40, (1 << 63) + 5, (1 << 64) - 1):
         for m, n, k in ((huge, 5, 5), (5, huge, 5), (5, 5, huge), (huge, huge, huge)):
             L.nz_fp8_linear_workspace_bytes(m, n, k, 0), L.nz_fp8_linear_workspace_bytes(m, n, k, 2)
-            L.nz_fp8_linear_grad_workspace_bytes(P, 0, m, n, n, k)
+            L.nz_fp8_linear_grad_workspace_bytes(P, 0, m, n, n, k, 128)
             L.nz_fp8_weight_grad_workspace_bytes(P, 1, m, n, n, k)
 
 

@@ -249,6 +249,23 @@ def test_gradients_of_whole_numbers_are_exact(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n,k", [(4096, 1024, 1030), (2050, 520, 2051), (1000, 6000, 300), (5000, 257, 4100)])
+def test_large_gradients_of_whole_numbers_are_exact(m, n, k, dtype):
+    """the larger tiles, whole and in parts, their ends, and scales of their own in every block"""
+    g, xd = whole_numbers(m, n, 7, 1, dtype).to(DEV), whole_numbers(m, k, 7, 3).to(DEV)
+    up = torch.exp2(torch.arange(n) // 128 % 5 - 2.0).to(DEV)[:, None] * torch.exp2(torch.arange(k) // 128 % 3 - 1.0).to(DEV)
+    wd = whole_numbers(n, k, 7, 2).to(DEV) * up
+    x = xd.to(dtype).requires_grad_(True)
+    want = round_to((g.double() @ wd.double()).cpu(), dtype)
+    for block_rows in (1, 128):
+        y = ops.fp8_linear(x, ops.fp8_quantize(wd, block_rows))
+        same(torch.autograd.grad(y, x, g)[0], want)
+    down = torch.exp2(torch.arange(m) % 5 - 2.0).to(DEV)[:, None]
+    same(ops.fp8_weight_gradient((g / down).to(dtype), ops.fp8_quantize(xd * down)),
+         round_to((g.double().t() @ xd.double()).cpu(), dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("m,n,k", [(40, 300, 200), (333, 257, 130), (700, 128, 1021), (2048, 64, 128)])
 def test_gradients_of_random_values(m, n, k, dtype):
     """Sums in 32 bits over as many products as the type of the gradient has planes of bf16 numbers, and half a step"""
