@@ -162,6 +162,8 @@ def parse_args():
     ap.add_argument("--seq-len", type=int, default=1024)
     ap.add_argument("--verify-steps", type=int, default=10,
                     help="gpt2m: steps of the side-by-side dense / compressed weight comparison")
+    ap.add_argument("--saved-bits", type=int, default=16, choices=[16, 8],
+                    help="gpt2m: 8 measures steps that keep activations in 8 bits for the backward pass, too")
     ap.add_argument("--no-gpt2m", action="store_true",
                     help="skip the GPT-2-medium-shaped training block (BASELINE config 4) of the default line")
     ap.add_argument("--no-llama", action="store_true",
@@ -814,6 +816,16 @@ def gpt2m_measure(args, torch):
     lomo, _, _ = run(1, hooks_only=True)
     for hd in handles:
         hd.remove()
+    saved8 = None
+    if args.saved_bits == 8:
+        saved8 = {}
+        for name in ("16_bits", "8_bits"):
+            torch.cuda.reset_peak_memory_stats()
+            with neuzip_amd.DecompressAhead(mgr, model, ahead=False):
+                m, _, _ = run(per_launch)
+            saved8[name] = {k: m[k] for k in ("ms_per_step", "first_loss", "last_loss")}
+            saved8[name]["peak_mib"] = round(torch.cuda.max_memory_allocated() / 2 ** 20)
+            neuzip_amd.fp8_activations(model)
     mgr._be.check()
     # writes that went into the entries' existing buffers (no allocation, no wait for the size)
     in_place, outgrown = be.rewrite_stats()
@@ -878,6 +890,7 @@ def gpt2m_measure(args, torch):
             "reference_update_hooks_per_linear": lomo_plain,
             "reference_update_hooks_order_learned": lomo,
             "lockstep_check_lossless": lockstep,
+            **({"activations_kept_in": saved8} if saved8 else {}),
             "rewrites": rewrites,
             "compressed_tensors": n_comp,
             "manager": how,

@@ -171,6 +171,7 @@ class GPT2Block(torch.nn.Module):
         self.proj = torch.nn.Linear(d, d)
         self.ln2 = torch.nn.LayerNorm(d)
         self.fc = torch.nn.Linear(d, 4 * d)
+        self.act = torch.nn.GELU()  # a module, which neuzip_amd.fp8_activations replaces
         self.fc2 = torch.nn.Linear(4 * d, d)
         for m in (self.qkv, self.proj, self.fc, self.fc2):
             _init_linear(m)
@@ -180,7 +181,7 @@ class GPT2Block(torch.nn.Module):
         q, k, v = self.qkv(self.ln1(x)).view(B, T, 3, self.heads, D // self.heads).permute(2, 0, 3, 1, 4)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         x = x + self.proj(a.transpose(1, 2).reshape(B, T, D))
-        return x + self.fc2(F.gelu(self.fc(self.ln2(x))))
+        return x + self.fc2(self.act(self.fc(self.ln2(x))))
 
 
 class GPT2Shaped(torch.nn.Module):

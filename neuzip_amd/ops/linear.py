@@ -15,6 +15,7 @@ Behaviour follows the reference's ``CompressedLinear`` (neuzip/ops/linear.py:11-
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from neuzip_amd.ops.blocks8 import FP8Tensor, _saved, _unsaved, fp8_quantize, fp8_weight_gradient
 
@@ -70,6 +71,7 @@ class CompressedLinearHeld8(torch.autograd.Function):
         return _p.linear(x, bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         _p, held, has_bias = ctx.carry
         (held,) = _unsaved(ctx, held)

@@ -206,6 +206,29 @@ def test_product_keeps_nan_where_it_is(m, dtype):
         assert torch.equal(torch.isnan(got), want)
 
 
+@pytest.mark.parametrize("block_rows", (1, 128))
+def test_large_tiles_keep_nan_where_it_is(block_rows):
+    m, n, k = 2500, 2300, 1024
+    x, wd = rnd(m, k, dtype=torch.bfloat16).to(DEV), rnd(n, k, seed=1).to(DEV)
+    x[2049, 5], wd[130, 600] = math.nan, math.inf
+    w = ops.fp8_quantize(wd, block_rows)
+    bad = slice(130, 131) if block_rows == 1 else slice(128, 256)
+    want = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+    want[2049] = True
+    want[:, bad] = True
+    assert torch.equal(torch.isnan(ops.fp8_linear(x, w)), want)
+    g = rnd(m, n, seed=2, dtype=torch.bfloat16).to(DEV)
+    leaf = x.clone().requires_grad_(True)
+    dx = torch.autograd.grad(ops.fp8_linear(leaf, w), leaf, g)[0]
+    want = torch.zeros(m, k, dtype=torch.bool, device=DEV)
+    want[:, 512:640] = True  # the block of columns that the infinity is in
+    assert torch.equal(torch.isnan(dx), want)
+    dw = ops.fp8_weight_gradient(g, ops.fp8_quantize(x))
+    want = torch.zeros(n, k, dtype=torch.bool, device=DEV)
+    want[:, :128] = True
+    assert torch.equal(torch.isnan(dw), want)
+
+
 def test_product_shapes_strides_and_empty():
     wd = whole_numbers(24, 96, 7, 1)
     w = ops.fp8_quantize(wd.to(DEV), 128)

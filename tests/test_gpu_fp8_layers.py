@@ -81,6 +81,24 @@ def test_autocast_and_inputs_without_a_gradient():
         assert not layer(x.bfloat16()).requires_grad
 
 
+def test_one_row_no_rows_and_a_second_derivative():
+    layer, _ = pair(8)
+    x, g = rnd(200), rnd(96, seed=1)
+    layer(x.clone().requires_grad_(True)).backward(g)
+    want = ops.fp8_weight_gradient(g[None], ops.fp8_quantize(x[None]))
+    assert torch.equal(layer.weight._gradient, want)
+    layer.weight._gradient = None
+    a = rnd(0, 200).requires_grad_(True)
+    layer(a).sum().backward()
+    assert a.grad.shape == (0, 200) and not layer.weight._gradient.any()
+    a = rnd(3, 200).requires_grad_(True)
+    w = ops.fp8_quantize(rnd(96, 200, seed=2), 128)
+    for f in (layer, ops.fp8_activation, lambda t: ops.fp8_linear(t, w)):
+        (d,) = torch.autograd.grad(f(a).float().pow(2).sum(), a, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            d.sum().backward()
+
+
 class Block(torch.nn.Module):
     def __init__(self, d=256):
         super().__init__()
