@@ -172,17 +172,18 @@ def _input_gradient(grad: torch.Tensor, weight: FP8Tensor) -> torch.Tensor:
     return dx
 
 
-def _saved(ctx, *held) -> None:
-    """Save what ``held`` tensors in 8 bits consist of.  An inference tensor has no version to check."""
-    if not any(t.data.is_inference() for t in held):
-        ctx.save_for_backward(*(part for t in held for part in (t.data, t.scales)))
+def _saved(ctx, held: FP8Tensor) -> None:
+    """Save what ``held`` consists of.  An inference tensor has no version to check."""
+    if not held.data.is_inference():
+        ctx.save_for_backward(held.data, held.scales)
 
 
-def _unsaved(ctx, *held):
-    """The same again, as hooks of saved tensors hand it back; raises if it has been written to since."""
+def _unsaved(ctx, held: FP8Tensor) -> FP8Tensor:
+    """The same again; raises if it has been written to since.  Hooks of saved tensors may hand back others."""
     parts = ctx.saved_tensors
-    return [FP8Tensor(parts[2 * i], parts[2 * i + 1], t.shape, t.block_rows) if parts else t
-            for i, t in enumerate(held)]
+    if parts and (parts[0] is not held.data or parts[1] is not held.scales):
+        return FP8Tensor(*parts, held.shape, held.block_rows)
+    return held
 
 
 class BlockLinear(torch.autograd.Function):
@@ -202,8 +203,7 @@ class BlockLinear(torch.autograd.Function):
     def backward(ctx, grad_output):
         grad_x = grad_b = None
         if ctx.needs_input_grad[0]:
-            (weight,) = _unsaved(ctx, ctx.weight)
-            grad_x = _input_gradient(grad_output, weight)
+            grad_x = _input_gradient(grad_output, _unsaved(ctx, ctx.weight))
         if ctx.needs_input_grad[2]:
             grad_b = _bias_gradient(grad_output, ctx.weight.shape[0])
         return grad_x, None, grad_b, None
@@ -283,45 +283,67 @@ def fp8_weight_gradient(grad: torch.Tensor, x: FP8Tensor, out=None) -> torch.Ten
     return out
 
 
+@lru_cache(maxsize=1024)
+def _kept_places(rows: int, cols: int, tensors: int):
+    """Where a buffer holds the codes and scales of ``tensors`` (1 or 2) tensors, and its size"""
+    data, scales = (rows * size for size in _row_sizes(cols))
+    first = data * tensors
+    second = first + -(-scales // 16) * 16
+    if tensors == 1:
+        return 0, first, None, None, first + scales
+    return 0, first, data, second, second + scales
+
+
+def _kept_parts(at: int, places):
+    """the addresses of these in a buffer at ``at``: x's codes and scales, up's"""
+    x, x_scales, up, up_scales, _ = places
+    return at + x, at + x_scales, None if up is None else at + up, None if up is None else at + up_scales
+
+
 def _activate(x, kind: int, up, keep: bool):
-    """the result, and ``x`` and ``up`` in 8 bits where they are kept"""
+    """the result, and what is kept of ``x`` and ``up``"""
     code, cols = _dtype_code(x.dtype), x.shape[-1]
     index = _on_gpu(x=x, up=up)
     y = x.new_empty(x.shape)
     rows, n, stride = _as_rows(x, cols)
-    held = [_room_for(x, x.shape, n) for t in (x, up) if t is not None] if keep else []
-    at = [part.data_ptr() for t in held for part in (t.data, t.scales)] + [None] * 4
-    u, u_at, u_stride = None, None, 0
+    u_at, u_stride = None, 0
     if up is not None:
         u, _, u_stride = _as_rows(up, cols)
         u_at = u.data_ptr()
+    kept, parts = None, (None, None, None, None)
+    if keep:
+        places = _kept_places(n, cols, 1 if up is None else 2)
+        kept = x.new_empty(places[4], dtype=torch.uint8)
+        parts = _kept_parts(kept.data_ptr(), places)
     _call(_lib.load().nz_fp8_activation, index, kind, rows.data_ptr(), code, n, cols, stride, u_at, u_stride,
-          y.data_ptr(), *at[:4])
-    return y, held
+          y.data_ptr(), *parts)
+    return y, kept
 
 
 class HeldActivation(torch.autograd.Function):
-    """``f(x)``, or ``f(x) * up``, that keeps ``x`` and ``up`` in 8 bits."""
+    """``f(x)``, or ``f(x) * up``, that keeps ``x`` and ``up`` in 8 bits (in one buffer)."""
 
     @staticmethod
     def forward(ctx, x, kind, up):
-        y, held = _activate(x, kind, up, True)
-        ctx.kind, ctx.shapes = kind, [t.shape for t in held]
-        ctx.save_for_backward(*(part for t in held for part in (t.data, t.scales)))
+        y, kept = _activate(x, kind, up, True)
+        ctx.kind, ctx.tensors = kind, 1 if up is None else 2
+        ctx.save_for_backward(kept)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        parts = ctx.saved_tensors
-        index = _on_gpu(grad=grad_output, x=parts[0])
+        (kept,) = ctx.saved_tensors
+        index = _on_gpu(grad=grad_output, x=kept)
         cols = grad_output.shape[-1]
         rows, n, stride = _as_rows(grad_output, cols)
         dx = grad_output.new_empty(grad_output.shape)
-        dup = torch.empty_like(dx) if len(parts) == 4 else None
-        at = [t.data_ptr() for t in parts] + [None] * 2
+        dup = dup_at = None
+        if ctx.tensors == 2:
+            dup = grad_output.new_empty(grad_output.shape)
+            dup_at = dup.data_ptr()
         _call(_lib.load().nz_fp8_activation_grad, index, ctx.kind, rows.data_ptr(), _dtype_code(grad_output.dtype), n,
-              cols, stride, *at[:4], dx.data_ptr(), dup.data_ptr() if dup is not None else None)
+              cols, stride, *_kept_parts(kept.data_ptr(), _kept_places(n, cols, ctx.tensors)), dx.data_ptr(), dup_at)
         return dx, None, dup
 
 

@@ -74,7 +74,7 @@ class CompressedLinearHeld8(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_output):
         _p, held, has_bias = ctx.carry
-        (held,) = _unsaved(ctx, held)
+        held = _unsaved(ctx, held)
         go2d = _as_rows(grad_output)
         dense_w = _p.shared()
 

@@ -232,7 +232,7 @@ def test_inference_tensors_and_hooks_of_saved_tensors(without_gpu):
     y.sum().backward()
     assert seen == [w.data.shape, w.scales.shape]
     z.sum().backward()
-    assert len(seen) == 6 and up.grad.shape == up.shape
+    assert len(seen) == 3 and up.grad.shape == up.shape
 
 
 def test_writes_into_a_given_gradient_are_seen(without_gpu):
@@ -252,6 +252,8 @@ def test_what_an_activation_function_keeps(without_gpu):
         assert not kept
         ops.fp8_activation(x.requires_grad_(True))
         assert sum(t.numel() * t.element_size() for t in kept) == 3 * (512 + 4)
+        ops.fp8_activation(x, "silu", x.detach())
+        assert sum(t.numel() * t.element_size() for t in kept[1:]) == 2 * 3 * (512 + 4) + 4  # scales begin at 16 bytes
 
 
 def test_the_oracle_itself():
