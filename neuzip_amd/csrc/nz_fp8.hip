@@ -54,7 +54,8 @@ __device__ inline void values_of(uint2 codes, uint32_t s, float (&v)[8]) {
 
 // ---- quantisation and values -----------------------------------------------------------------------------------
 //
-// One wavefront per 512 values of a row: 8 values a lane, 16 lanes a block.
+// One wavefront per 512 values of a row: 8 values a lane, 16 lanes a block.  Memory bounds them: 8192x4096 of bf16 to
+// rows in 8 bits 22 to 24 us (4.3 TB/s), 16384x4096 to values 29.8 (6.8 TB/s, written and read; a fill reaches 6.8).
 
 // Division of the number of a wavefront, below 2^26 in one launch, by the groups of 512 values in a row: n / d is
 // n mul >> shift with mul = floor(2^shift / d) + 1 and 2^shift >= 2^26 d, for then n (mul d - 2^shift) < 2^shift.
@@ -92,7 +93,8 @@ __global__ __launch_bounds__(256) void nz_fp8_quantize_kernel(const T* x, uint64
 }
 
 // A workgroup per block of 128 x 128 values, which stay in registers between the search for the largest and the
-// rounding: 16 lanes a row, 16 rows at a time.
+// rounding: 16 lanes a row, 16 rows at a time.  16384x4096 of bf16: 42.5 us, 4.7 TB/s read and written (a large copy:
+// 5.15).
 template <class T>
 __global__ __launch_bounds__(256) void nz_fp8_quantize_blocks_kernel(const T* x, uint64_t stride, uint64_t rows,
                                                                      uint32_t cols, uint32_t blocks, uint32_t pitch,
@@ -220,6 +222,9 @@ __device__ inline float gate(float x, float& slope) {
 
 // y = f(x), times `up` where GATED; x (and `up`) in 8 bits, where they are to be kept.  A wavefront per 512 values of a
 // row, as above.
+//
+// Instructions bound gelu (8192x4096 of bf16: 35.6 us, 4.7 TB/s, and 37.5 back, 4.5 TB/s), memory silu with
+// a second factor (2048x14336: 42.6 and 39.6 us, 5.5 and 5.9 TB/s; a large copy: 5.15).
 template <int KIND, bool GATED, class T>
 __global__ __launch_bounds__(256) void nz_fp8_activation_kernel(const T* x, uint64_t stride, const T* up,
                                                                 uint64_t up_stride, uint32_t cols, uint32_t waves,
@@ -317,6 +322,10 @@ __device__ inline b8v bf16_of_codes(uint2 codes, uint32_t s) {
 // arrived and that the stage before is used up.  Staged rows are exchanged in chunks of 16 bytes (chunk c of row r at
 // c ^ (r & 7)) so that eight lanes in turn read from all banks, and the weight rows of a wavefront are staged in an
 // order that leaves each lane 4 TN consecutive columns of the result.  Scales are staged once per 512 values.
+//
+// 64 x (4096x14336) in tiles of 64x64 and 4 parts: 12.2 to 13.2 us, the weight at 4.4 to 4.8 TB/s (3.1 more for the rows,
+// 2.2 to 3.9 for the join).  Of larger products 256x256 (below) gives more where k is a multiple of 512; the figures at
+// `kTiles` decide.
 template <int WM, int WN, int TM, int TN, int NS, int EU, class T>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU, EU))) void nz_fp8_tiles_kernel(
     const uint8_t* xd, const uint8_t* xs, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t shift, uint32_t n,
@@ -659,6 +668,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 // are on their way.
 // Results in float32 are summed by bf16 instructions (why, see `step`), for which a lane takes both sides to bf16: of
 // the 128 values of a step those it holds, 8 at a time (both sides in the same order, which is all that counts).
+//
+// What bounds it is memory's way to few lines at a time: one row of 14336x4096 12.8 to 14.4 us (4.1 to 4.6 TB/s of the
+// weight), 7 of 5003x3001 9.7.
 constexpr uint32_t kHeld = 528;  // bytes of 512 values of a row and their scales in LDS
 
 template <int N, class T>
@@ -799,6 +811,11 @@ enum Product { kForward, kInput, kWeight };
 // c ^ (row & 7)); a step ahead, the codes are written to LDS once more as bf16, once for all wavefronts.  Where rows
 // run along the summed axis the tile lies as in memory, and the operand is read by the instruction that transposes
 // 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns.
+//
+// The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 75.5 us, 0.91 PFLOP/s (a library's
+// bf16 product of the same sizes 85), and 7.3 for the join.  LDS bounds it (43 % of the cycles, 11 % conflicts, beside
+// matrix units busy for 45 %): wavefronts of 64x64 read 128 KB a step.  Four wavefronts of 128x64, which read 96, took 82
+// (each waits for itself then); tiles of 256x256 8 % less at 4096x4096, but four parts and so more at 4096x1024.
 template <int WM, int WN, int TM, int TN, Product P, bool ADD, class T>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_fp8_tiles16_kernel(
     const nz_bf16* a, uint64_t a_stride, uint32_t a_width, uint64_t a_plane, uint32_t m, const uint8_t* bd,
@@ -1065,6 +1082,9 @@ __device__ inline void step16_in_place(b8v b, b8v a, f4& acc) {
 // Steps of 64 values in two halves, whose operands are read while the other half's are multiplied.  In the middle is the
 // step's barrier: the next step has arrived and this one has been read, so that the third behind it goes there, two steps
 // ahead of its use.
+//
+// 8192 rows: 4096x1024 in tiles of 256x128 62 to 65 us, 1.08 PFLOP/s (68.5 by the kernel above), 4096x4096 in tiles of
+// 256x256 191 us, 1.43 PFLOP/s (258).
 template <int TN, class T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void nz_fp8_input_kernel(
     const nz_bf16* a, uint64_t a_stride, uint32_t m, const uint8_t* bd, const uint8_t* bs, uint32_t b_rows,
@@ -1434,6 +1454,11 @@ int launch_tiles16(const Cut& c, const Rows16& a, uint64_t m, const Held8& b, ui
 }
 
 // Rows that go to the kernel for few (one tile of the instruction), and those that are brought to 8 bits inside it.
+// The others go to tiles where the weight is large, for those read it in longer runs and their further launches count
+// less.  us, weights from memory, rows as they are, the kernel for few against tiles (of 17 rows): 8x4096x4096 9.9, 12.6;
+// 4x4096x4096 8.1, 12.6; 16x4096x4096 (rows brought to 8 bits before) 9.7, 12.7; 1x4096x14336 15.2, 19.1; 8x14336x4096
+// 18.5, 17.2; 8x50257x4096 51 (rows in 8 bits, two wavefronts for each), 43.3.  Of small k and many rows the few lose
+// up to 2.5 us: 16x4096x1024 6.7, 6.0; 16x14336x2048 12.7, 10.2.
 bool few_inside(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   const uint64_t groups = m * nz_ceil_div(k, kGroup);
   return m <= 16 && groups <= 64 && (groups <= 32 || n * k <= 1ull << 26 || dtype == NZ_DTYPE_F32);
@@ -1446,6 +1471,10 @@ template <int N, class T>
 void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, const void* wd, const void* ws,
                 uint32_t shift, uint64_t n, uint32_t k, const T* bias, T* y, hipStream_t st) {
   const uint32_t groups = (k + kGroup - 1) / kGroup;
+  // As many wavefronts for a row as it has groups for, while there are not enough rows of the weight to fill the card;
+  // beyond that two for many rows of x, else four.  us with 1, 2, 4, 8 of them:
+  // 1x4096x14336 54, 30, 18, 13.4; 7x5003x3001 16.5, 11, 8.8, 10.5; 1x14336x4096 19, 14, 14.5, 14.2; 8x14336x4096 22, 17.5,
+  // 19, 24; 4x128256x1024 22.9, 22.6, 27, 39.
   uint32_t kw = groups >= 8 ? 8 : groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
   const uint64_t t = nz_ceil_div(n, 16);
   const uint32_t cus = nz_compute_units();

@@ -1,4 +1,4 @@
-// What the operators beside the codec (nz_mx.hip, nz_embedding.hip) share.
+// What the operators beside the codec (nz_mx.hip, nz_fp8.hip, nz_embedding.hip) share.
 #pragma once
 
 #include <hip/hip_runtime.h>

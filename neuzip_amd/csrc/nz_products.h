@@ -134,12 +134,12 @@ __device__ inline void tile_of(uint32_t id, uint32_t mt, uint32_t nt, uint32_t& 
   tn = at / high;
 }
 
-// Add the bias (ADD: what y holds) to a workgroup's tile and store it, or store it as it is among the parts.  A lane (r, g) of wavefront
-// (wm, wn) holds rows m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], 4 TN consecutive columns.
+// Store a workgroup's tile in y, plus the bias (ADD: what y holds).  A lane (r, g) of wavefront (wm, wn) holds rows
+// m0 + (wm TM + i) 16 + r and, from acc[i][0] to acc[i][TN - 1], 4 TN consecutive columns.
 //
-// The tile (PARTS_TOO: one of the parts as well) goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold
-// pieces of 16 rows, 8192 x (4096x1024) takes 53 us in tiles of 128x256 instead of 37, 8192 x (14336x4096) 434 instead
-// of 409. (In tiles of 128x128 39 instead of 37 and 462 instead of 466.)
+// It goes through LDS once more, so that a wavefront stores whole lines: straight from the lanes, which hold pieces of
+// 16 rows, 8192 x (4096x1024) takes 53 us in tiles of 128x256 instead of 37, 8192 x (14336x4096) 434 instead of 409. (In
+// tiles of 128x128 39 instead of 37 and 462 instead of 466.)
 template <int WM, int WN, int TM, int TN, int LDS, bool ADD, class T>
 __device__ inline void store_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
                                   const T* bias, T* y) {
@@ -185,6 +185,8 @@ __device__ inline void store_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, u
   }
 }
 
+// The end of a tile: to y as above, or as it is to its place among the parts.  A part goes through LDS too where
+// PARTS_TOO: of the gradient of a weight, two parts of 4096x1024, 75 us instead of 81.5.
 template <int WM, int WN, int TM, int TN, int LDS, bool ADD = false, bool PARTS_TOO = false, class T>
 __device__ inline void finish_tile(f4 (&acc)[TM][TN], uint8_t* lds, uint32_t m, uint32_t n, uint32_t m0, uint32_t n0,
                                    const T* bias, T* y, float* part) {
