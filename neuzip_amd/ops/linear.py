@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from neuzip_amd.ops.blocks8 import FP8Tensor, _saved, _unsaved, fp8_quantize, fp8_weight_gradient
+from neuzip_amd.ops.blocks8 import FP8Tensor, fp8_quantize, fp8_weight_gradient
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -66,21 +66,21 @@ class CompressedLinearHeld8(torch.autograd.Function):
         if torch.is_autocast_enabled():
             x = x.to(torch.get_autocast_gpu_dtype())
         held = fp8_quantize(x)
-        ctx.carry = (_p, held, bias is not None)
-        _saved(ctx, held)
+        ctx.carry = (_p, held.shape, bias is not None)
+        ctx.save_for_backward(held.data, held.scales)  # and held by nothing else: hooks may take them elsewhere
         return _p.linear(x, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        _p, held, has_bias = ctx.carry
-        held = _unsaved(ctx, held)
+        data, scales = ctx.saved_tensors
+        _p, shape, has_bias = ctx.carry
         go2d = _as_rows(grad_output)
         dense_w = _p.shared()
 
-        grad_x = torch.mm(go2d, dense_w).reshape(held.shape).to(ctx._inputs_dtype)
+        grad_x = torch.mm(go2d, dense_w).reshape(shape).to(ctx._inputs_dtype)
         del dense_w
-        held = FP8Tensor._of(held.data, held.scales, (go2d.shape[0], held.shape[-1]), 1)
+        held = FP8Tensor(data, scales, (go2d.shape[0], shape[-1]), 1)
         into = _p._gradient
         if into is None:
             _p._gradient = fp8_weight_gradient(go2d, held)

@@ -263,3 +263,18 @@ def test_compiled_functions_make_the_calls():
     compiled = torch.compile(work, backend="eager")
     for scale in (1.0, 3.0):
         assert torch.equal(compiled(x * scale), work(x * scale))
+
+
+def test_kept_inputs_that_hooks_take_elsewhere_are_not_held():
+    """A hook that moves saved tensors to the host frees their memory until the backward pass."""
+    layer, _ = pair(8, rows=128, cols=4096)
+    x, g = rnd(2048, 4096), rnd(2048, 128, seed=1, scale=1e-2)
+    layer(x.requires_grad_(True)).backward(g)
+    want, layer.weight._gradient = layer.weight._gradient, None
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        y = layer(x)
+    assert torch.cuda.memory_allocated() - before < 2048 * 4096 // 2  # y alone is 2048 * 128 * 2
+    y.backward(g)
+    assert torch.equal(layer.weight._gradient, want)
