@@ -813,9 +813,12 @@ enum Product { kForward, kInput, kWeight };
 // 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns.
 //
 // The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 75.5 us, 0.91 PFLOP/s (a library's
-// bf16 product of the same sizes 85), and 7.3 for the join.  LDS bounds it (43 % of the cycles, 11 % conflicts, beside
-// matrix units busy for 45 %): wavefronts of 64x64 read 128 KB a step.  Four wavefronts of 128x64, which read 96, took 82
-// (each waits for itself then); tiles of 256x256 8 % less at 4096x4096, but four parts and so more at 4096x1024.
+// bf16 product of the same sizes 85), and 7.3 for the join.  Matrix units are busy for 45 % of it, LDS for 43 (11 of
+// conflicts), and the wavefronts wait for a third of their time at the one barrier of a step.  Neither LDS nor memory
+// alone bounds it: without conflicts (rows exchanging halves in every other eight), with half of what is fetched (tiles
+// numbered two high) and with codes read half a step before they are converted it took 74 to 78.  Four wavefronts of
+// 128x64, which read 96 KB of LDS a step instead of 128, took 82 (nothing covers what each waits for); tiles of 256x256 8 %
+// less at 4096x4096, but four parts and so more at 4096x1024.
 template <int WM, int WN, int TM, int TN, Product P, bool ADD, class T>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2, 2))) void nz_fp8_tiles16_kernel(
     const nz_bf16* a, uint64_t a_stride, uint32_t a_width, uint64_t a_plane, uint32_t m, const uint8_t* bd,
