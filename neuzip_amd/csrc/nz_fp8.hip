@@ -1077,8 +1077,8 @@ __device__ inline void step16_in_place(b8v b, b8v a, f4& acc) {
 // The gradient of the rows where 128 rows of the weight share a scale: tiles of 256 x 32 TN, four wavefronts of 128 x
 // 16 TN each, a compute unit's own.
 //
-// What bounds the kernel above is LDS: its wavefronts' tiles of 64x64 read 128 KB a step, and the codes pass it twice
-// more, 40 % of its time in addition to the rows' way in.  Here a wavefront's tile is as large as its registers allow
+// In the kernel above much passes LDS: its wavefronts' tiles of 64x64 read 128 KB a step, and the codes go through it twice
+// more.  Here a wavefront's tile is as large as its registers allow
 // (96 KB a step of 256x128, 128 KB of 256x256), and codes are read as they are, eight of a column by the instruction that
 // transposes 8 x 16 bytes on the way, and converted in the wavefront that multiplies them: a step has one scale.
 //
