@@ -144,11 +144,13 @@ def fp8_activations(module: torch.nn.Module, skip=(), prefix: str = "") -> torch
     """In place: what a training step keeps of activations is kept in 8 bits.  Compressed
     Linear layers (``neuzip_amd.nn.Linear``) get ``saved_bits = 8``; ``nn.GELU`` and
     ``nn.SiLU`` become ``neuzip_amd.nn.FP8Activation``.  Modules whose attribute name
-    contains one of ``skip`` are left as they are, and so is what stands below them:
+    contains one of ``skip`` (names, or one) are left as they are, and so is what stands below them:
     layers that share their input keep one of 16 bits together, but 8 bits each, so for
     three of them (q, k and v) 16 bits are less."""
     from neuzip_amd.nn import FP8Activation, Linear
 
+    if isinstance(skip, str) and skip:
+        skip = (skip,)  # one name, not its letters
     kept = _heads(module, *skip) if skip else set()
 
     def make(m):

@@ -48,3 +48,14 @@ def test_what_keeps_8_bits():
     assert isinstance(model.relu, torch.nn.ReLU) and type(block.dense) is torch.nn.Linear
     neuzip_amd.fp8_activations(model)
     assert block.q.saved_bits == 8 and block.act.kind == "gelu"
+
+
+def test_one_name_to_skip():
+    """a text is one mark, not a mark for each of its letters"""
+    block = Holder(q_proj=nn.Linear(Held(), linear()), o=nn.Linear(Held(), linear()), act=torch.nn.GELU())
+    neuzip_amd.fp8_activations(Holder(block=block), skip="q_proj")
+    assert (block.q_proj.saved_bits, block.o.saved_bits) == (16, 8) and isinstance(block.act, nn.FP8Activation)
+    for nothing in ("", (), None):
+        block = Holder(q_proj=nn.Linear(Held(), linear()))
+        neuzip_amd.fp8_activations(Holder(block=block), skip=nothing)
+        assert block.q_proj.saved_bits == 8
