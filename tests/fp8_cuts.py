@@ -86,16 +86,16 @@ def forward(m, n, k, bits, held=False):
     return cut(ROWS8, m, n, up(k, 512), 4, 2, k % 512 == 0)
 
 
-def planes(bits):
-    """bf16 numbers to a value of a gradient: ``bits`` is "bf16", "fp16" or "fp32" """
-    return {"bf16": 1, "fp16": 2, "fp32": 3}[bits]
+def planes(dtype):
+    """bf16 numbers for a value of a gradient (of "bf16", "fp16" or "fp32")"""
+    return {"bf16": 1, "fp16": 2, "fp32": 3}[dtype]
 
 
-def rows_gradient(m, n, k, bits, block_rows):
+def rows_gradient(m, n, k, dtype, block_rows):
     """(bm, bn, parts) of the gradient of m rows of k values"""
-    return cut(INPUT if block_rows == 128 else ROWS16, m, k, up(n, 64) * planes(bits), 1, 8)
+    return cut(INPUT if block_rows == 128 else ROWS16, m, k, up(n, 64) * planes(dtype), 1, 8)
 
 
-def weight_gradient(m, n, k, bits):
+def weight_gradient(m, n, k, dtype):
     """(bm, bn, parts) of the gradient of n rows of k values"""
-    return cut(ROWS16, n, k, up(m, 64) * planes(bits), 1, 8)
+    return cut(ROWS16, n, k, up(m, 64) * planes(dtype), 1, 8)
