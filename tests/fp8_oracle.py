@@ -90,3 +90,23 @@ def function(kind, x):
         u, du = c * (x + 0.044715 * x ** 3), c * (1 + 3 * 0.044715 * x * x)
     p, rest = torch.sigmoid(u), torch.sigmoid(-u)
     return x * p, p + x * p * rest * du, u.abs()
+
+
+def float32_tolerances(kind, x):
+    """f and f' at ``x`` (float64), and how far float32 results may be off them, where neither the exponential nor the
+    result is below the normal range.  In units of 2^-23, u the magnitude of the exponent:
+
+    silu: the exponential's rounding is put back, so t = exp(-|x|) is off by 1 (the instruction's) and a rounding, 1.5;
+    1 / (1 + t) by 0.75 of that, a rounding and the reciprocal's 1, 2.25; t / (1 + t) by 4.25; times x 4.75.
+    gelu: its square's rounding is put back too, the exponential is off by 2.  t = 1 / (1 + 0.35 |x|) is off by 1.5, which
+    the polynomial r(t) t passes on at most 2.3 times (the most, at 0, is 0.798 / 0.35): 3.5; its own roundings are at most
+    1.5 of it (with t <= 1 the partial sums are at most 2.9 times what it is), its fit 0.3 (3.2e-8), two products 1: 8.3,
+    times x 8.8.  Above zero it is 1 less that: less.
+    gelu_tanh: u itself has three roundings of products and one of a sum, and two of constants, 3 u, which the exponential
+    passes on.
+    f' is p(x) + x p'(x): the second term has the errors of two such factors where the first has one, 8 and for gelu_tanh 3 of
+    x u' beside.  10 u's aside, 13 for gelu_tanh, hold all of these, the last rounding too, of the terms' magnitudes."""
+    f, slope, u = function(kind, x)
+    rel = (13.0 + 3 * u if kind == "gelu_tanh" else torch.full_like(u, 10.0)) * 2.0 ** -23
+    p = torch.where(x == 0, torch.full_like(x, 0.5), f / x)
+    return f, slope, rel * f.abs(), rel * (p.abs() + (slope - p).abs())
