@@ -1,4 +1,4 @@
-"""Random-init decoder models of the shapes BASELINE.json names, for bench.py.
+"""Random-init decoder models of the shapes that bench.py measures.
 
 Only shapes and layer types matter here (all weights are N(0, 0.02) from a
 seed, all inputs uniform random token ids): the benchmark measures the codec

@@ -223,8 +223,8 @@ __device__ inline float gate(float x, float& slope) {
 // y = f(x), times `up` where GATED; x (and `up`) in 8 bits, where they are to be kept.  A wavefront per 512 values of a
 // row, as above.
 //
-// Instructions bound gelu (8192x4096 of bf16: 35.6 us, 4.7 TB/s, and 37.5 back, 4.5 TB/s), memory silu with
-// a second factor (2048x14336: 42.6 and 39.6 us, 5.5 and 5.9 TB/s; a large copy: 5.15).
+// Instructions bound gelu (8192x4096 of bf16: 35.5 to 37 us, 4.5 to 4.7 TB/s, and 37.7 back, 4.5 TB/s), memory silu with
+// a second factor (2048x14336: 43 and 39.6 us, 5.5 and 5.9 TB/s; a large copy: 5.2).
 template <int KIND, bool GATED, class T>
 __global__ __launch_bounds__(256) void nz_fp8_activation_kernel(const T* x, uint64_t stride, const T* up,
                                                                 uint64_t up_stride, uint32_t cols, uint32_t waves,
@@ -323,8 +323,8 @@ __device__ inline b8v bf16_of_codes(uint2 codes, uint32_t s) {
 // c ^ (r & 7)) so that eight lanes in turn read from all banks, and the weight rows of a wavefront are staged in an
 // order that leaves each lane 4 TN consecutive columns of the result.  Scales are staged once per 512 values.
 //
-// 64 x (4096x14336) in tiles of 64x64 and 4 parts: 12.2 to 13.2 us, the weight at 4.4 to 4.8 TB/s (3.1 more for the rows,
-// 2.2 to 3.9 for the join).  Of larger products 256x256 (below) gives more where k is a multiple of 512; the figures at
+// 64 x (4096x14336) in tiles of 64x64 and 4 parts: 12.2 to 13.6 us, the weight at 4.3 to 4.8 TB/s (3.1 more for the rows,
+// 2.2 to 4 for the join).  Of larger products 256x256 (below) gives more where k is a multiple of 512; the figures at
 // `kTiles` decide.
 template <int WM, int WN, int TM, int TN, int NS, int EU, class T>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU, EU))) void nz_fp8_tiles_kernel(
@@ -475,9 +475,11 @@ __device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memor
 // other across tiles: the loads run ahead into the next tile, whose first operands are there when the result has been
 // stored.  It goes through a part of LDS that is each wavefront's own, 16 rows at a time.
 //
-// 8192 x (14336x4096): 363 to 378 us, 2.55 to 2.65 PFLOP/s (the tiles of 128x256 above 520 beside them; a library's
-// 8-bit product of 8192^3 reaches 2.75).  Of that some 50 are the stores of the results, in which all compute units meet
-// seven times; letting them start apart by up to half a tile gained nothing.
+// 8192 x (14336x4096): 360 to 376 us where passes go on without a pause, 2.56 to 2.67 PFLOP/s (a library's 8-bit product
+// of these sizes 321 to 329; k = 4000 in the tiles of 128x256 above 416).  One by itself takes 382 to 384, and of passes
+// that begin behind a pause the first fifty up to 510, while the card settles its clock (the library's first twenty 415).
+// Of that some 50 are the stores of the results, in which all compute units meet seven times; letting them start apart by
+// up to half a tile gained nothing.
 template <class T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void nz_fp8_wide_kernel(
     const uint8_t* xd, const uint8_t* xs, uint32_t m, const uint8_t* wd, const uint8_t* ws, uint32_t shift, uint32_t n,
@@ -669,8 +671,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 // Results in float32 are summed by bf16 instructions (why, see `step`), for which a lane takes both sides to bf16: of
 // the 128 values of a step those it holds, 8 at a time (both sides in the same order, which is all that counts).
 //
-// What bounds it is memory's way to few lines at a time: one row of 14336x4096 12.8 to 14.4 us (4.1 to 4.6 TB/s of the
-// weight), 7 of 5003x3001 9.7.
+// What bounds it is memory's way to few lines at a time: one row of 14336x4096 13.8 to 14.4 us (4.1 to 4.3 TB/s of the
+// weight), 7 of 5003x3001 8.8 to 9.2, launches in a row (in a kernel trace, which adds to short ones, up to 15.3 and 10.6).
 constexpr uint32_t kHeld = 528;  // bytes of 512 values of a row and their scales in LDS
 
 template <int N, class T>
@@ -783,7 +785,11 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
 //
 // What the scaled instruction cannot do: the gradients, one of whose sides is not in 8 bits, and results in float32.
 // What is held in 8 bits is exact in bf16; a gradient of 16 or 32 bits is the sum of two or three bf16 numbers, laid
-// side by side along the summed axis.
+// side by side along the summed axis.  (A float16 gradient does not go to float16 instructions as it is: they would take
+// the codes, but not with their scales, which reach from 2^-127 to 2^125.)
+//
+// 8192 rows, 4096x1024, calls without a pause: the rows' gradient in bf16, float16 and float32 57, 128 and 224 us, the
+// weight's 76, 154 and 226, a float32 result 88.
 
 // What 8 bits of float32 rows stand for, as bf16 numbers, rows filled up to whole steps: the rows' side of a product
 // with a float32 result.
@@ -812,9 +818,9 @@ enum Product { kForward, kInput, kWeight };
 // run along the summed axis the tile lies as in memory, and the operand is read by the instruction that transposes
 // 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns.
 //
-// The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 75.5 us, 0.91 PFLOP/s (a library's
-// bf16 product of the same sizes 85), and 7.3 for the join.  Matrix units are busy for 45 % of it, LDS for 43 (11 of
-// conflicts), and the wavefronts wait for a third of their time at the one barrier of a step.  Neither LDS nor memory
+// The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 75.5 to 79 us, 0.87 to 0.91 PFLOP/s
+// (a library's bf16 product of the same sizes 85), and 7.3 for the join.  Matrix units are busy for 45 % of it, LDS for 43
+// (11 of conflicts), and the wavefronts wait for a third of their time at the one barrier of a step.  Neither LDS nor memory
 // alone bounds it: without conflicts (rows exchanging halves in every other eight), with half of what is fetched (tiles
 // numbered two high) and with codes read half a step before they are converted it took 74 to 78.  Four wavefronts of
 // 128x64, which read 96 KB of LDS a step instead of 128, took 82 (nothing covers what each waits for); tiles of 256x256 8 %
@@ -1458,10 +1464,10 @@ int launch_tiles16(const Cut& c, const Rows16& a, uint64_t m, const Held8& b, ui
 
 // Rows that go to the kernel for few (one tile of the instruction), and those that are brought to 8 bits inside it.
 // The others go to tiles where the weight is large, for those read it in longer runs and their further launches count
-// less.  us, weights from memory, rows as they are, the kernel for few against tiles (of 17 rows): 8x4096x4096 9.9, 12.6;
-// 4x4096x4096 8.1, 12.6; 16x4096x4096 (rows brought to 8 bits before) 9.7, 12.7; 1x4096x14336 15.2, 19.1; 8x14336x4096
-// 18.5, 17.2; 8x50257x4096 51 (rows in 8 bits, two wavefronts for each), 43.3.  Of small k and many rows the few lose
-// up to 2.5 us: 16x4096x1024 6.7, 6.0; 16x14336x2048 12.7, 10.2.
+// less.  us a call in a captured graph, weights from memory, rows as they are, the kernel for few against tiles (of 17
+// rows): 8x4096x4096 9.9, 12.6; 4x4096x4096 8.1, 12.6; 16x4096x4096 (rows brought to 8 bits before) 9.7, 12.7;
+// 1x4096x14336 15.2, 19.1; 8x14336x4096 18.5, 17.2; 8x50257x4096 51 (rows in 8 bits, two wavefronts for each), 43.3.  Of
+// small k and many rows the few lose up to 2.5 us: 16x4096x1024 6.7, 6.0; 16x14336x2048 12.7, 10.2.
 bool few_inside(uint64_t m, uint64_t n, uint64_t k, int dtype) {
   const uint64_t groups = m * nz_ceil_div(k, kGroup);
   return m <= 16 && groups <= 64 && (groups <= 32 || n * k <= 1ull << 26 || dtype == NZ_DTYPE_F32);
@@ -1475,9 +1481,9 @@ void launch_few(const void* x, uint64_t stride, const void* xs, uint64_t m, cons
                 uint32_t shift, uint64_t n, uint32_t k, const T* bias, T* y, hipStream_t st) {
   const uint32_t groups = (k + kGroup - 1) / kGroup;
   // As many wavefronts for a row as it has groups for, while there are not enough rows of the weight to fill the card;
-  // beyond that two for many rows of x, else four.  us with 1, 2, 4, 8 of them:
-  // 1x4096x14336 54, 30, 18, 13.4; 7x5003x3001 16.5, 11, 8.8, 10.5; 1x14336x4096 19, 14, 14.5, 14.2; 8x14336x4096 22, 17.5,
-  // 19, 24; 4x128256x1024 22.9, 22.6, 27, 39.
+  // beyond that two for many rows of x, else four.  us with 1, 2, 4, 8 of them, launches in a row, weights from memory:
+  // 1x4096x14336 54, 30, 18, 13.4; 7x5003x3001 16.6, 11.3, 8.8, 10.6; 1x14336x4096 18.9, 14.0, 14.4, 14.2; 8x14336x4096
+  // 22.5, 17.6, 18.7, 23.7; 4x128256x1024 23.0, 22.8, 27.3, 38.6.
   uint32_t kw = groups >= 8 ? 8 : groups >= 4 ? 4 : groups >= 2 ? 2 : 1;
   const uint64_t t = nz_ceil_div(n, 16);
   const uint32_t cus = nz_compute_units();

@@ -221,7 +221,8 @@ def fp8_linear(x, weight: FP8Tensor, bias=None, dtype=None) -> torch.Tensor:
     A bfloat16 or float16 result may lack, of each product, what lies below 2^-12 of the
     largest of the eight consecutive products that it is added with: usually far
     below its own rounding, but not where large products cancel.  A float32 result is
-    summed in 32 bits throughout."""
+    summed in 32 bits throughout; rows of any type have one by
+    ``fp8_linear(fp8_quantize(x), weight, dtype=torch.float32)``."""
     if not isinstance(weight, FP8Tensor) or len(weight.shape) != 2:
         raise ValueError("weight must be a matrix in 8 bits (fp8_quantize)")
     n, k = weight.shape

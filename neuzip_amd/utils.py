@@ -146,7 +146,10 @@ def fp8_activations(module: torch.nn.Module, skip=(), prefix: str = "") -> torch
     ``nn.SiLU`` become ``neuzip_amd.nn.FP8Activation``.  Modules whose attribute name
     contains one of ``skip`` (names, or one) are left as they are, and so is what stands below them:
     layers that share their input keep one of 16 bits together, but 8 bits each, so for
-    three of them (q, k and v) 16 bits are less."""
+    three of them (q, k and v) 16 bits are less.
+
+    A product ``silu(gate) * up`` is no module: its factors are kept as they were, until
+    the block calls ``ops.fp8_activation(gate, "silu", up)`` itself."""
     from neuzip_amd.nn import FP8Activation, Linear
 
     if isinstance(skip, str) and skip:
