@@ -18,11 +18,22 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from neuzip_amd.ops.blocks8 import FP8Tensor, fp8_quantize, fp8_weight_gradient
+from neuzip_amd.ops.microscaled import _DTYPES, _bias_gradient
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
     """Collapse all leading dimensions: [..., k] -> [m, k]."""
     return t.reshape(-1, t.shape[-1])
+
+
+def _column_sums(rows: torch.Tensor) -> torch.Tensor:
+    """The gradient of a bias.  A library's sum over many rows clears its counters with a node
+    that the replays of a captured graph do not keep to, so there it is the kernel of the
+    microscaled layers (like the library's in 32 bits and rounded once, in another order)."""
+    if (rows.is_cuda and torch.cuda.is_current_stream_capturing() and rows.dtype in _DTYPES
+            and not (torch.is_grad_enabled() and rows.requires_grad)):
+        return _bias_gradient(rows, rows.shape[1])
+    return rows.sum(0)
 
 
 class CompressedLinear(torch.autograd.Function):
@@ -54,7 +65,7 @@ class CompressedLinear(torch.autograd.Function):
         else:
             _p._gradient.add_(grad_w)
 
-        grad_b = go2d.sum(0) if bias is not None else None
+        grad_b = _column_sums(go2d) if bias is not None else None
         return grad_x, torch.empty_like(_p.data), grad_b
 
 
@@ -89,5 +100,5 @@ class CompressedLinearHeld8(torch.autograd.Function):
         else:
             into.add_(fp8_weight_gradient(go2d, held))
 
-        grad_b = go2d.sum(0) if has_bias else None
+        grad_b = _column_sums(go2d) if has_bias else None
         return grad_x, torch.empty_like(_p.data), grad_b
