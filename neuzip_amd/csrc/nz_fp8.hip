@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256) void nz_fp8_activation_grad_kernel(const T* g,
     float slope;
     const float f = gate<KIND, std::is_same<T, float>::value, true>(v[i], slope);
     if constexpr (GATED) {
-      a[i] = d[i] * u[i] * slope;
+      a[i] = d[i] * slope * u[i];  // d u may overflow where the slope is zero
       b[i] = d[i] * (v[i] * f);
     } else {
       a[i] = d[i] * slope;

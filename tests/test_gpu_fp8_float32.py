@@ -43,3 +43,23 @@ def test_float32_results_and_gradients(kind, gated):
     near(got[0], g64 * u8 * slope, slope_tol * (g64 * u8).abs())
     if gated:
         near(got[1], g64 * f8, f8_tol * g64.abs())
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32), ids=("bf16", "fp32"))
+@pytest.mark.parametrize("kind", FAR)
+def test_factors_whose_product_would_overflow(kind, dtype):
+    """The slope is zero far below, however large g up is; and a small g stands beside a slope above 1 and a large factor"""
+    big = 3e38
+    x = torch.tensor([-1e4, 2.25, -1e4, 2.25], dtype=dtype)[:, None].expand(4, 128).contiguous()
+    up = torch.tensor([-big, -big, big, big], dtype=dtype)[:, None].expand(4, 128).contiguous()
+    g = torch.tensor([4.0, 0.125, -1000.0, 0.5], dtype=dtype)[:, None].expand(4, 128).contiguous()
+    a, b = x.to(DEV).requires_grad_(True), up.to(DEV).requires_grad_(True)
+    y = ops.fp8_activation(a, kind, b)
+    da, db = (t.cpu().double() for t in torch.autograd.grad(y, (a, b), g.to(DEV)))
+    assert (da[[0, 2]] == 0).all() and (db[[0, 2]] == 0).all() and (y.detach()[[0, 2]] == 0).all()
+    _, slope, _, tol = float32_tolerances(kind, torch.tensor(2.25, dtype=torch.float64))
+    assert slope > 1
+    want = g[[1, 3]].double() * held(up[[1, 3]]) * slope
+    half = torch.finfo(dtype).eps / 2
+    # 16-bit formulas are off by up to 2^-19 more (their exponent's rounding is below 2^-22 of it here)
+    assert ((da[[1, 3]] - want).abs() <= (half + tol / slope + 2.0 ** -19) * want.abs()).all()
