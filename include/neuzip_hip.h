@@ -526,6 +526,11 @@ int nz_embedding_gradient(const void* dev_indices, uint64_t count, const void* d
  * smallest, not below 0, with which its largest magnitude is at most 448 X; a
  * value v is held as v / X rounded to an e4m3 number, to the nearest, ties to the
  * even code.  A block with a NaN or an infinity has s = 255 and reads as NaN.
+ * Magnitudes from 31/32 of 2^128 on (the lowest value of bfloat16 and float32
+ * among them) are held as 2^128, which no 32 bits hold: nz_fp8_dequantize gives an
+ * infinity for it, and sums in 32 bits and gradients of activation functions take
+ * it for the largest bfloat16 number, so that a zero beside it counts for zero.  (As
+ * a weight it is an infinity in sums in 32 bits.)
  * Data: rows of nz_fp8_row_bytes(cols), values in order, filled up to 128 values
  * with zeros.  Scales: a row of nz_fp8_scale_bytes(cols) for each row (or 128
  * rows), one byte s per block in order, filled up to 4 bytes with zeros.  Both are

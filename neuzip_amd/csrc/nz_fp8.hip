@@ -42,7 +42,29 @@ __device__ inline uint32_t block_scale(float (&v)[8]) {
   return s;
 }
 
-// Values of 8 codes.  The conversion takes the exponent field of its scale: a scale byte there is what it means.
+// With the largest scale byte that finite values have, what is 31/32 of 2^128 or more is held as 256 times 2^120.  No 32
+// bits hold that; where it goes into sums (and would make infinity times zero of a masked place) it counts as the largest
+// bf16 number.  (The look for that byte costs the gradient of a weight 1 to 2 %, one row of 14336x4096 in float32 0.6 of
+// 16.6 us.)
+constexpr uint32_t kTopScale = 247;
+__device__ inline void below_infinity(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(v[i]);
+    if ((u & 0x7FFFFFFFu) == 0x7F800000u) v[i] = __uint_as_float(u - 0x10000u);
+  }
+}
+__device__ inline void below_infinity(b8v& v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t u = __builtin_bit_cast(uint16_t, (nz_bf16)v[i]);
+    if ((u & 0x7FFF) == 0x7F80) v[i] = __builtin_bit_cast(nz_bf16, (uint16_t)(u - 1));
+  }
+}
+
+// Values of 8 codes, 2^128 as it is (infinity) or, FINITE, as above.  The conversion takes the exponent field of its
+// scale: a scale byte there is what it means.
+template <bool FINITE = true>
 __device__ inline void values_of(uint2 codes, uint32_t s, float (&v)[8]) {
   const float scale = __uint_as_float(s << 23);
   const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.x, scale, false);
@@ -50,6 +72,7 @@ __device__ inline void values_of(uint2 codes, uint32_t s, float (&v)[8]) {
   const f2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.y, scale, false);
   const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes.y, scale, true);
   v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+  if (FINITE && s == kTopScale) below_infinity(v);
 }
 
 // ---- quantisation and values -----------------------------------------------------------------------------------
@@ -142,7 +165,7 @@ __global__ __launch_bounds__(256) void nz_fp8_quantize_blocks_kernel(const T* x,
   if (across + 1 == blocks && threadIdx.x > 0 && across + threadIdx.x < pitch) to[threadIdx.x] = 0;
 }
 
-template <class T>
+template <bool FINITE, class T>
 __global__ __launch_bounds__(256) void nz_fp8_values_kernel(const uint8_t* data, const uint8_t* scales, uint32_t shift,
                                                             uint64_t first, uint32_t cols, uint32_t waves,
                                                             Groups groups, T* out) {
@@ -154,8 +177,8 @@ __global__ __launch_bounds__(256) void nz_fp8_values_kernel(const uint8_t* data,
   if (at >= cols) return;
   const uint32_t filled = (cols + kStep - 1) / kStep * kStep;
   float v[8];
-  values_of(*reinterpret_cast<const uint2*>(data + row * filled + at),
-            scales[(row >> shift) * (groups.count * 4ull) + at / kStep], v);
+  values_of<FINITE>(*reinterpret_cast<const uint2*>(data + row * filled + at),
+                    scales[(row >> shift) * (groups.count * 4ull) + at / kStep], v);
   store8_upto(out + row * cols + at, cols - at, v);
 }
 
@@ -305,7 +328,7 @@ __device__ inline f4 step(i4v w0, i4v w1, i4v x0, i4v x1, f4 acc, uint32_t sw, u
   }
 }
 
-// 8 codes as bf16 numbers, by such a conversion too.
+// 8 codes as bf16 numbers, by such a conversion too (2^128 as infinity: below_infinity).
 __device__ inline b8v bf16_of_codes(uint2 codes, uint32_t s) {
   const float scale = __uint_as_float(s << 23);
   const b2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes.x, scale, false);
@@ -746,7 +769,9 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
         for (int q = 0; q < 4; ++q) {
           const i4v xq = q < 2 ? x0 : x1, wq = h.w[i][q / 2];
           const uint2 xc = make_uint2(xq[q % 2 * 2], xq[q % 2 * 2 + 1]), wc = make_uint2(wq[q % 2 * 2], wq[q % 2 * 2 + 1]);
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(wc, sw), bf16_of_codes(xc, s), acc, 0, 0, 0);
+          b8v xv = bf16_of_codes(xc, s);
+          if (s == kTopScale) below_infinity(xv);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf16_of_codes(wc, sw), xv, acc, 0, 0, 0);
         }
       } else {
         acc = step(h.w[i][0], h.w[i][1], x0, x1, acc, h.s, sx, i);
@@ -935,10 +960,11 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2,
   const auto convert = [&](uint32_t buf, uint32_t half) {
     const uint4 codes = *(const uint4*)(lds + c_at + buf * CB);
     const uint32_t scale = lds[s_at + buf * SB + (ROWS ? n0 / kStep & 3 : c_step / 2 & 3)];
-    *(b8v*)(lds + to[0] + half * BB) =
-        bf16_of_codes(swap ? make_uint2(codes.y, codes.x) : make_uint2(codes.x, codes.y), scale);
-    *(b8v*)(lds + to[1] + half * BB) =
-        bf16_of_codes(swap ? make_uint2(codes.w, codes.z) : make_uint2(codes.z, codes.w), scale);
+    b8v first = bf16_of_codes(swap ? make_uint2(codes.y, codes.x) : make_uint2(codes.x, codes.y), scale);
+    b8v second = bf16_of_codes(swap ? make_uint2(codes.w, codes.z) : make_uint2(codes.z, codes.w), scale);
+    if (TURN && scale == kTopScale) below_infinity(first), below_infinity(second);  // rows; else a weight
+    *(b8v*)(lds + to[0] + half * BB) = first;
+    *(b8v*)(lds + to[1] + half * BB) = second;
     c_step = c_step + 1 == steps_1 ? 0 : c_step + 1;
   };
   // TURN: rows of A that a plane's last step has once more count as zeros.
@@ -1342,16 +1368,14 @@ int launch_quantize(const void* x, int dtype, uint64_t rows, uint32_t cols, uint
   return nz_launched();
 }
 
-int launch_values(const void* data, const void* scales, uint32_t shift, uint64_t rows, uint64_t cols, void* out,
-                  int dtype, hipStream_t st) {
+template <bool FINITE, class T>
+int launch_values(const void* data, const void* scales, uint32_t shift, uint64_t rows, uint64_t cols, T* out,
+                  hipStream_t st) {
   const Groups groups = groups_of(cols);
   nz_in_pieces(rows, groups.count * 64ull, [&](uint64_t first, uint64_t count) {
     const uint32_t waves = (uint32_t)(count * groups.count);
-    by_dtype(dtype, [&](auto t) {
-      using T = decltype(t);
-      nz_fp8_values_kernel<T><<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
-          (const uint8_t*)data, (const uint8_t*)scales, shift, first, (uint32_t)cols, waves, groups, (T*)out);
-    });
+    nz_fp8_values_kernel<FINITE><<<(uint32_t)nz_ceil_div(waves, 4), 256, 0, st>>>(
+        (const uint8_t*)data, (const uint8_t*)scales, shift, first, (uint32_t)cols, waves, groups, out);
   });
   return nz_launched();
 }
@@ -1539,7 +1563,7 @@ int launch_product(const void* xd, const void* xs, uint64_t m, const Held8& w, c
     return nz_launched();
   }
   if (dtype == NZ_DTYPE_F32) {
-    if (int rc = launch_values(xd, xs, 0, m, filled(k), workspace + room.values, NZ_DTYPE_BF16, st)) return rc;
+    if (int rc = launch_values<true>(xd, xs, 0, m, filled(k), (nz_bf16*)(workspace + room.values), st)) return rc;
     return launch_wide(m, w, bias, y, room, workspace, st);
   }
   const Cut& c = room.cut;
@@ -1640,7 +1664,12 @@ int nz_fp8_dequantize(const void* dev_data, const void* dev_scales, uint64_t row
   if (int rc = check_rows(rows, cols)) return rc;
   if (!dev_out) return nz_fail(NZ_ERR_ARG, "null output");
   if (int rc = check_fp8(dev_data, dev_scales)) return rc;
-  return launch_values(dev_data, dev_scales, shift_of(block_rows), rows, cols, dev_out, dtype, (hipStream_t)stream);
+  int rc = NZ_OK;
+  by_dtype(dtype, [&](auto t) {
+    rc = launch_values<false>(dev_data, dev_scales, shift_of(block_rows), rows, cols, (decltype(t)*)dev_out,
+                              (hipStream_t)stream);
+  });
+  return rc;
 }
 
 uint64_t nz_fp8_linear_workspace_bytes(uint64_t m, uint64_t n, uint64_t k, int dtype) {

@@ -84,7 +84,8 @@ class FP8Tensor:
         return FP8Tensor(self.data.to(device), self.scales.to(device), self.shape, self.block_rows)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values as a dense tensor (bfloat16 holds all of them without rounding, subnormals aside)."""
+        """The values as a dense tensor (bfloat16 holds all of them without rounding, subnormals aside, and an infinity
+        for 2^128, as which magnitudes above 3.29e38 are held)."""
         code = _dtype_code(dtype)
         data = self.data
         index = _on_gpu(data=data)
