@@ -246,8 +246,8 @@ __device__ inline float gate(float x, float& slope) {
 // y = f(x), times `up` where GATED; x (and `up`) in 8 bits, where they are to be kept.  A wavefront per 512 values of a
 // row, as above.
 //
-// Instructions bound gelu (8192x4096 of bf16: 35.5 to 37 us, 4.5 to 4.7 TB/s, and 37.7 back, 4.5 TB/s), memory silu with
-// a second factor (2048x14336: 43 and 39.6 us, 5.5 and 5.9 TB/s; a large copy: 5.2).
+// Instructions bound gelu (8192x4096 of bf16: 35.5 to 37 us, 4.5 to 4.7 TB/s, and 35.4 to 37.7 back), memory silu with
+// a second factor (2048x14336: 43 and 39.7 us, 5.5 and 5.9 TB/s; a large copy: 5.2).
 template <int KIND, bool GATED, class T>
 __global__ __launch_bounds__(256) void nz_fp8_activation_kernel(const T* x, uint64_t stride, const T* up,
                                                                 uint64_t up_stride, uint32_t cols, uint32_t waves,
@@ -290,8 +290,13 @@ __global__ __launch_bounds__(256) void nz_fp8_activation_grad_kernel(const T* g,
   const uint64_t code = row * filled + at, scale = row * (groups.count * 4ull) + at / kStep;
   float v[8], u[8], d[8], a[8], b[8];
   load8_upto(g + row * stride + at, n, d);
-  values_of(*reinterpret_cast<const uint2*>(x_data + code), x_scales[scale], v);
-  if constexpr (GATED) values_of(*reinterpret_cast<const uint2*>(up_data + code), up_scales[scale], u);
+  const uint32_t sx = x_scales[scale], su = GATED ? up_scales[scale] : 0;
+  values_of<false>(*reinterpret_cast<const uint2*>(x_data + code), sx, v);
+  if constexpr (GATED) values_of<false>(*reinterpret_cast<const uint2*>(up_data + code), su, u);
+  if (sx == kTopScale || su == kTopScale) {  // (one look for both)
+    below_infinity(v);
+    if constexpr (GATED) below_infinity(u);
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float slope;
@@ -499,7 +504,7 @@ __device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memor
 // stored.  It goes through a part of LDS that is each wavefront's own, 16 rows at a time.
 //
 // 8192 x (14336x4096): 360 to 376 us where passes go on without a pause, 2.56 to 2.67 PFLOP/s (a library's 8-bit product
-// of these sizes 321 to 329; k = 4000 in the tiles of 128x256 above 416).  One by itself takes 382 to 384, and of passes
+// of these sizes 315 to 329; k = 4000 in the tiles of 128x256 above 416).  One by itself takes 374 to 384, and of passes
 // that begin behind a pause the first fifty up to 510, while the card settles its clock (the library's first twenty 415).
 // Of that some 50 are the stores of the results, in which all compute units meet seven times; letting them start apart by
 // up to half a tile gained nothing.
@@ -813,8 +818,8 @@ __global__ __launch_bounds__(512) void nz_fp8_few_kernel(const void* x, uint64_t
 // side by side along the summed axis.  (A float16 gradient does not go to float16 instructions as it is: they would take
 // the codes, but not with their scales, which reach from 2^-127 to 2^125.)
 //
-// 8192 rows, 4096x1024, calls without a pause: the rows' gradient in bf16, float16 and float32 57, 128 and 224 us, the
-// weight's 76, 154 and 226, a float32 result 88.
+// 8192 rows, 4096x1024, calls without a pause: the rows' gradient in bf16, float16 and float32 57 to 60, 130 and 224 us,
+// the weight's 76 to 78, 157 and 233, a float32 result 90.
 
 // What 8 bits of float32 rows stand for, as bf16 numbers, rows filled up to whole steps: the rows' side of a product
 // with a float32 result.
@@ -843,7 +848,7 @@ enum Product { kForward, kInput, kWeight };
 // run along the summed axis the tile lies as in memory, and the operand is read by the instruction that transposes
 // 4 x 16 values on the way.  A lane ends with 4 TN consecutive columns.
 //
-// The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 75.5 to 79 us, 0.87 to 0.91 PFLOP/s
+// The gradient of a 4096x1024 weight from 8192 rows, tiles of 256x128 in two parts: 76.5 to 80 us, 0.86 to 0.90 PFLOP/s
 // (a library's bf16 product of the same sizes 85), and 7.3 for the join.  Matrix units are busy for 45 % of it, LDS for 43
 // (11 of conflicts), and the wavefronts wait for a third of their time at the one barrier of a step.  Neither LDS nor memory
 // alone bounds it: without conflicts (rows exchanging halves in every other eight), with half of what is fetched (tiles
